@@ -347,6 +347,98 @@ WKV_API int wkv_set_debug_pipeline(long long wait_limit_cycles, int withhold_fir
 
 
 /*
+ * Short causal convolution of every channel with its own W <= 4 taps (no reference
+ * counterpart; next to the recurrences it feeds a selective scan):
+ *   u[b][t][c] = bias[c] + sum_j weight[c][j] x[b][t - W + 1 + j][c],
+ *   y = silu ? u * sigmoid(u) : u
+ * x is [B, T, C] with unit channel stride and the given strides (in elements) of b
+ * and t; y, grad_x and the windows are contiguous. weight is float32 [C, W], bias
+ * float32 [C] or null. window_in [B, W-1, C] holds the rows before t = 0 (null:
+ * zeros), window_out receives the last W - 1 rows (null: not wanted). lengths [B]
+ * (int32, null: all T): the rows past a sequence's length are not read, their y and
+ * grad_x are zero, and window_out holds the last rows inside the length.
+ * The backward takes what the forward took and writes every gradient that is asked
+ * for (grad_bias, grad_window may be null); the parameters' sums have a fixed order.
+ * causal_conv_step is one token, x [B, C]: y from the window and x, and the window
+ * moved on by x in place.
+ */
+WKV_API int causal_conv_forward(int dtype, const void* x, const float* weight, const float* bias, const void* window_in,
+                        const int* lengths, void* y, void* window_out, int64_t B, int64_t T, int64_t C, int W,
+                        int64_t x_stride_b, int64_t x_stride_t, int silu, void* stream);
+WKV_API size_t causal_conv_workspace_size(int64_t B, int64_t T, int64_t C, int W);
+WKV_API int causal_conv_backward(int dtype, const void* grad_y, const void* x, const float* weight, const float* bias,
+                         const void* window_in, const int* lengths, void* grad_x, float* grad_weight,
+                         float* grad_bias, void* grad_window, void* workspace, size_t workspace_bytes, int64_t B,
+                         int64_t T, int64_t C, int W, int64_t g_stride_b, int64_t g_stride_t, int64_t x_stride_b,
+                         int64_t x_stride_t, int silu, void* stream);
+WKV_API int causal_conv_step(int dtype, const void* x, const float* weight, const float* bias, void* window, void* y,
+                     int64_t B, int64_t C, int W, int64_t x_stride_b, int silu, void* stream);
+
+/*
+ * Selective state-space scan (no reference counterpart). Per sequence, channel c
+ * and state n < N (N <= 64), float32, with d = softplus(dt + dt_bias[c]) (softplus
+ * = 0: d = dt + dt_bias[c]):
+ *   h_t = exp(d_t A[c][n]) h_{t-1} + d_t B_t[n] x_t,
+ *   out_t = (sum_n C_t[n] h_t + D[c] x_t) * silu(z_t)
+ * x, dt, z are [B, T, C] and B, C [B, T, N], of the I/O dtype, with unit stride of
+ * the last index and the given strides (in elements) of b and t; out and the
+ * gradients are contiguous. A [C, N], D [C], dt_bias [C] and the states [B, C, N]
+ * are float32; D, z, dt_bias, state_in, lengths and state_out may be null. A row
+ * past its sequence's length is not read, leaves the state as it is and gives zeros.
+ * kept (selective_scan_state_size bytes, or null): the states that the backward
+ * starts from, written by the forward. The sums over sequences and channels have a
+ * fixed order. selective_scan_step is one token (x, dt, z [B, C]; B, C [B, N]) that
+ * updates the state in place.
+ */
+WKV_API size_t selective_scan_state_size(int64_t B, int64_t T, int64_t C, int64_t N);
+WKV_API size_t selective_scan_forward_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int64_t N);
+WKV_API int selective_scan_forward(int dtype, const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+                           const float* D, const void* z, const float* dt_bias, const float* state_in,
+                           const int* lengths, void* out, float* state_out, float* kept, size_t kept_bytes,
+                           void* workspace, size_t workspace_bytes, int64_t B, int64_t T, int64_t C, int64_t N,
+                           int64_t x_sb, int64_t x_st, int64_t dt_sb, int64_t dt_st, int64_t b_sb, int64_t b_st,
+                           int64_t c_sb, int64_t c_st, int64_t z_sb, int64_t z_st, int softplus, void* stream);
+WKV_API size_t selective_scan_backward_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int64_t N);
+WKV_API int selective_scan_backward(int dtype, const void* grad_out, const void* x, const void* dt, const float* A,
+                            const void* Bm, const void* Cm, const float* D, const void* z, const float* dt_bias,
+                            const float* kept, const int* lengths, const float* grad_state_out, void* grad_x,
+                            void* grad_dt, float* grad_A, void* grad_B, void* grad_C, float* grad_D, void* grad_z,
+                            float* grad_dt_bias, float* grad_state_in, void* workspace, size_t workspace_bytes,
+                            int64_t B, int64_t T, int64_t C, int64_t N, int64_t g_sb, int64_t g_st, int64_t x_sb,
+                            int64_t x_st, int64_t dt_sb, int64_t dt_st, int64_t b_sb, int64_t b_st, int64_t c_sb,
+                            int64_t c_st, int64_t z_sb, int64_t z_st, int softplus, void* stream);
+WKV_API int selective_scan_step(int dtype, const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+                        float* state, const float* D, const void* z, const float* dt_bias, void* out, int64_t B,
+                        int64_t C, int64_t N, int64_t x_sb, int64_t dt_sb, int64_t b_sb, int64_t c_sb, int64_t z_sb,
+                        int softplus, void* stream);
+
+/*
+ * Layer norm of rows [rows, C] (C <= 16384) with unit channel stride: y and grad_x
+ * contiguous in the I/O dtype, weight and bias float32 [C] or null, mean and rstd
+ * float32 [rows] from the forward for the backward. Biased variance; grad_weight and
+ * grad_bias (float32 [C], or null) are summed over the rows in a fixed order.
+ */
+WKV_API int layer_norm_forward(int dtype, const void* x, const float* weight, const float* bias, void* y, float* mean,
+                       float* rstd, int64_t rows, int64_t C, int64_t x_stride, float eps, void* stream);
+WKV_API size_t layer_norm_workspace_size(int dtype, int64_t rows, int64_t C);
+WKV_API int layer_norm_backward(int dtype, const void* grad_y, const void* x, const float* weight, const float* mean,
+                        const float* rstd, void* grad_x, float* grad_weight, float* grad_bias, void* workspace,
+                        size_t workspace_bytes, int64_t rows, int64_t C, int64_t g_stride, int64_t x_stride,
+                        void* stream);
+
+/*
+ * y[m][n] = bias[n] + sum_k x[m][k] scales[n][k / group] (q[n][k] - zeros[n][k / group]):
+ * 4-bit weights for a few tokens. packed has rows of ceil(K / 32) * 16 bytes, weight k
+ * in byte k / 2, even k in the low nibble (what lies past K is ignored). scales is
+ * bfloat16 and zeros uint8 (0..15; null: 8), both [N, ceil(K / group)], group a
+ * multiple of 32; bias float32 [N] or null. x [M, K] has unit stride of k; y is
+ * contiguous [M, N] of the same dtype. float32 sums.
+ */
+WKV_API int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scales, const uint8_t* zeros,
+              const float* bias, void* y, int64_t M, int64_t N, int64_t K, int64_t group, int64_t x_stride,
+              void* stream);
+
+/*
  * Launch accounting and per-kernel device timing (no reference counterpart; the
  * benchmark uses them for its launch count and roofline figures).
  * Kernel kinds 0 .. wkv_kernel_kinds()-1, named by wkv_kernel_name().

@@ -19,7 +19,7 @@ REPO_ROOT = PKG_ROOT.parent
 CSRC = PKG_ROOT / "csrc"
 LIB_DIR = PKG_ROOT / "lib"
 LIB = LIB_DIR / "libspikegpt_wkv.so"
-SOURCES = [CSRC / "wkv_capi.cu"]
+SOURCES = [CSRC / "wkv_capi.cu", CSRC / "mixer_capi.cu"]
 DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + [REPO_ROOT / "include" / "spikegpt_wkv.h"]
 
 NVCC_FLAGS = [
@@ -28,7 +28,6 @@ NVCC_FLAGS = [
     "-O3",
     "-lineinfo",
     "-std=c++17",
-    "-shared",
     "-Xcompiler",
     "-fPIC",
     "-Xcompiler",
@@ -52,8 +51,16 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     cmd = [nvcc(), *NVCC_FLAGS, "-I", str(REPO_ROOT / "include"), "-I", str(CSRC)]
     if verbose:
         cmd += ["-Xptxas", "-v"]
-    cmd += [*map(str, SOURCES), "-o", str(tmp)]
-    subprocess.run(cmd, check=True)
+    objects = [LIB_DIR / f"{src.stem}.{os.getpid()}.o" for src in SOURCES]
+    try:
+        jobs = [subprocess.Popen([*cmd, "-c", str(src), "-o", str(obj)]) for src, obj in zip(SOURCES, objects)]
+        status = [job.wait() for job in jobs]  # the sources compile side by side
+        if any(status):
+            raise subprocess.CalledProcessError(max(status, key=abs), cmd)
+        subprocess.run([nvcc(), "-shared", *NVCC_FLAGS, *map(str, objects), "-o", str(tmp)], check=True)
+    finally:
+        for obj in objects:
+            obj.unlink(missing_ok=True)
     tmp.replace(LIB)
     return LIB
 

@@ -1,0 +1,585 @@
+// C ABI of the selective-mixer operators (declared in include/spikegpt_wkv.h):
+// the short causal convolution, the selective scan, their single-token steps,
+// layer norm, and the matrix-vector product with 4-bit weights. Argument checks,
+// workspace layout, the choice of kernel variants and the launches; every entry
+// point is asynchronous on the caller's stream and allocates nothing.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <initializer_list>
+#include <type_traits>
+
+#include "capi_host.cuh"
+#include "causal_conv.cuh"
+#include "layer_norm.cuh"
+#include "q4_matvec.cuh"
+#include "selective_scan.cuh"
+
+namespace {
+
+using namespace wkv;
+using namespace wkv_host;
+
+constexpr int64_t kMaxDim = 1ll << 30;
+
+// Calls f with a value of the dtype's element type.
+template <class F>
+int with_type(int dtype, F&& f) {
+  switch (dtype) {
+    case WKV_DTYPE_F32: return f(float{});
+    case WKV_DTYPE_BF16: return f(__nv_bfloat16{});
+    default: return f(__half{});
+  }
+}
+
+int check_type(int dtype) {
+  return dtype_size(dtype) == 0 ? fail(WKV_ERR_INVALID_ARGUMENT, "unknown dtype code %d", dtype) : WKV_OK;
+}
+
+int check_sizes(std::initializer_list<int64_t> sizes) {
+  for (int64_t v : sizes) {
+    if (v < 0) return fail(WKV_ERR_INVALID_ARGUMENT, "negative size %lld", (long long)v);
+    if (v > kMaxDim) return fail(WKV_ERR_INVALID_ARGUMENT, "size out of range: %lld", (long long)v);
+  }
+  return WKV_OK;
+}
+
+int check_pointers(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (!p) return fail(WKV_ERR_INVALID_ARGUMENT, "null pointer");
+  return WKV_OK;
+}
+
+// The largest number of adjacent elements (a power of two up to `most`) that
+// every pointer and row pitch lets a thread move as one aligned word.
+int vector_width(size_t es, int most, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> pitches) {
+  int v = most;
+  for (const void* p : ptrs)
+    while (v > 1 && reinterpret_cast<uintptr_t>(p) % (v * es) != 0) v /= 2;
+  for (int64_t s : pitches)
+    while (v > 1 && s % v != 0) v /= 2;
+  return v;
+}
+
+int launch_column_sums(ColSumArgs a, cudaStream_t st) {
+  const int64_t width = a.C * a.blocks;
+  if (width == 0) return WKV_OK;
+  launch(K_COL_SUM, st, [&] { column_sum_kernel<<<(unsigned)((width + 31) / 32), dim3(32, 32), 0, st>>>(a); });
+  return launched("column sum launch");
+}
+
+// ----------------------------------------------------------- causal convolution
+
+int conv_check(int dtype, int64_t B, int64_t T, int64_t C, int W) {
+  if (int rc = check_type(dtype)) return rc;
+  if (int rc = check_sizes({B, T, C})) return rc;
+  if (W < 1 || W > kConvMaxTaps)
+    return fail(WKV_ERR_INVALID_ARGUMENT, "the convolution's width must be 1..%d, got %d", kConvMaxTaps, W);
+  if (B > 0 && C > 0 && ((T + kConvSteps - 1) / kConvSteps + 1) * ((C + kConvThreads - 1) / kConvThreads) > INT_MAX / B)
+    return fail(WKV_ERR_INVALID_ARGUMENT, "sizes out of range B=%lld T=%lld C=%lld", (long long)B, (long long)T,
+                (long long)C);
+  return WKV_OK;
+}
+
+int conv_chunks(int64_t T) { return (int)std::max<int64_t>(1, (T + kConvSteps - 1) / kConvSteps); }
+
+// Calls f(element, integral constant V, integral constant W).
+template <class F>
+int conv_dispatch(int dtype, int V, int W, F&& f) {
+  return with_type(dtype, [&](auto e) {
+    using T = decltype(e);
+    auto taps = [&](auto v) {
+      switch (W) {
+        case 1: return f(e, v, std::integral_constant<int, 1>{});
+        case 2: return f(e, v, std::integral_constant<int, 2>{});
+        case 3: return f(e, v, std::integral_constant<int, 3>{});
+        default: return f(e, v, std::integral_constant<int, 4>{});
+      }
+    };
+    if (V >= 4) return taps(std::integral_constant<int, 4>{});
+    if (V >= 2) return taps(std::integral_constant<int, 2>{});
+    return taps(std::integral_constant<int, 1>{});
+  });
+}
+
+ConvArgs conv_args(const void* x, const float* w, const float* bias, const void* front, const int* lengths,
+                   int64_t B, int64_t T, int64_t C, int64_t x_sb, int64_t x_st, int silu) {
+  ConvArgs a{};
+  a.x = x;
+  a.w = w;
+  a.bias = bias;
+  a.front = front;
+  a.lengths = lengths;
+  a.x_sb = x_sb;
+  a.x_st = x_st;
+  a.B = (int)B;
+  a.T = (int)T;
+  a.C = (int)C;
+  a.chunks = conv_chunks(T);
+  a.silu = silu;
+  return a;
+}
+
+// ---------------------------------------------------------------- layer norm
+
+int norm_check(int dtype, int64_t rows, int64_t C) {
+  if (int rc = check_type(dtype)) return rc;
+  if (int rc = check_sizes({rows, C})) return rc;
+  if (C > kNormMaxC) return fail(WKV_ERR_INVALID_ARGUMENT, "layer norm takes rows of up to %d, got %lld", kNormMaxC, (long long)C);
+  return WKV_OK;
+}
+
+int norm_grid(int64_t rows) { return (int)std::min<int64_t>(rows, 2 * sm_count()); }
+
+// --------------------------------------------------------------------- scan
+
+int scan_check(int dtype, int64_t B, int64_t T, int64_t C, int64_t N) {
+  if (int rc = check_type(dtype)) return rc;
+  if (int rc = check_sizes({B, T, C, N})) return rc;
+  if (N < 1 || N > kScanMaxN)
+    return fail(WKV_ERR_INVALID_ARGUMENT, "the state size must be 1..%d, got %lld", kScanMaxN, (long long)N);
+  if (B > 0 && (C + 31) / 32 > INT_MAX / B)
+    return fail(WKV_ERR_INVALID_ARGUMENT, "sizes out of range B=%lld C=%lld", (long long)B, (long long)C);
+  return WKV_OK;
+}
+
+template <class F>
+int scan_dispatch(int dtype, int64_t N, F&& f) {
+  return with_type(dtype, [&](auto e) {
+    if (N <= 8) return f(e, std::integral_constant<int, 8>{});
+    if (N <= 16) return f(e, std::integral_constant<int, 16>{});
+    if (N <= 32) return f(e, std::integral_constant<int, 32>{});
+    return f(e, std::integral_constant<int, 64>{});
+  });
+}
+
+int64_t scan_ckpts(int64_t T) { return (T + kScanCkpt - 1) / kScanCkpt; }
+
+struct ScanBwdWs {
+  float *bc, *a, *d;
+  int slices;
+  size_t bytes;
+};
+ScanBwdWs scan_bwd_ws(int64_t B, int64_t T, int64_t C, int64_t N, void* base) {
+  ScanBwdWs w{};
+  w.slices = (int)((C + 31) / 32);
+  char* cur = static_cast<char*>(base);
+  auto take = [&](size_t n) {
+    float* r = reinterpret_cast<float*>(cur);
+    const size_t sz = round_up(n * sizeof(float));
+    if (cur) cur += sz;
+    w.bytes += sz;
+    return r;
+  };
+  w.bc = take((size_t)w.slices * B * T * 2 * N);
+  w.a = take((size_t)B * C * N);
+  w.d = take((size_t)B * 2 * C);
+  return w;
+}
+
+// --------------------------------------------------------------- 4-bit weights
+
+int q4_check(int dtype, int64_t M, int64_t N, int64_t K, int64_t G) {
+  if (int rc = check_type(dtype)) return rc;
+  if (int rc = check_sizes({M, N, K})) return rc;
+  if (G < 32 || G % 32 != 0 || G > kMaxDim)
+    return fail(WKV_ERR_INVALID_ARGUMENT, "the group size must be a positive multiple of 32, got %lld", (long long)G);
+  return WKV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int causal_conv_forward(int dtype, const void* x, const float* weight, const float* bias, const void* window_in,
+                        const int* lengths, void* y, void* window_out, int64_t B, int64_t T, int64_t C, int W,
+                        int64_t x_stride_b, int64_t x_stride_t, int silu, void* stream) {
+  g_last_error[0] = '\0';
+  if (int rc = conv_check(dtype, B, T, C, W)) return rc;
+  if (B == 0 || C == 0 || (T == 0 && !window_out)) return WKV_OK;
+  if (int rc = check_pointers({weight})) return rc;
+  if (T > 0)
+    if (int rc = check_pointers({x, y})) return rc;
+  ConvArgs a = conv_args(x, weight, bias, window_in, lengths, B, T, C, x_stride_b, x_stride_t, silu);
+  a.y = y;
+  a.window = W > 1 ? window_out : nullptr;
+  const int V = vector_width(dtype_size(dtype), 4, {x, y, window_in, window_out}, {C, x_stride_b, x_stride_t});
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return conv_dispatch(dtype, V, W, [&](auto e, auto v, auto w) {
+    constexpr int kV = decltype(v)::value;
+    a.cblocks = (int)((C + kConvThreads * kV - 1) / (kConvThreads * kV));
+    launch(K_CONV_FWD, st, [&] {
+      causal_conv_fwd_kernel<decltype(e), kV, decltype(w)::value>
+          <<<(unsigned)(a.cblocks * (int64_t)a.chunks * B), kConvThreads, 0, st>>>(a);
+    });
+    return launched("causal_conv forward launch");
+  });
+}
+
+size_t causal_conv_workspace_size(int64_t B, int64_t T, int64_t C, int W) {
+  if (conv_check(WKV_DTYPE_F32, B, T, C, W)) return 0;
+  return round_up((size_t)B * conv_chunks(T) * (W + 1) * C * sizeof(float));
+}
+
+int causal_conv_backward(int dtype, const void* grad_y, const void* x, const float* weight, const float* bias,
+                         const void* window_in, const int* lengths, void* grad_x, float* grad_weight,
+                         float* grad_bias, void* grad_window, void* workspace, size_t workspace_bytes, int64_t B,
+                         int64_t T, int64_t C, int W, int64_t g_stride_b, int64_t g_stride_t, int64_t x_stride_b,
+                         int64_t x_stride_t, int silu, void* stream) {
+  g_last_error[0] = '\0';
+  if (int rc = conv_check(dtype, B, T, C, W)) return rc;
+  if (C == 0) return WKV_OK;
+  if (int rc = check_pointers({weight, grad_weight})) return rc;
+  if (T > 0 && B > 0)
+    if (int rc = check_pointers({grad_y, x, grad_x})) return rc;
+  const size_t need = causal_conv_workspace_size(B, T, C, W);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(WKV_ERR_WORKSPACE_TOO_SMALL, "causal_conv backward needs %zu workspace bytes, got %zu", need,
+                workspace_bytes);
+  ConvArgs a = conv_args(x, weight, bias, window_in, lengths, B, T, C, x_stride_b, x_stride_t, silu);
+  a.gy = grad_y;
+  a.gy_sb = g_stride_b;
+  a.gy_st = g_stride_t;
+  a.y = grad_x;
+  a.window = W > 1 ? grad_window : nullptr;
+  a.partial = static_cast<float*>(workspace);
+  const int V = vector_width(dtype_size(dtype), 4, {x, grad_y, grad_x, window_in, grad_window},
+                             {C, x_stride_b, x_stride_t, g_stride_b, g_stride_t});
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (B > 0) {
+    const int rc = conv_dispatch(dtype, V, W, [&](auto e, auto v, auto w) {
+      constexpr int kV = decltype(v)::value;
+      a.cblocks = (int)((C + kConvThreads * kV - 1) / (kConvThreads * kV));
+      launch(K_CONV_BWD, st, [&] {
+        causal_conv_bwd_kernel<decltype(e), kV, decltype(w)::value>
+            <<<(unsigned)(a.cblocks * (int64_t)a.chunks * B), kConvThreads, 0, st>>>(a);
+      });
+      return launched("causal_conv backward launch");
+    });
+    if (rc) return rc;
+  }
+  ColSumArgs s{};
+  s.in = a.partial;
+  s.rows = (int)(B * a.chunks);
+  s.blocks = W + 1;
+  s.C = C;
+  for (int j = 0; j < W; ++j) {
+    s.out[j] = grad_weight + j;
+    s.step[j] = W;
+  }
+  s.out[W] = grad_bias;
+  s.step[W] = 1;
+  return launch_column_sums(s, st);
+}
+
+int causal_conv_step(int dtype, const void* x, const float* weight, const float* bias, void* window, void* y,
+                     int64_t B, int64_t C, int W, int64_t x_stride_b, int silu, void* stream) {
+  g_last_error[0] = '\0';
+  if (int rc = conv_check(dtype, B, 1, C, W)) return rc;
+  if (B == 0 || C == 0) return WKV_OK;
+  if (int rc = check_pointers({x, weight, y})) return rc;
+  if (W > 1 && !window) return fail(WKV_ERR_INVALID_ARGUMENT, "null pointer");
+  ConvArgs a = conv_args(x, weight, bias, nullptr, nullptr, B, 1, C, x_stride_b, C, silu);
+  a.y = y;
+  a.window = window;
+  const int V = vector_width(dtype_size(dtype), 4, {x, y, window}, {C, x_stride_b});
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return conv_dispatch(dtype, V, W, [&](auto e, auto v, auto w) {
+    constexpr int kV = decltype(v)::value;
+    a.cblocks = (int)((C + kConvThreads * kV - 1) / (kConvThreads * kV));
+    launch(K_CONV_STEP, st, [&] {
+      causal_conv_step_kernel<decltype(e), kV, decltype(w)::value>
+          <<<(unsigned)(a.cblocks * B), kConvThreads, 0, st>>>(a);
+    });
+    return launched("causal_conv step launch");
+  });
+}
+
+size_t selective_scan_state_size(int64_t B, int64_t T, int64_t C, int64_t N) {
+  if (scan_check(WKV_DTYPE_F32, B, T, C, N)) return 0;
+  return (size_t)B * scan_ckpts(T) * C * N * sizeof(float);
+}
+
+int selective_scan_forward(int dtype, const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+                           const float* D, const void* z, const float* dt_bias, const float* state_in,
+                           const int* lengths, void* out, float* state_out, float* kept, size_t kept_bytes,
+                           void* workspace, size_t workspace_bytes, int64_t B, int64_t T, int64_t C, int64_t N,
+                           int64_t x_sb, int64_t x_st, int64_t dt_sb, int64_t dt_st, int64_t b_sb, int64_t b_st,
+                           int64_t c_sb, int64_t c_st, int64_t z_sb, int64_t z_st, int softplus, void* stream) {
+  g_last_error[0] = '\0';
+  if (int rc = scan_check(dtype, B, T, C, N)) return rc;
+  if (B == 0 || C == 0 || (T == 0 && !state_out)) return WKV_OK;
+  if (int rc = check_pointers({A})) return rc;
+  if (T > 0)
+    if (int rc = check_pointers({x, dt, Bm, Cm, out})) return rc;
+  if (kept && kept_bytes < selective_scan_state_size(B, T, C, N))
+    return fail(WKV_ERR_WORKSPACE_TOO_SMALL, "selective_scan keeps %zu bytes of states, got %zu",
+                selective_scan_state_size(B, T, C, N), kept_bytes);
+  ScanArgs a{};
+  a.x = x;
+  a.dt = dt;
+  a.A = A;
+  a.Bm = Bm;
+  a.Cm = Cm;
+  a.D = D;
+  a.z = z;
+  a.bias = dt_bias;
+  a.h0 = state_in;
+  a.lengths = lengths;
+  a.out = out;
+  a.h_last = state_out;
+  a.ckpt = kept;
+  a.x_sb = x_sb, a.x_st = x_st, a.dt_sb = dt_sb, a.dt_st = dt_st, a.b_sb = b_sb, a.b_st = b_st;
+  a.c_sb = c_sb, a.c_st = c_st, a.z_sb = z_sb, a.z_st = z_st;
+  a.B = (int)B, a.T = (int)T, a.C = (int)C, a.N = (int)N;
+  a.softplus = softplus;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return scan_dispatch(dtype, N, [&](auto e, auto n) {
+    launch(K_SCAN_FWD, st, [&] {
+      scan_fwd_kernel<decltype(e), decltype(n)::value><<<(unsigned)(B * ((C + 31) / 32)), 32, 0, st>>>(a);
+    });
+    return launched("selective_scan forward launch");
+  });
+}
+
+size_t selective_scan_forward_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int64_t N) {
+  if (scan_check(dtype, B, T, C, N)) return 0;
+  return 0;
+}
+
+size_t selective_scan_backward_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int64_t N) {
+  if (scan_check(dtype, B, T, C, N)) return 0;
+  return scan_bwd_ws(B, T, C, N, nullptr).bytes;
+}
+
+int selective_scan_backward(int dtype, const void* grad_out, const void* x, const void* dt, const float* A,
+                            const void* Bm, const void* Cm, const float* D, const void* z, const float* dt_bias,
+                            const float* kept, const int* lengths, const float* grad_state_out, void* grad_x,
+                            void* grad_dt, float* grad_A, void* grad_B, void* grad_C, float* grad_D, void* grad_z,
+                            float* grad_dt_bias, float* grad_state_in, void* workspace, size_t workspace_bytes,
+                            int64_t B, int64_t T, int64_t C, int64_t N, int64_t g_sb, int64_t g_st, int64_t x_sb,
+                            int64_t x_st, int64_t dt_sb, int64_t dt_st, int64_t b_sb, int64_t b_st, int64_t c_sb,
+                            int64_t c_st, int64_t z_sb, int64_t z_st, int softplus, void* stream) {
+  g_last_error[0] = '\0';
+  if (int rc = scan_check(dtype, B, T, C, N)) return rc;
+  if (C == 0) return WKV_OK;
+  if (int rc = check_pointers({A, grad_A})) return rc;
+  if (B > 0 && T > 0)
+    if (int rc = check_pointers({grad_out, x, dt, Bm, Cm, kept, grad_x, grad_dt, grad_B, grad_C})) return rc;
+  if (B > 0 && T > 0 && (z != nullptr) != (grad_z != nullptr))
+    return fail(WKV_ERR_INVALID_ARGUMENT, "z and grad_z go together");
+  const size_t need = scan_bwd_ws(B, T, C, N, nullptr).bytes;
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(WKV_ERR_WORKSPACE_TOO_SMALL, "selective_scan backward needs %zu workspace bytes, got %zu", need,
+                workspace_bytes);
+  const ScanBwdWs ws = scan_bwd_ws(B, T, C, N, workspace);
+  ScanArgs a{};
+  a.gout = grad_out;
+  a.x = x;
+  a.dt = dt;
+  a.A = A;
+  a.Bm = Bm;
+  a.Cm = Cm;
+  a.D = D;
+  a.z = z;
+  a.bias = dt_bias;
+  a.ckpt = const_cast<float*>(kept);
+  a.lengths = lengths;
+  a.gh_last = grad_state_out;
+  a.gx = grad_x;
+  a.gdt = grad_dt;
+  a.gz = grad_z;
+  a.gh0 = grad_state_in;
+  a.part_bc = ws.bc;
+  a.part_a = ws.a;
+  a.part_d = ws.d;
+  a.x_sb = x_sb, a.x_st = x_st, a.dt_sb = dt_sb, a.dt_st = dt_st, a.b_sb = b_sb, a.b_st = b_st;
+  a.c_sb = c_sb, a.c_st = c_st, a.z_sb = z_sb, a.z_st = z_st, a.g_sb = g_sb, a.g_st = g_st;
+  a.B = (int)B, a.T = (int)T, a.C = (int)C, a.N = (int)N;
+  a.softplus = softplus;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (B > 0) {
+    int rc = scan_dispatch(dtype, N, [&](auto e, auto n) {
+      launch(K_SCAN_BWD, st, [&] {
+        scan_bwd_kernel<decltype(e), decltype(n)::value><<<(unsigned)(B * ((C + 31) / 32)), 32, 0, st>>>(a);
+      });
+      return launched("selective_scan backward launch");
+    });
+    if (rc) return rc;
+    const int64_t cells = B * T * 2 * N;
+    if (cells > 0) {
+      rc = with_type(dtype, [&](auto e) {
+        launch(K_SCAN_RED, st, [&] {
+          scan_reduce_kernel<decltype(e)><<<(unsigned)((cells + 255) / 256), 256, 0, st>>>(ws.bc, ws.slices, B * T,
+                                                                                          (int)N, grad_B, grad_C);
+        });
+        return launched("selective_scan reduction launch");
+      });
+      if (rc) return rc;
+    }
+  }
+  ColSumArgs s{};
+  s.in = ws.a;
+  s.rows = (int)B;
+  s.blocks = 1;
+  s.C = C * N;
+  s.out[0] = grad_A;
+  s.step[0] = 1;
+  if (int rc = launch_column_sums(s, st)) return rc;
+  if (!grad_D && !grad_dt_bias) return WKV_OK;
+  s.in = ws.d;
+  s.blocks = 2;
+  s.C = C;
+  s.out[0] = grad_D;
+  s.out[1] = grad_dt_bias;
+  s.step[1] = 1;
+  return launch_column_sums(s, st);
+}
+
+int selective_scan_step(int dtype, const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+                        float* state, const float* D, const void* z, const float* dt_bias, void* out, int64_t B,
+                        int64_t C, int64_t N, int64_t x_sb, int64_t dt_sb, int64_t b_sb, int64_t c_sb, int64_t z_sb,
+                        int softplus, void* stream) {
+  g_last_error[0] = '\0';
+  if (int rc = scan_check(dtype, B, 1, C, N)) return rc;
+  if (B == 0 || C == 0) return WKV_OK;
+  if (int rc = check_pointers({x, dt, A, Bm, Cm, state, out})) return rc;
+  ScanArgs a{};
+  a.x = x;
+  a.dt = dt;
+  a.A = A;
+  a.Bm = Bm;
+  a.Cm = Cm;
+  a.D = D;
+  a.z = z;
+  a.bias = dt_bias;
+  a.out = out;
+  a.h_last = state;
+  a.x_sb = x_sb, a.dt_sb = dt_sb, a.b_sb = b_sb, a.c_sb = c_sb, a.z_sb = z_sb;
+  a.B = (int)B, a.T = 1, a.C = (int)C, a.N = (int)N;
+  a.softplus = softplus;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return scan_dispatch(dtype, N, [&](auto e, auto n) {
+    launch(K_SCAN_STEP, st, [&] {
+      scan_step_kernel<decltype(e), decltype(n)::value><<<(unsigned)((B * C + 127) / 128), 128, 0, st>>>(a);
+    });
+    return launched("selective_scan step launch");
+  });
+}
+
+int layer_norm_forward(int dtype, const void* x, const float* weight, const float* bias, void* y, float* mean,
+                       float* rstd, int64_t rows, int64_t C, int64_t x_stride, float eps, void* stream) {
+  g_last_error[0] = '\0';
+  if (int rc = norm_check(dtype, rows, C)) return rc;
+  if (rows == 0 || C == 0) return WKV_OK;
+  if (int rc = check_pointers({x, y, mean, rstd})) return rc;
+  NormArgs a{};
+  a.x = x;
+  a.w = weight;
+  a.b = bias;
+  a.y = y;
+  a.mean = mean;
+  a.rstd = rstd;
+  a.rows = rows;
+  a.C = (int)C;
+  a.x_s = x_stride;
+  a.eps = eps;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return with_type(dtype, [&](auto e) {
+    launch(K_LN_FWD, st, [&] { layer_norm_fwd_kernel<decltype(e)><<<(unsigned)rows, kNormThreads, 0, st>>>(a); });
+    return launched("layer_norm forward launch");
+  });
+}
+
+size_t layer_norm_workspace_size(int dtype, int64_t rows, int64_t C) {
+  if (norm_check(dtype, rows, C)) return 0;
+  return round_up((size_t)norm_grid(rows) * 2 * C * sizeof(float));
+}
+
+int layer_norm_backward(int dtype, const void* grad_y, const void* x, const float* weight, const float* mean,
+                        const float* rstd, void* grad_x, float* grad_weight, float* grad_bias, void* workspace,
+                        size_t workspace_bytes, int64_t rows, int64_t C, int64_t g_stride, int64_t x_stride,
+                        void* stream) {
+  g_last_error[0] = '\0';
+  if (int rc = norm_check(dtype, rows, C)) return rc;
+  if (C == 0) return WKV_OK;
+  if (rows > 0)
+    if (int rc = check_pointers({grad_y, x, mean, rstd, grad_x})) return rc;
+  const size_t need = layer_norm_workspace_size(dtype, rows, C);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(WKV_ERR_WORKSPACE_TOO_SMALL, "layer_norm backward needs %zu workspace bytes, got %zu", need,
+                workspace_bytes);
+  NormArgs a{};
+  a.x = x;
+  a.w = weight;
+  a.gy = grad_y;
+  a.y = grad_x;
+  a.mean = const_cast<float*>(mean);
+  a.rstd = const_cast<float*>(rstd);
+  a.partial = static_cast<float*>(workspace);
+  a.rows = rows;
+  a.C = (int)C;
+  a.x_s = x_stride;
+  a.gy_s = g_stride;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int grid = norm_grid(rows);
+  if (rows > 0) {
+    const int rc = with_type(dtype, [&](auto e) {
+      using T = decltype(e);
+      const cudaError_t err = allow_smem(layer_norm_bwd_kernel<T>, 2 * kNormMaxC * sizeof(float));
+      if (err != cudaSuccess) return cuda_fail(err, "setting the layer_norm backward kernel's shared memory size");
+      launch(K_LN_BWD, st,
+             [&] { layer_norm_bwd_kernel<T><<<(unsigned)grid, kNormThreads, 2 * C * sizeof(float), st>>>(a); });
+      return launched("layer_norm backward launch");
+    });
+    if (rc) return rc;
+  }
+  if (!grad_weight && !grad_bias) return WKV_OK;
+  ColSumArgs s{};
+  s.in = a.partial;
+  s.rows = grid;
+  s.blocks = 2;
+  s.C = C;
+  s.out[0] = grad_weight;
+  s.out[1] = grad_bias;
+  s.step[0] = s.step[1] = 1;
+  return launch_column_sums(s, st);
+}
+
+int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scales, const uint8_t* zeros,
+              const float* bias, void* y, int64_t M, int64_t N, int64_t K, int64_t group, int64_t x_stride,
+              void* stream) {
+  g_last_error[0] = '\0';
+  if (int rc = q4_check(dtype, M, N, K, group)) return rc;
+  if (M == 0 || N == 0) return WKV_OK;
+  if (int rc = check_pointers({y})) return rc;
+  if (K > 0)
+    if (int rc = check_pointers({x, packed, scales})) return rc;
+  Q4Args a{};
+  a.x = x;
+  a.q = packed;
+  a.scale = static_cast<const __nv_bfloat16*>(scales);
+  a.zero = zeros;
+  a.bias = bias;
+  a.y = y;
+  a.x_s = x_stride;
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.G = (int)group;
+  a.groups = (int)((K + group - 1) / group);
+  a.pitch = (int)((K + 31) / 32 * 16);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t my = (M + kQ4Tokens - 1) / kQ4Tokens;
+  if (my > 65535) return fail(WKV_ERR_INVALID_ARGUMENT, "too many tokens: %lld", (long long)M);
+  return with_type(dtype, [&](auto e) {
+    launch(K_Q4, st, [&] {
+      q4_matvec_kernel<decltype(e)>
+          <<<dim3((unsigned)((N + kQ4Threads / 32 - 1) / (kQ4Threads / 32)), (unsigned)my), kQ4Threads, 0, st>>>(a);
+    });
+    return launched("q4_matvec launch");
+  });
+}
+
+}  // extern "C"

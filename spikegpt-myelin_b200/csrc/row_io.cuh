@@ -1,0 +1,119 @@
+// Typed vector access for the mixer kernels: V adjacent elements of float,
+// bfloat16 or float16 moved as one word and widened to float32.
+#pragma once
+
+#include "wkv_device.cuh"
+
+namespace wkv {
+
+template <int kBytes>
+struct Word;
+template <>
+struct Word<2> {
+  using type = uint16_t;
+};
+template <>
+struct Word<4> {
+  using type = uint32_t;
+};
+template <>
+struct Word<8> {
+  using type = uint2;
+};
+template <>
+struct Word<16> {
+  using type = uint4;
+};
+
+// V elements of T as they lie in memory (V * sizeof(T) is 2, 4, 8 or 16 bytes,
+// and addresses are multiples of that).
+template <typename T, int V>
+struct Vec {
+  using word = typename Word<V * static_cast<int>(sizeof(T))>::type;
+  union {
+    word w;
+    T e[V];
+  };
+  __device__ __forceinline__ Vec() {}
+  __device__ __forceinline__ static Vec load(const T* p) {
+    Vec r;
+    r.w = *reinterpret_cast<const word*>(p);
+    return r;
+  }
+  __device__ __forceinline__ static Vec load_once(const T* p) {  // read-only data that no other thread reads again
+    Vec r;
+    if constexpr (V * sizeof(T) == 2)
+      r.w = __ldcs(reinterpret_cast<const unsigned short*>(p));
+    else
+      r.w = __ldcs(reinterpret_cast<const word*>(p));
+    return r;
+  }
+  __device__ __forceinline__ static Vec zero() {
+    Vec r;
+    r.w = word{};
+    return r;
+  }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<word*>(p) = w; }
+  __device__ __forceinline__ void get(float (&f)[V]) const {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(&w);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const f2 p = Pair<T>::unpack(u[i]);
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = Pair<T>::scalar(e[i]);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[V]) {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+      uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) u[i] = Pair<T>::pack(f2{f[2 * i], f[2 * i + 1]});
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = Pair<T>::from_float(f[i]);
+    }
+  }
+};
+
+// 1 / (1 + e^-v); 0 and 1 at the infinities.
+__device__ __forceinline__ float sigmoid1(float v) { return __fdividef(1.f, 1.f + ex2(-v * kL2E)); }
+
+// Column sums of `rows` float32 rows of `blocks` groups of C columns, in row
+// order within each of 32 strides and then over the strides in order, so the
+// result does not depend on timing. Group k goes to out[k][c * step[k]].
+constexpr int kSumGroups = 6;
+struct ColSumArgs {
+  const float* in;
+  float* out[kSumGroups];
+  int step[kSumGroups];
+  int rows, blocks;
+  int64_t C;
+};
+
+__global__ void __launch_bounds__(1024) column_sum_kernel(ColSumArgs a) {
+  __shared__ float red[32][33];
+  const int64_t width = a.C * a.blocks;
+  const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  float s = 0.f;
+  if (col < width) {
+    const float* p = a.in + col;
+    for (int r = threadIdx.y; r < a.rows; r += 32) s += p[(int64_t)r * width];
+  }
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && col < width) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t += red[i][threadIdx.x];
+    const int k = (int)(col / a.C);
+    const int64_t c = col - (int64_t)k * a.C;
+    if (a.out[k]) a.out[k][c * a.step[k]] = t;
+  }
+}
+
+}  // namespace wkv

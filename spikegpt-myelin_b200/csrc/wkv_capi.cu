@@ -8,17 +8,15 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 #include <atomic>
-#include <cstdarg>
-#include <cstdio>
+#include <cmath>
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
 #include <type_traits>
 #include <vector>
 
-#include "spikegpt_wkv.h"
+#include "capi_host.cuh"
 #include "gates.cuh"
 #include "lif.cuh"
 #include "ln_mix.cuh"
@@ -30,8 +28,8 @@
 namespace {
 
 using namespace wkv;
+using namespace wkv_host;
 
-thread_local char g_last_error[512] = "";
 std::atomic<int> g_force_segments{0};
 std::atomic<int> g_force_generic{0};
 std::atomic<int> g_force_slow{0};
@@ -40,107 +38,11 @@ std::atomic<int> g_withhold_first{0};
 
 __device__ unsigned g_device_error_flags = 0;
 
-// ------------------------------------------------ launch accounting / timing
-//
-// Every kernel launch goes through launch(): it bumps a per-kind counter and,
-// while timing is enabled, brackets the launch with CUDA events recorded on the
-// launch stream, so per-kernel device time can be read back by the caller.
-
-enum Kind {
-  K_FWD_Y, K_FWD_STATE, K_BWD_GRAD, K_BWD_ADJ, K_CARRY_FWD, K_CARRY_ADJ, K_STEP, K_LIF_FWD, K_LIF_BWD,
-  K_MIX_FWD, K_MIX_BWD, K_MIX_RED,
-  K_GATE_FWD, K_GATE_BWD, K_RSQ_FWD, K_RSQ_BWD, K_RESID, K_LIF_SUM, K_R7_FWD, K_XENT_FWD, K_XENT_BWD,
-  K_COUNT
-};
-const char* const kKindNames[K_COUNT] = {
-    "wkv_fwd_kernel<y>",      "wkv_fwd_kernel<state>", "wkv_bwd_kernel<grad>",
-    "wkv_bwd_kernel<adjoint>", "wkv_carry_fwd_kernel",  "wkv_carry_adj_kernel",
-    "wkv_step_kernel",        "lif_fwd_kernel",        "lif_bwd_kernel",
-    "ln_mix_fwd_kernel",      "ln_mix_bwd_kernel",     "ln_mix_reduce_kernel",
-    "gate_fwd_kernel",        "gate_bwd_kernel",       "relu_square_fwd_kernel",
-    "relu_square_bwd_kernel", "residual_add_kernel",   "lif_bwd_summary_kernel",
-    "rwkv7_fwd_kernel",       "xent_fwd_kernel",       "xent_bwd_kernel"};
-
-std::atomic<long long> g_launches[K_COUNT];
-std::atomic<bool> g_timing{false};
-std::mutex g_timing_mu;
-struct TimedLaunch {
-  int kind;
-  cudaEvent_t start, stop;
-};
-std::vector<TimedLaunch> g_timed;
-std::vector<cudaEvent_t> g_event_pool;
-
-cudaEvent_t pooled_event() {
-  std::lock_guard<std::mutex> lk(g_timing_mu);
-  if (!g_event_pool.empty()) {
-    cudaEvent_t e = g_event_pool.back();
-    g_event_pool.pop_back();
-    return e;
-  }
-  cudaEvent_t e = nullptr;
-  if (cudaEventCreate(&e) != cudaSuccess) return nullptr;
-  return e;
-}
-
-template <class F>
-void launch(int kind, cudaStream_t st, F&& f) {
-  g_launches[kind].fetch_add(1, std::memory_order_relaxed);
-  if (!g_timing.load(std::memory_order_relaxed)) {
-    f();
-    return;
-  }
-  cudaEvent_t a = pooled_event(), b = pooled_event();
-  if (a) cudaEventRecord(a, st);
-  f();
-  if (b) cudaEventRecord(b, st);
-  if (a && b) {
-    std::lock_guard<std::mutex> lk(g_timing_mu);
-    g_timed.push_back(TimedLaunch{kind, a, b});
-  }
-}
-
-int fail(int status, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
-  va_end(ap);
-  return status;
-}
-
-int cuda_fail(cudaError_t e, const char* what) {
-  return fail(WKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
-size_t dtype_size(int dtype) {
-  switch (dtype) {
-    case WKV_DTYPE_F32: return 4;
-    case WKV_DTYPE_BF16: return 2;
-    case WKV_DTYPE_F16: return 2;
-    default: return 0;
-  }
-}
-
-int sm_count() {
-  static int cached[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (cached[dev] == 0) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-      n = 148;
-    cached[dev] = n;
-  }
-  return cached[dev];
-}
-
 struct Plan {
   bool tma;
   int nseg;
   int seg_len;
 };
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Segments (the chunked two-level scan across CTAs) against one sequential
 // sweep per lane set, chosen from a sweep of measured step times (forward +
@@ -180,8 +82,6 @@ Plan make_plan(int dtype, int64_t B, int64_t T, int64_t C, bool ptrs_aligned) {
   return p;
 }
 
-constexpr size_t kAlign = 256;
-size_t round_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
 
 struct FwdWs {
   float* seg;
@@ -364,24 +264,6 @@ int check_dims(int dtype, int64_t B, int64_t T, int64_t C) {
     return fail(WKV_ERR_INVALID_ARGUMENT, "size out of range B=%lld T=%lld C=%lld", (long long)B,
                 (long long)T, (long long)C);
   return WKV_OK;
-}
-
-// Kernels whose dynamic shared memory exceeds the 48 KB default opt in once per
-// device.
-template <typename K>
-cudaError_t allow_smem(K* kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return cudaSuccess;
-  static std::mutex mu;
-  static std::vector<std::pair<const void*, int>> done;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lk(mu);
-  for (auto& d : done)
-    if (d.first == reinterpret_cast<const void*>(kernel) && d.second == dev) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e == cudaSuccess) done.emplace_back(reinterpret_cast<const void*>(kernel), dev);
-  return e;
 }
 
 // ----------------------------------------------------------- launch helpers
@@ -1402,11 +1284,6 @@ int gate_check(int64_t n, std::initializer_list<const void*> ptrs) {
     if (!aligned16(p)) return fail(WKV_ERR_INVALID_ARGUMENT, "bf16 tensors must be 16-byte aligned");
   }
   return WKV_OK;
-}
-
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? WKV_OK : cuda_fail(e, what);
 }
 
 }  // namespace

@@ -13,6 +13,9 @@ from __future__ import annotations
 from . import _capi
 from ._ops import set_state_saving, state_saving_enabled, validate_wkv_inputs
 from .lif import SpikingSequenceLIF, surrogate_lif
+from .norm import layer_norm
+from .q4 import dequantize_q4, q4_linear, quantize_q4
+from .selective import causal_conv, causal_conv_step_, selective_scan, selective_scan_step_
 from .step import initial_step_state, weighted_key_value_step, weighted_key_value_step_
 from .wkv import weighted_key_value_cuda, weighted_key_value_triton
 from .wkv_bf16 import weighted_key_value_cuda_bf16io, weighted_key_value_triton_bf16io
@@ -30,5 +33,13 @@ __all__ = [
     "weighted_key_value_cuda_bf16io",
     "weighted_key_value_triton",
     "weighted_key_value_triton_bf16io",
+    "causal_conv",
+    "causal_conv_step_",
+    "selective_scan",
+    "selective_scan_step_",
+    "layer_norm",
+    "quantize_q4",
+    "dequantize_q4",
+    "q4_linear",
     "_capi",
 ]

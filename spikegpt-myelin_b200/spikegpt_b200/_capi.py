@@ -108,6 +108,44 @@ def lib() -> ctypes.CDLL:
         handle.cross_entropy_forward.restype = ci
         handle.cross_entropy_backward.argtypes = [vp, i64, vp, vp, vp, vp, i64, i64, vp]
         handle.cross_entropy_backward.restype = ci
+        handle.causal_conv_forward.argtypes = [ci, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, ci, i64, i64, ci, vp]
+        handle.causal_conv_forward.restype = ci
+        handle.causal_conv_workspace_size.argtypes = [i64, i64, i64, ci]
+        handle.causal_conv_workspace_size.restype = sz
+        handle.causal_conv_backward.argtypes = [
+            ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i64, i64, i64, ci, i64, i64, i64, i64, ci, vp,
+        ]
+        handle.causal_conv_backward.restype = ci
+        handle.causal_conv_step.argtypes = [ci, vp, vp, vp, vp, vp, i64, i64, ci, i64, ci, vp]
+        handle.causal_conv_step.restype = ci
+        handle.selective_scan_state_size.argtypes = [i64, i64, i64, i64]
+        handle.selective_scan_state_size.restype = sz
+        handle.selective_scan_forward.argtypes = [
+            ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp, sz, i64, i64, i64, i64, i64, i64, i64,
+            i64, i64, i64, i64, i64, i64, i64, ci, vp,
+        ]
+        handle.selective_scan_forward.restype = ci
+        handle.selective_scan_forward_workspace_size.argtypes = [ci, i64, i64, i64, i64]
+        handle.selective_scan_forward_workspace_size.restype = sz
+        handle.selective_scan_backward_workspace_size.argtypes = [ci, i64, i64, i64, i64]
+        handle.selective_scan_backward_workspace_size.restype = sz
+        handle.selective_scan_backward.argtypes = [
+            ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i64,
+            i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, ci, vp,
+        ]
+        handle.selective_scan_backward.restype = ci
+        handle.selective_scan_step.argtypes = [
+            ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, ci, vp,
+        ]
+        handle.selective_scan_step.restype = ci
+        handle.layer_norm_forward.argtypes = [ci, vp, vp, vp, vp, vp, vp, i64, i64, i64, f32, vp]
+        handle.layer_norm_forward.restype = ci
+        handle.layer_norm_workspace_size.argtypes = [ci, i64, i64]
+        handle.layer_norm_workspace_size.restype = sz
+        handle.layer_norm_backward.argtypes = [ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i64, i64, i64, i64, vp]
+        handle.layer_norm_backward.restype = ci
+        handle.q4_matvec.argtypes = [ci, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp]
+        handle.q4_matvec.restype = ci
         handle.wkv_state_size.argtypes = [ci, i64, i64, i64]
         handle.wkv_state_size.restype = sz
         handle.wkv_forward_with_state.argtypes = [ci, vp, vp, vp, vp, vp, vp, sz, i64, i64, i64, vp, sz, vp]
@@ -215,4 +253,4 @@ def declared_symbols() -> list[str]:
     import re
 
     text = HEADER_PATH.read_text()
-    return sorted(set(re.findall(r"WKV_API\s+[\w\s\*]+?\b((?:wkv|lif|ln_mix|gate|relu_square|residual_add|rwkv7|cross_entropy)_\w+)\s*\(", text)))
+    return sorted(set(re.findall(r"WKV_API\s+[\w\s\*]+?\b((?:wkv|lif|ln_mix|gate|relu_square|residual_add|rwkv7|cross_entropy|causal_conv|selective_scan|layer_norm|q4)_\w+)\s*\(", text)))
