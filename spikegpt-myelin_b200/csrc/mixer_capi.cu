@@ -22,6 +22,8 @@ using namespace wkv;
 using namespace wkv_host;
 
 constexpr int64_t kMaxDim = 1ll << 30;
+constexpr int kScanMaxSegments = 64;
+constexpr int kScanMinSegment = 64;
 
 // Calls f with a value of the dtype's element type.
 template <class F>
@@ -139,31 +141,64 @@ int scan_check(int dtype, int64_t B, int64_t T, int64_t C, int64_t N) {
   if (int rc = check_sizes({B, T, C, N})) return rc;
   if (N < 1 || N > kScanMaxN)
     return fail(WKV_ERR_INVALID_ARGUMENT, "the state size must be 1..%d, got %lld", kScanMaxN, (long long)N);
-  if (B > 0 && (C + 31) / 32 > INT_MAX / B)
-    return fail(WKV_ERR_INVALID_ARGUMENT, "sizes out of range B=%lld C=%lld", (long long)B, (long long)C);
+  if (T > (1 << 23) || (B > 0 && (C + 7) / 8 * kScanMaxSegments > INT_MAX / B))
+    return fail(WKV_ERR_INVALID_ARGUMENT, "sizes out of range B=%lld T=%lld C=%lld", (long long)B, (long long)T,
+                (long long)C);
   return WKV_OK;
 }
+
+// Lanes that share a channel: four states each.
+int scan_lanes(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 template <class F>
 int scan_dispatch(int dtype, int64_t N, F&& f) {
   return with_type(dtype, [&](auto e) {
-    if (N <= 8) return f(e, std::integral_constant<int, 8>{});
-    if (N <= 16) return f(e, std::integral_constant<int, 16>{});
-    if (N <= 32) return f(e, std::integral_constant<int, 32>{});
-    return f(e, std::integral_constant<int, 64>{});
+    switch (scan_lanes(N)) {
+      case 1: return f(e, std::integral_constant<int, 1>{});
+      case 2: return f(e, std::integral_constant<int, 2>{});
+      case 4: return f(e, std::integral_constant<int, 4>{});
+      case 8: return f(e, std::integral_constant<int, 8>{});
+      default: return f(e, std::integral_constant<int, 16>{});
+    }
   });
 }
 
 int64_t scan_ckpts(int64_t T) { return (T + kScanCkpt - 1) / kScanCkpt; }
 
-struct ScanBwdWs {
-  float *bc, *a, *d;
-  int slices;
+// How a call is cut: CTAs of `channels` channels and segments of seg_len steps.
+struct ScanPlan {
+  int groups, cblocks, nseg, seg_len;
+};
+// Segments where the channels alone do not give `want` CTAs; a segment is a
+// multiple of kScanRows steps and at least kScanMinSegment of them.
+ScanPlan scan_plan(int64_t B, int64_t T, int64_t C, int channels, int64_t want) {
+  ScanPlan p{1, (int)((C + channels - 1) / channels), 1, 0};
+  const int64_t sets = B * p.cblocks;
+  int64_t nseg = sets > 0 && sets < want ? (want + sets - 1) / sets : 1;
+  nseg = std::max<int64_t>(1, std::min<int64_t>({nseg, T / kScanMinSegment, kScanMaxSegments}));
+  const int64_t len = ((T + nseg - 1) / nseg + kScanRows - 1) / kScanRows * kScanRows;
+  p.seg_len = (int)std::max<int64_t>(len, kScanRows);
+  p.nseg = (int)std::max<int64_t>(1, (T + p.seg_len - 1) / p.seg_len);
+  return p;
+}
+ScanPlan scan_forward_plan(int64_t B, int64_t T, int64_t C, int64_t N) {
+  return scan_plan(B, T, C, kScanThreads / scan_lanes(N), 4 * sm_count());
+}
+ScanPlan scan_backward_plan(int64_t B, int64_t T, int64_t C, int64_t N) {
+  const int lanes = scan_lanes(N), channels = kScanThreads / lanes;
+  int g = std::min(4, lanes);
+  while (g > 1 && B * ((C + g * channels - 1) / (g * channels)) < 2 * sm_count()) g /= 2;
+  ScanPlan p = scan_plan(B, T, C, g * channels, 2 * sm_count());
+  p.groups = g;
+  return p;
+}
+
+struct ScanWs {
+  float *seg_h, *seg_d, *bc, *a, *d;
   size_t bytes;
 };
-ScanBwdWs scan_bwd_ws(int64_t B, int64_t T, int64_t C, int64_t N, void* base) {
-  ScanBwdWs w{};
-  w.slices = (int)((C + 31) / 32);
+ScanWs scan_ws(const ScanPlan& p, bool backward, int64_t B, int64_t T, int64_t C, int64_t N, void* base) {
+  ScanWs w{};
   char* cur = static_cast<char*>(base);
   auto take = [&](size_t n) {
     float* r = reinterpret_cast<float*>(cur);
@@ -172,10 +207,39 @@ ScanBwdWs scan_bwd_ws(int64_t B, int64_t T, int64_t C, int64_t N, void* base) {
     w.bytes += sz;
     return r;
   };
-  w.bc = take((size_t)w.slices * B * T * 2 * N);
-  w.a = take((size_t)B * C * N);
-  w.d = take((size_t)B * 2 * C);
+  if (p.nseg > 1) {
+    w.seg_h = take((size_t)B * p.nseg * C * N);
+    w.seg_d = take((size_t)B * p.nseg * C);
+  }
+  if (backward) {
+    w.bc = take((size_t)p.cblocks * B * T * 2 * N);
+    w.a = take((size_t)B * p.nseg * C * N);
+    w.d = take((size_t)B * p.nseg * 2 * C);
+  }
   return w;
+}
+
+template <class E, int kLanesPer>
+constexpr size_t scan_bwd_smem_max() {
+  using L = ScanBwdSmem<E, kLanesPer>;
+  size_t most = 0;
+  for (int g = 1; g <= L::M; g *= 2) most = most < (size_t)L::bytes(g) ? (size_t)L::bytes(g) : most;
+  return most;
+}
+
+void scan_layout(ScanArgs& a, const ScanPlan& p, const ScanWs& w, int dtype, std::initializer_list<const void*> rows,
+                 std::initializer_list<const void*> states) {
+  a.groups = p.groups;
+  a.cblocks = p.cblocks;
+  a.nseg = p.nseg;
+  a.seg_len = p.seg_len;
+  a.seg_h = w.seg_h;
+  a.seg_d = w.seg_d;
+  const int es = (int)dtype_size(dtype);
+  a.wide = a.C % 8 == 0 && vector_width(es, 16 / es, rows,
+                                        {a.x_sb, a.x_st, a.dt_sb, a.dt_st, a.z_sb, a.z_st, a.g_sb, a.g_st}) == 16 / es;
+  a.wide_bc = a.N % 4 == 0 && vector_width(es, 4, {a.Bm, a.Cm}, {a.b_sb, a.b_st, a.c_sb, a.c_st}) == 4;
+  a.wide_n = a.N % 4 == 0 && vector_width(4, 4, states, {}) == 4;
 }
 
 // --------------------------------------------------------------- 4-bit weights
@@ -334,10 +398,25 @@ int selective_scan_forward(int dtype, const void* x, const void* dt, const float
   a.c_sb = c_sb, a.c_st = c_st, a.z_sb = z_sb, a.z_st = z_st;
   a.B = (int)B, a.T = (int)T, a.C = (int)C, a.N = (int)N;
   a.softplus = softplus;
+  const ScanPlan p = scan_forward_plan(B, T, C, N);
+  const size_t need = scan_ws(p, false, B, T, C, N, nullptr).bytes;
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(WKV_ERR_WORKSPACE_TOO_SMALL, "selective_scan forward needs %zu workspace bytes, got %zu", need,
+                workspace_bytes);
+  scan_layout(a, p, scan_ws(p, false, B, T, C, N, workspace), dtype, {x, dt, z, out}, {A, state_in, state_out, kept});
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return scan_dispatch(dtype, N, [&](auto e, auto n) {
+  return scan_dispatch(dtype, N, [&](auto e, auto lanes) {
+    using E = decltype(e);
+    constexpr int kLanesPer = decltype(lanes)::value;
+    if (p.nseg > 1) {
+      launch(K_SCAN_SUM, st, [&] {
+        scan_summary_kernel<E, kLanesPer, false>
+            <<<(unsigned)(B * p.cblocks * (p.nseg - 1)), kScanThreads, 0, st>>>(a);
+      });
+      if (int rc = launched("selective_scan summary launch")) return rc;
+    }
     launch(K_SCAN_FWD, st, [&] {
-      scan_fwd_kernel<decltype(e), decltype(n)::value><<<(unsigned)(B * ((C + 31) / 32)), 32, 0, st>>>(a);
+      scan_fwd_kernel<E, kLanesPer><<<(unsigned)(B * p.cblocks * p.nseg), kScanThreads, 0, st>>>(a);
     });
     return launched("selective_scan forward launch");
   });
@@ -345,12 +424,12 @@ int selective_scan_forward(int dtype, const void* x, const void* dt, const float
 
 size_t selective_scan_forward_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int64_t N) {
   if (scan_check(dtype, B, T, C, N)) return 0;
-  return 0;
+  return scan_ws(scan_forward_plan(B, T, C, N), false, B, T, C, N, nullptr).bytes;
 }
 
 size_t selective_scan_backward_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int64_t N) {
   if (scan_check(dtype, B, T, C, N)) return 0;
-  return scan_bwd_ws(B, T, C, N, nullptr).bytes;
+  return scan_ws(scan_backward_plan(B, T, C, N), true, B, T, C, N, nullptr).bytes;
 }
 
 int selective_scan_backward(int dtype, const void* grad_out, const void* x, const void* dt, const float* A,
@@ -369,11 +448,12 @@ int selective_scan_backward(int dtype, const void* grad_out, const void* x, cons
     if (int rc = check_pointers({grad_out, x, dt, Bm, Cm, kept, grad_x, grad_dt, grad_B, grad_C})) return rc;
   if (B > 0 && T > 0 && (z != nullptr) != (grad_z != nullptr))
     return fail(WKV_ERR_INVALID_ARGUMENT, "z and grad_z go together");
-  const size_t need = scan_bwd_ws(B, T, C, N, nullptr).bytes;
+  const ScanPlan p = scan_backward_plan(B, T, C, N);
+  const size_t need = scan_ws(p, true, B, T, C, N, nullptr).bytes;
   if (workspace_bytes < need || (need > 0 && !workspace))
     return fail(WKV_ERR_WORKSPACE_TOO_SMALL, "selective_scan backward needs %zu workspace bytes, got %zu", need,
                 workspace_bytes);
-  const ScanBwdWs ws = scan_bwd_ws(B, T, C, N, workspace);
+  const ScanWs ws = scan_ws(p, true, B, T, C, N, workspace);
   ScanArgs a{};
   a.gout = grad_out;
   a.x = x;
@@ -399,10 +479,26 @@ int selective_scan_backward(int dtype, const void* grad_out, const void* x, cons
   a.B = (int)B, a.T = (int)T, a.C = (int)C, a.N = (int)N;
   a.softplus = softplus;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  scan_layout(a, p, ws, dtype, {grad_out, x, dt, z, grad_x, grad_dt, grad_z},
+              {A, kept, grad_state_out, grad_state_in});
   if (B > 0) {
-    int rc = scan_dispatch(dtype, N, [&](auto e, auto n) {
+    int rc = scan_dispatch(dtype, N, [&](auto e, auto lanes) {
+      using E = decltype(e);
+      constexpr int kLanesPer = decltype(lanes)::value;
+      if (p.nseg > 1) {
+        ScanArgs s = a;  // the summary kernel's channel blocks are one group wide
+        s.cblocks = (int)((C + kScanThreads / kLanesPer - 1) / (kScanThreads / kLanesPer));
+        launch(K_SCAN_ADJ, st, [&] {
+          scan_summary_kernel<E, kLanesPer, true>
+              <<<(unsigned)(B * s.cblocks * (p.nseg - 1)), kScanThreads, 0, st>>>(s);
+        });
+        if (int rc = launched("selective_scan adjoint launch")) return rc;
+      }
+      const cudaError_t err = allow_smem(scan_bwd_kernel<E, kLanesPer>, scan_bwd_smem_max<E, kLanesPer>());
+      if (err != cudaSuccess) return cuda_fail(err, "setting the selective_scan backward kernel's shared memory size");
       launch(K_SCAN_BWD, st, [&] {
-        scan_bwd_kernel<decltype(e), decltype(n)::value><<<(unsigned)(B * ((C + 31) / 32)), 32, 0, st>>>(a);
+        scan_bwd_kernel<E, kLanesPer><<<(unsigned)(B * p.cblocks * p.nseg), kScanThreads,
+                                        ScanBwdSmem<E, kLanesPer>::bytes(p.groups), st>>>(a);
       });
       return launched("selective_scan backward launch");
     });
@@ -411,7 +507,7 @@ int selective_scan_backward(int dtype, const void* grad_out, const void* x, cons
     if (cells > 0) {
       rc = with_type(dtype, [&](auto e) {
         launch(K_SCAN_RED, st, [&] {
-          scan_reduce_kernel<decltype(e)><<<(unsigned)((cells + 255) / 256), 256, 0, st>>>(ws.bc, ws.slices, B * T,
+          scan_reduce_kernel<decltype(e)><<<(unsigned)((cells + 255) / 256), 256, 0, st>>>(ws.bc, p.cblocks, B * T,
                                                                                           (int)N, grad_B, grad_C);
         });
         return launched("selective_scan reduction launch");
@@ -421,7 +517,7 @@ int selective_scan_backward(int dtype, const void* grad_out, const void* x, cons
   }
   ColSumArgs s{};
   s.in = ws.a;
-  s.rows = (int)B;
+  s.rows = (int)(B * p.nseg);
   s.blocks = 1;
   s.C = C * N;
   s.out[0] = grad_A;
@@ -460,9 +556,9 @@ int selective_scan_step(int dtype, const void* x, const void* dt, const float* A
   a.B = (int)B, a.T = 1, a.C = (int)C, a.N = (int)N;
   a.softplus = softplus;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return scan_dispatch(dtype, N, [&](auto e, auto n) {
+  return with_type(dtype, [&](auto e) {
     launch(K_SCAN_STEP, st, [&] {
-      scan_step_kernel<decltype(e), decltype(n)::value><<<(unsigned)((B * C + 127) / 128), 128, 0, st>>>(a);
+      scan_step_kernel<decltype(e)><<<(unsigned)((B * C + 127) / 128), 128, 0, st>>>(a);
     });
     return launched("selective_scan step launch");
   });

@@ -329,7 +329,7 @@ def _scan_op(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor |
 
 
 def _kept_bytes(b, t, c, n):
-    return b * ((t + 15) // 16) * c * n * 4
+    return b * ((t + 7) // 8) * c * n * 4
 
 
 @_scan_op.register_fake
@@ -440,7 +440,7 @@ def selective_scan(
     zeros); ``return_state`` adds the last state to the result. With ``lengths`` [B],
     what lies past a sequence's length is not read, gives zeros, and leaves the
     state as it is. Differentiable in every tensor but lengths; the backward keeps
-    the state of every 16th step (float32, N / 4 bytes for each element of x)."""
+    the state of every 8th step (float32, N / 2 bytes for each element of x)."""
     if x.ndim != 3:
         raise ValueError(f"x must have shape [B, T, C]; got {list(x.shape)}")
     b, t, c = x.shape
