@@ -147,18 +147,22 @@ int scan_check(int dtype, int64_t B, int64_t T, int64_t C, int64_t N) {
   return WKV_OK;
 }
 
-// Lanes that share a channel: four states each.
-int scan_lanes(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+// Lanes that share a channel, with `per` states each: a power of two.
+int scan_lanes(int64_t N, int per) {
+  int lanes = 1;
+  while (lanes * per < N) lanes *= 2;
+  return lanes;
+}
 
+// Calls f(element, lanes): eight states a lane in the forward, four in the backward.
 template <class F>
-int scan_dispatch(int dtype, int64_t N, F&& f) {
+int scan_dispatch(int dtype, int lanes, F&& f) {
   return with_type(dtype, [&](auto e) {
-    switch (scan_lanes(N)) {
+    switch (lanes) {
       case 1: return f(e, std::integral_constant<int, 1>{});
       case 2: return f(e, std::integral_constant<int, 2>{});
       case 4: return f(e, std::integral_constant<int, 4>{});
-      case 8: return f(e, std::integral_constant<int, 8>{});
-      default: return f(e, std::integral_constant<int, 16>{});
+      default: return f(e, std::integral_constant<int, 8>{});
     }
   });
 }
@@ -167,14 +171,18 @@ int64_t scan_ckpts(int64_t T) { return (T + kScanCkpt - 1) / kScanCkpt; }
 
 // How a call is cut: CTAs of `channels` channels and segments of seg_len steps.
 struct ScanPlan {
-  int groups, cblocks, nseg, seg_len;
+  int cblocks, nseg, seg_len;
 };
-// Segments where the channels alone do not give `want` CTAs; a segment is a
-// multiple of kScanRows steps and at least kScanMinSegment of them.
+// Segments where the channels alone give fewer than two CTAs an SM: as many as make
+// `want` CTAs. A segment is a multiple of kScanRows steps and at least
+// kScanMinSegment of them. The first pass over the segments takes about half as long
+// as the scan, which pays only where SMs would idle: 128 channel blocks of 2000 steps
+// 308 us in one piece and 220 us in seven, 384 blocks of 1024 steps 245 us in one
+// piece and 320 us in two.
 ScanPlan scan_plan(int64_t B, int64_t T, int64_t C, int channels, int64_t want) {
-  ScanPlan p{1, (int)((C + channels - 1) / channels), 1, 0};
+  ScanPlan p{(int)((C + channels - 1) / channels), 1, 0};
   const int64_t sets = B * p.cblocks;
-  int64_t nseg = sets > 0 && sets < want ? (want + sets - 1) / sets : 1;
+  int64_t nseg = sets > 0 && sets < 2 * sm_count() ? (want + sets - 1) / sets : 1;
   nseg = std::max<int64_t>(1, std::min<int64_t>({nseg, T / kScanMinSegment, kScanMaxSegments}));
   const int64_t len = ((T + nseg - 1) / nseg + kScanRows - 1) / kScanRows * kScanRows;
   p.seg_len = (int)std::max<int64_t>(len, kScanRows);
@@ -182,15 +190,10 @@ ScanPlan scan_plan(int64_t B, int64_t T, int64_t C, int channels, int64_t want) 
   return p;
 }
 ScanPlan scan_forward_plan(int64_t B, int64_t T, int64_t C, int64_t N) {
-  return scan_plan(B, T, C, kScanThreads / scan_lanes(N), 4 * sm_count());
+  return scan_plan(B, T, C, kScanThreads / scan_lanes(N, 8), 6 * sm_count());
 }
 ScanPlan scan_backward_plan(int64_t B, int64_t T, int64_t C, int64_t N) {
-  const int lanes = scan_lanes(N), channels = kScanThreads / lanes;
-  int g = std::min(4, lanes);
-  while (g > 1 && B * ((C + g * channels - 1) / (g * channels)) < 2 * sm_count()) g /= 2;
-  ScanPlan p = scan_plan(B, T, C, g * channels, 2 * sm_count());
-  p.groups = g;
-  return p;
+  return scan_plan(B, T, C, kScanBwdPer * kScanBwdThreads / scan_lanes(N, 4), 2 * sm_count());
 }
 
 struct ScanWs {
@@ -219,25 +222,20 @@ ScanWs scan_ws(const ScanPlan& p, bool backward, int64_t B, int64_t T, int64_t C
   return w;
 }
 
-template <class E, int kLanesPer>
-constexpr size_t scan_bwd_smem_max() {
-  using L = ScanBwdSmem<E, kLanesPer>;
-  size_t most = 0;
-  for (int g = 1; g <= L::M; g *= 2) most = most < (size_t)L::bytes(g) ? (size_t)L::bytes(g) : most;
-  return most;
-}
-
 void scan_layout(ScanArgs& a, const ScanPlan& p, const ScanWs& w, int dtype, std::initializer_list<const void*> rows,
                  std::initializer_list<const void*> states) {
-  a.groups = p.groups;
   a.cblocks = p.cblocks;
   a.nseg = p.nseg;
   a.seg_len = p.seg_len;
   a.seg_h = w.seg_h;
   a.seg_d = w.seg_d;
   const int es = (int)dtype_size(dtype);
-  a.wide = a.C % 8 == 0 && vector_width(es, 16 / es, rows,
-                                        {a.x_sb, a.x_st, a.dt_sb, a.dt_st, a.z_sb, a.z_st, a.g_sb, a.g_st}) == 16 / es;
+  const int width =
+      vector_width(es, 16 / es, rows, {a.C, a.x_sb, a.x_st, a.dt_sb, a.dt_st, a.z_sb, a.z_st, a.g_sb, a.g_st});
+  a.wide = width == 16 / es;
+  a.pairs = width >= 2;
+  a.near = 1;
+  for (int64_t s : {a.x_st, a.dt_st, a.z_st, a.g_st, (int64_t)a.C}) a.near = a.near && s >= 0 && s < (1 << 25);
   a.wide_bc = a.N % 4 == 0 && vector_width(es, 4, {a.Bm, a.Cm}, {a.b_sb, a.b_st, a.c_sb, a.c_st}) == 4;
   a.wide_n = a.N % 4 == 0 && vector_width(4, 4, states, {}) == 4;
 }
@@ -405,7 +403,7 @@ int selective_scan_forward(int dtype, const void* x, const void* dt, const float
                 workspace_bytes);
   scan_layout(a, p, scan_ws(p, false, B, T, C, N, workspace), dtype, {x, dt, z, out}, {A, state_in, state_out, kept});
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return scan_dispatch(dtype, N, [&](auto e, auto lanes) {
+  return scan_dispatch(dtype, scan_lanes(N, 8), [&](auto e, auto lanes) {
     using E = decltype(e);
     constexpr int kLanesPer = decltype(lanes)::value;
     if (p.nseg > 1) {
@@ -482,26 +480,34 @@ int selective_scan_backward(int dtype, const void* grad_out, const void* x, cons
   scan_layout(a, p, ws, dtype, {grad_out, x, dt, z, grad_x, grad_dt, grad_z},
               {A, kept, grad_state_out, grad_state_in});
   if (B > 0) {
-    int rc = scan_dispatch(dtype, N, [&](auto e, auto lanes) {
-      using E = decltype(e);
-      constexpr int kLanesPer = decltype(lanes)::value;
-      if (p.nseg > 1) {
-        ScanArgs s = a;  // the summary kernel's channel blocks are one group wide
-        s.cblocks = (int)((C + kScanThreads / kLanesPer - 1) / (kScanThreads / kLanesPer));
+    int rc = WKV_OK;
+    if (p.nseg > 1) {
+      rc = scan_dispatch(dtype, scan_lanes(N, 8), [&](auto e, auto lanes) {
+        constexpr int kLanesPer = decltype(lanes)::value, kChannels = kScanThreads / kLanesPer;
+        ScanArgs s = a;
+        s.cblocks = (int)((C + kChannels - 1) / kChannels);
         launch(K_SCAN_ADJ, st, [&] {
-          scan_summary_kernel<E, kLanesPer, true>
+          scan_summary_kernel<decltype(e), kLanesPer, true>
               <<<(unsigned)(B * s.cblocks * (p.nseg - 1)), kScanThreads, 0, st>>>(s);
         });
-        if (int rc = launched("selective_scan adjoint launch")) return rc;
-      }
-      const cudaError_t err = allow_smem(scan_bwd_kernel<E, kLanesPer>, scan_bwd_smem_max<E, kLanesPer>());
+        return launched("selective_scan adjoint launch");
+      });
+      if (rc) return rc;
+    }
+    auto main = [&](auto e, auto lanes) {
+      using E = decltype(e);
+      constexpr int kLanesPer = decltype(lanes)::value;
+      const cudaError_t err = allow_smem(scan_bwd_kernel<E, kLanesPer>, ScanBwdSmem<E, kLanesPer>::kBytes);
       if (err != cudaSuccess) return cuda_fail(err, "setting the selective_scan backward kernel's shared memory size");
       launch(K_SCAN_BWD, st, [&] {
-        scan_bwd_kernel<E, kLanesPer><<<(unsigned)(B * p.cblocks * p.nseg), kScanThreads,
-                                        ScanBwdSmem<E, kLanesPer>::bytes(p.groups), st>>>(a);
+        scan_bwd_kernel<E, kLanesPer><<<(unsigned)(B * p.cblocks * p.nseg), kScanBwdThreads,
+                                        ScanBwdSmem<E, kLanesPer>::kBytes, st>>>(a);
       });
       return launched("selective_scan backward launch");
-    });
+    };
+    const int lanes = scan_lanes(N, 4);
+    rc = lanes == 16 ? with_type(dtype, [&](auto e) { return main(e, std::integral_constant<int, 16>{}); })
+                     : scan_dispatch(dtype, lanes, main);
     if (rc) return rc;
     const int64_t cells = B * T * 2 * N;
     if (cells > 0) {

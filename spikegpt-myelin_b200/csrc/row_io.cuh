@@ -81,7 +81,7 @@ struct Vec {
 };
 
 // 1 / (1 + e^-v); 0 and 1 at the infinities.
-__device__ __forceinline__ float sigmoid1(float v) { return __fdividef(1.f, 1.f + ex2(-v * kL2E)); }
+__device__ __forceinline__ float sigmoid1(float v) { return rcp(1.f + ex2(-v * kL2E)); }
 
 // Column sums of `rows` float32 rows of `blocks` groups of C columns, in row
 // order within each of 32 strides and then over the strides in order, so the

@@ -43,18 +43,40 @@ struct ScanArgs {
   int64_t x_sb, x_st, dt_sb, dt_st, z_sb, z_st, b_sb, b_st, c_sb, c_st, g_sb, g_st;
   int B, T, C, N;
   int nseg, seg_len, cblocks;
-  int groups;   // backward: channel groups of a CTA
   int wide;     // rows of x, dt, z, gout move as aligned 16-byte words
+  int pairs;    // two adjacent channels of every row move as one aligned word
+  int near;     // a tile's rows lie within 2^31 elements
   int wide_bc;  // four adjacent states of B and C move as one aligned word
   int wide_n;   // four adjacent float32 states move as one aligned word (N % 4 == 0)
   int softplus;
 };
 
-// softplus and its slope; log1p keeps the small values' relative accuracy.
-__device__ __forceinline__ float scan_delta(float v, int softplus) {
-  return softplus ? fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))) : v;
+// softplus(v) = max(v, 0) + log1p(u), u = e^-|v|. The exponent v log2(e) is split in
+// two floats so that u keeps float32's relative accuracy at large |v|, and log1p(u) =
+// 2 atanh(u / (2 + u)) is its power series: the argument is at most 1/3, so seven
+// terms leave 2e-8 of the value, small steps' relative accuracy included. About 17
+// instructions a value against about 45 for the library's exp and log1p, which took
+// as many issue slots as the scan itself.
+__device__ __forceinline__ f2 softplus2(f2 v) {
+  const f2 n{fmaxf(-fabsf(v.x), -100.f), fmaxf(-fabsf(v.y), -100.f)};
+  const f2 hi = mul2(n, splat(kL2E));
+  const f2 lo = fma2(n, splat(1.9259629911e-8f), fma2(n, splat(kL2E), f2{-hi.x, -hi.y}));  // log2(e) - kL2E
+  f2 u = ex2x2(hi);
+  u = fma2(mul2(u, splat(0.6931471806f)), lo, u);
+  const f2 s = mul2(u, rcpx2(add2(u, splat(2.f)))), w = mul2(s, s);
+  f2 p = fma2(w, splat(1.f / 13.f), splat(1.f / 11.f));
+  p = fma2(w, p, splat(1.f / 9.f));
+  p = fma2(w, p, splat(1.f / 7.f));
+  p = fma2(w, p, splat(1.f / 5.f));
+  p = fma2(w, p, splat(1.f / 3.f));
+  const f2 s2 = add2(s, s);
+  p = fma2(mul2(s2, w), p, s2);
+  return add2(f2{v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y}, p);  // a NaN stays one
 }
-__device__ __forceinline__ float scan_delta_slope(float v, int softplus) { return softplus ? sigmoid1(v) : 1.f; }
+__device__ __forceinline__ f2 scan_delta(f2 v, int softplus) { return softplus ? softplus2(v) : v; }
+__device__ __forceinline__ f2 sigmoid2(f2 v) {
+  return rcpx2(add2(ex2x2(mul2(v, splat(-kL2E))), splat(1.f)));
+}
 
 __device__ __forceinline__ int scan_length(const ScanArgs& a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
@@ -83,63 +105,97 @@ __device__ __forceinline__ void reduce_scatter(float* v) {
   }
 }
 
-// Four adjacent states of one channel, as two packed pairs.
-struct Quad {
-  f2 lo, hi;
+// kS adjacent states of one channel, as packed pairs.
+template <int kS>
+struct States {
+  f2 p[kS / 2];
+  __device__ __forceinline__ static States zero() {
+    States r;
+#pragma unroll
+    for (int i = 0; i < kS / 2; ++i) r.p[i] = f2{0.f, 0.f};
+    return r;
+  }
+  // states n .. n + kS - 1 of a row of N float32 states; past N: zeros. `wide`: four
+  // adjacent states move as one aligned word, and N is a multiple of 4.
+  __device__ __forceinline__ static States load(const float* row, int n, int N, int wide) {
+    States r;
+#pragma unroll
+    for (int i = 0; i < kS; i += 4) {
+      if (wide) {
+        const float4 v = n + i < N ? *reinterpret_cast<const float4*>(row + n + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        r.p[i / 2] = f2{v.x, v.y};
+        r.p[i / 2 + 1] = f2{v.z, v.w};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j += 2)
+          r.p[(i + j) / 2] = f2{n + i + j < N ? row[n + i + j] : 0.f, n + i + j + 1 < N ? row[n + i + j + 1] : 0.f};
+      }
+    }
+    return r;
+  }
+  __device__ __forceinline__ void store(float* row, int n, int N, int wide) const {
+#pragma unroll
+    for (int i = 0; i < kS; i += 4) {
+      const f2 u = p[i / 2], v = p[i / 2 + 1];
+      if (wide) {
+        if (n + i < N) *reinterpret_cast<float4*>(row + n + i) = make_float4(u.x, u.y, v.x, v.y);
+      } else {
+        if (n + i < N) row[n + i] = u.x;
+        if (n + i + 1 < N) row[n + i + 1] = u.y;
+        if (n + i + 2 < N) row[n + i + 2] = v.x;
+        if (n + i + 3 < N) row[n + i + 3] = v.y;
+      }
+    }
+  }
+  // A row of B or C in shared memory.
+  __device__ __forceinline__ static States shared(const float* row) {
+    States r;
+#pragma unroll
+    for (int i = 0; i < kS; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(row + i);
+      r.p[i / 2] = f2{v.x, v.y};
+      r.p[i / 2 + 1] = f2{v.z, v.w};
+    }
+    return r;
+  }
+  __device__ __forceinline__ void scale(float k) {
+#pragma unroll
+    for (int i = 0; i < kS / 2; ++i) p[i] = mul2(p[i], splat(k));
+  }
 };
-__device__ __forceinline__ Quad quad(float4 v) { return Quad{f2{v.x, v.y}, f2{v.z, v.w}}; }
-__device__ __forceinline__ float4 quad4(Quad q) { return make_float4(q.lo.x, q.lo.y, q.hi.x, q.hi.y); }
-__device__ __forceinline__ Quad load_quad(const float* p, int n, int N, int wide) {
-  if (n >= N) return Quad{f2{0.f, 0.f}, f2{0.f, 0.f}};
-  if (wide) return quad(*reinterpret_cast<const float4*>(p + n));
-  return Quad{f2{p[n], n + 1 < N ? p[n + 1] : 0.f}, f2{n + 2 < N ? p[n + 2] : 0.f, n + 3 < N ? p[n + 3] : 0.f}};
+
+// Two adjacent channels of one row; `live` false or channels past C: zeros. `pairs`:
+// the rows allow a word for both.
+template <typename T>
+__device__ __forceinline__ Vec<T, 2> load_pair(const T* row, int c, int C, bool live, int pairs) {
+  Vec<T, 2> r = Vec<T, 2>::zero();
+  if (!live || c >= C) return r;
+  if (pairs) return Vec<T, 2>::load(row + c);
+  r.e[0] = row[c];
+  if (c + 1 < C) r.e[1] = row[c + 1];
+  return r;
 }
-__device__ __forceinline__ void store_quad(float* p, int n, int N, int wide, Quad q) {
-  if (n >= N) return;
-  if (wide) {
-    *reinterpret_cast<float4*>(p + n) = quad4(q);
+template <typename T>
+__device__ __forceinline__ void store_pair(T* row, int c, int C, int pairs, f2 v) {
+  if (c >= C) return;
+  Vec<T, 2> r;
+  r.set({v.x, v.y});
+  if (pairs) {
+    r.store(row + c);
     return;
   }
-  p[n] = q.lo.x;
-  if (n + 1 < N) p[n + 1] = q.lo.y;
-  if (n + 2 < N) p[n + 2] = q.hi.x;
-  if (n + 3 < N) p[n + 3] = q.hi.y;
+  row[c] = r.e[0];
+  if (c + 1 < C) row[c + 1] = r.e[1];
 }
-// exp(d A) of four states: A2 is A log2(e).
-__device__ __forceinline__ Quad decay(Quad A2, f2 d) { return Quad{ex2x2(mul2(A2.lo, d)), ex2x2(mul2(A2.hi, d))}; }
-
-// Eight adjacent channels of one row; `live` false or channels past C: zeros.
 template <typename T>
-struct Eight {
-  alignas(16) T e[8];
-  __device__ __forceinline__ void load(const T* row, int c, int C, bool live, int wide) {
-    uint4* w = reinterpret_cast<uint4*>(e);
-    if (wide) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        w[i] = live && c < C ? reinterpret_cast<const uint4*>(row + c)[i] : make_uint4(0, 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = live && c + i < C ? row[c + i] : Pair<T>::from_float(0.f);
-    }
-  }
-  __device__ __forceinline__ void store(T* row, int c, int C, int wide) const {
-    if (wide) {
-      const uint4* w = reinterpret_cast<const uint4*>(e);
-      if (c < C)
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(row + c)[i] = w[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < C) row[c + i] = e[i];
-    }
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Pair<T>::scalar(e[i]);
-  }
-};
+__device__ __forceinline__ f2 pair_of(const Vec<T, 2>& r) {
+  float f[2];
+  r.get(f);
+  return f2{f[0], f[1]};
+}
+__device__ __forceinline__ f2 param_pair(const float* p, int c, int C) {
+  return f2{p && c < C ? p[c] : 0.f, p && c + 1 < C ? p[c + 1] : 0.f};
+}
 
 // Four adjacent states of a row of B or C; past N: zeros.
 template <typename T>
@@ -153,126 +209,167 @@ __device__ __forceinline__ Vec<T, 4> load_bc(const T* row, int n, int N, bool li
   return r;
 }
 
-// The layout of a CTA's work, by the lanes that share a channel (four states each).
-template <int LPC>
+// The layout of a CTA's work, by the lanes that share a channel and the states of
+// a lane. A thread stages pairs of channels: always the same pair, of every kStep-th
+// row.
+template <int LPC, int kS, int kThr, int kTT, int kPer = 1>
 struct ScanShape {
-  static constexpr int NP = 4 * LPC;               // states, padded
-  static constexpr int CH = kScanThreads / LPC;    // channels of a CTA (of a group in the backward)
-  static constexpr int TT = LPC < 4 ? 8 * LPC : kScanRows;  // steps of a staged tile: TT * CH <= 1024
-  static constexpr int VPR = CH / 8;               // eights of a row
+  static constexpr int NP = kS * LPC;           // states, padded
+  static constexpr int CH = kThr / LPC * kPer;  // channels of a CTA, kPer of them a lane group's
+  static constexpr int TT = kTT;         // steps of a staged tile
+  static constexpr int kPairs = CH / 2;
+  static constexpr int kStep = kThr / kPairs;
+  static constexpr int kRows = TT < kStep ? 1 : TT / kStep;
+  static constexpr bool kIdle = TT < kStep;  // threads of the rows past the tile stage nothing
+  static_assert(kIdle || kRows * kStep == TT, "whole rows a thread");
 };
+
+// The forward's and the summaries': eight states a lane (half the instructions of
+// four a lane for the reads of d, d x and the exchange of y), 1024 cells a tile.
+template <int LPC>
+using FwdShape = ScanShape<LPC, 8, kScanThreads, 8 * LPC < kScanRows ? 8 * LPC : kScanRows>;
 
 // The state a segment starts from: the earlier segments' contributions in order
 // (forward), or the adjoint that the later segments hand back.
-__device__ __forceinline__ Quad scan_carry(const ScanArgs& a, int b, int c, int n, Quad h, Quad A2, int from, int to,
-                                           int step) {
+template <int kS>
+__device__ __forceinline__ States<kS> scan_carry(const ScanArgs& a, int b, int c, int n, States<kS> h,
+                                                 const States<kS>& A2, int from, int to, int step) {
   for (int s = from; s != to; s += step) {
     const int64_t at = ((int64_t)b * a.nseg + s) * a.C + c;
-    const Quad add = load_quad(a.seg_h + at * a.N, n, a.N, a.wide_n);
-    const Quad e = decay(A2, splat(a.seg_d[at]));
-    h.lo = fma2(e.lo, h.lo, add.lo);
-    h.hi = fma2(e.hi, h.hi, add.hi);
+    const States<kS> add = States<kS>::load(a.seg_h + at * a.N, n, a.N, a.wide_n);
+    const f2 d = splat(a.seg_d[at]);
+#pragma unroll
+    for (int i = 0; i < kS / 2; ++i) h.p[i] = fma2(ex2x2(mul2(A2.p[i], d)), h.p[i], add.p[i]);
   }
   return h;
+}
+
+// Rows of one sequence as a thread stages them: its channel pair of kRows rows.
+// `plain`: the CTA's channels all exist, pairs move as words and offsets within a
+// tile fit 32 bits; a whole tile is then read without a test per row.
+template <typename T, class S>
+struct RowSource {
+  const T* base;  // channel 0 of row 0
+  int64_t pitch;
+  __device__ __forceinline__ void fetch(Vec<T, 2> (&to)[S::kRows], int t0, int row0, int cp, const ScanArgs& a, int t_end,
+                                        bool plain) const {
+    if (plain && t0 + S::TT <= t_end) {
+      const T* tile = base + t0 * pitch;
+      const uint32_t p = (uint32_t)pitch, at = row0 * p + cp;
+#pragma unroll
+      for (int k = 0; k < S::kRows; ++k) to[k] = Vec<T, 2>::load(tile + (at + k * S::kStep * p));
+    } else {
+#pragma unroll
+      for (int k = 0; k < S::kRows; ++k) {
+        const int t = t0 + row0 + k * S::kStep;
+        to[k] = load_pair(base + t * pitch, cp, a.C, t < t_end, a.pairs);
+      }
+    }
+  }
+};
+__device__ __forceinline__ bool scan_plain(const ScanArgs& a, int c_end) {
+  return a.pairs && a.near && c_end <= a.C;
 }
 
 // What a segment adds to a zero state (kAdjoint: to a zero adjoint, walking back:
 // g <- a (g + C gy)), and its sum of d: the decay across it is exp(A sum d).
 template <typename T, int LPC, bool kAdjoint>
 __global__ void __launch_bounds__(kScanThreads) scan_summary_kernel(ScanArgs a) {
-  using S = ScanShape<LPC>;
-  __shared__ float2 sdx[S::TT][S::CH];
+  using S = FwdShape<LPC>;
+  using St = States<8>;
+  __shared__ float4 sdx[S::TT][S::CH];  // d, d, w, w: pairs as the packed arithmetic reads them
   __shared__ __align__(16) float sn[S::TT][S::NP];
   // the last segment's sum serves no later one (the first's, walking back)
   const int cb = blockIdx.x % a.cblocks, seg = blockIdx.x / a.cblocks % (a.nseg - 1) + (kAdjoint ? 1 : 0);
   const int b = blockIdx.x / a.cblocks / (a.nseg - 1);
-  const int q = threadIdx.x % LPC, ch = threadIdx.x / LPC, c = cb * S::CH + ch;
+  const int q = threadIdx.x % LPC, ch = threadIdx.x / LPC, c0 = cb * S::CH, c = c0 + ch;
   const int t_begin = seg * a.seg_len, t_end = min(t_begin + a.seg_len, scan_length(a, b));
-  Quad A2 = load_quad(a.A + (int64_t)min(c, a.C - 1) * a.N, 4 * q, a.N, a.wide_n);
-  A2.lo = mul2(A2.lo, splat(kL2E));
-  A2.hi = mul2(A2.hi, splat(kL2E));
-  Quad h{f2{0.f, 0.f}, f2{0.f, 0.f}};
-  float dsum = 0.f;
-  const int row = threadIdx.x / S::VPR, vc = threadIdx.x % S::VPR * 8;
+  St A2 = St::load(a.A + (int64_t)min(c, a.C - 1) * a.N, 8 * q, a.N, a.wide_n);
+  A2.scale(kL2E);
+  St h = St::zero();
+  f2 dsum{0.f, 0.f};
+  const int row0 = threadIdx.x / S::kPairs, cp = c0 + threadIdx.x % S::kPairs * 2;
+  const bool plain = scan_plain(a, c0 + S::CH);
+  const f2 bias = param_pair(a.bias, cp, a.C);
+  const RowSource<T, S> px{static_cast<const T*>(kAdjoint ? a.gout : a.x) + b * (kAdjoint ? a.g_sb : a.x_sb),
+                           kAdjoint ? a.g_st : a.x_st};
+  const RowSource<T, S> pd{static_cast<const T*>(a.dt) + b * a.dt_sb, a.dt_st};
+  const RowSource<T, S> pz{static_cast<const T*>(a.z) + (a.z ? b * a.z_sb : 0), a.z_st};
+  const T* pn = static_cast<const T*>(kAdjoint ? a.Cm : a.Bm) + b * (kAdjoint ? a.c_sb : a.b_sb);
+  const int64_t sbc = kAdjoint ? a.c_st : a.b_st;
   const int tiles = t_end > t_begin ? (t_end - t_begin + S::TT - 1) / S::TT : 0;
-  float bias[8];
+  constexpr int kQ = S::NP / 4, kN = (S::TT * kQ + kScanThreads - 1) / kScanThreads;
+  Vec<T, 2> rx[S::kRows], rd[S::kRows], rz[S::kRows];
+  Vec<T, 4> rn[kN];
+  auto fetch = [&](int t0) {
+    px.fetch(rx, t0, row0, cp, a, t_end, plain);
+    pd.fetch(rd, t0, row0, cp, a, t_end, plain);
+    if (kAdjoint && a.z) pz.fetch(rz, t0, row0, cp, a, t_end, plain);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) bias[i] = a.bias && cb * S::CH + vc + i < a.C ? a.bias[cb * S::CH + vc + i] : 0.f;
-  for (int k = 0; k < tiles; ++k) {
-    const int t0 = t_begin + (kAdjoint ? tiles - 1 - k : k) * S::TT;
-    if (row < S::TT) {
-      const int t = t0 + row;
-      const bool live = t < t_end;
-      Eight<T> r;
-      float f[8], d[8], w[8];
-      r.load(static_cast<const T*>(a.dt) + b * a.dt_sb + (int64_t)t * a.dt_st + cb * S::CH, vc, a.C - cb * S::CH, live,
-             a.wide);
-      r.get(f);
+    for (int k = 0; k < kN; ++k) {
+      const int i = k * kScanThreads + threadIdx.x, t = t0 + i / kQ;
+      rn[k] = load_bc(pn + (int64_t)t * sbc, i % kQ * 4, a.N, i < S::TT * kQ && t < t_end, a.wide_bc);
+    }
+  };
+  if (tiles > 0) fetch(t_begin + (kAdjoint ? tiles - 1 : 0) * S::TT);
+  for (int tile = 0; tile < tiles; ++tile) {
+    const int t0 = t_begin + (kAdjoint ? tiles - 1 - tile : tile) * S::TT;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] = live ? scan_delta(f[i] + bias[i], a.softplus) : 0.f;
+    for (int k = 0; k < S::kRows; ++k) {
+      const int r = row0 + k * S::kStep;
+      f2 d = scan_delta(add2(pair_of(rd[k]), bias), a.softplus), w = pair_of(rx[k]);
+      if (t0 + r >= t_end) d = f2{0.f, 0.f};
       if constexpr (kAdjoint) {
-        r.load(static_cast<const T*>(a.gout) + b * a.g_sb + (int64_t)t * a.g_st + cb * S::CH, vc, a.C - cb * S::CH,
-               live, a.wide);
-        r.get(w);
         if (a.z) {
-          r.load(static_cast<const T*>(a.z) + b * a.z_sb + (int64_t)t * a.z_st + cb * S::CH, vc, a.C - cb * S::CH, live,
-                 a.wide);
-          r.get(f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] *= f[i] * sigmoid1(f[i]);
+          const f2 z = pair_of(rz[k]);
+          w = mul2(w, mul2(z, sigmoid2(z)));
         }
       } else {
-        r.load(static_cast<const T*>(a.x) + b * a.x_sb + (int64_t)t * a.x_st + cb * S::CH, vc, a.C - cb * S::CH, live,
-               a.wide);
-        r.get(f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = d[i] * f[i];
+        w = mul2(d, w);
       }
-#pragma unroll
-      for (int i = 0; i < 8; i += 2)
-        *reinterpret_cast<float4*>(&sdx[row][vc + i]) = make_float4(d[i], w[i], d[i + 1], w[i + 1]);
+      sdx[r][cp - c0] = make_float4(d.x, d.x, w.x, w.x);
+      sdx[r][cp - c0 + 1] = make_float4(d.y, d.y, w.y, w.y);
     }
-    for (int i = threadIdx.x; i < S::TT * LPC; i += kScanThreads) {
-      const int t = t0 + i / LPC, n = i % LPC * 4;
-      const T* p = kAdjoint ? static_cast<const T*>(a.Cm) + b * a.c_sb + (int64_t)t * a.c_st
-                            : static_cast<const T*>(a.Bm) + b * a.b_sb + (int64_t)t * a.b_st;
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      const int i = k * kScanThreads + threadIdx.x;
       float f[4];
-      load_bc(p, n, a.N, t < t_end, a.wide_bc).get(f);
-      *reinterpret_cast<float4*>(&sn[i / LPC][n]) = make_float4(f[0], f[1], f[2], f[3]);
+      rn[k].get(f);
+      if (i < S::TT * kQ) *reinterpret_cast<float4*>(&sn[i / kQ][i % kQ * 4]) = make_float4(f[0], f[1], f[2], f[3]);
     }
     __syncthreads();
-#pragma unroll 8
+    if (tile + 1 < tiles) fetch(t0 + (kAdjoint ? -S::TT : S::TT));
+#pragma unroll 4
     for (int j = 0; j < S::TT; ++j) {
       const int i = kAdjoint ? S::TT - 1 - j : j;
-      const float2 s = sdx[i][ch];
-      const Quad v = quad(*reinterpret_cast<const float4*>(&sn[i][4 * q]));
-      const Quad e = decay(A2, splat(s.x));
-      if constexpr (kAdjoint) {
-        h.lo = mul2(e.lo, fma2(v.lo, splat(s.y), h.lo));
-        h.hi = mul2(e.hi, fma2(v.hi, splat(s.y), h.hi));
-      } else {
-        h.lo = fma2(e.lo, h.lo, mul2(v.lo, splat(s.y)));
-        h.hi = fma2(e.hi, h.hi, mul2(v.hi, splat(s.y)));
+      const float4 s = sdx[i][ch];
+      const f2 d{s.x, s.y}, w{s.z, s.w};
+      const St v = St::shared(&sn[i][8 * q]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const f2 e = ex2x2(mul2(A2.p[n], d));
+        h.p[n] = kAdjoint ? mul2(e, fma2(v.p[n], w, h.p[n])) : fma2(e, h.p[n], mul2(v.p[n], w));
       }
-      dsum += s.x;
+      dsum = add2(dsum, d);
     }
     __syncthreads();
   }
   if (c >= a.C) return;
   const int64_t at = ((int64_t)b * a.nseg + seg) * a.C + c;
-  store_quad(a.seg_h + at * a.N, 4 * q, a.N, a.wide_n, h);
-  if (q == 0) a.seg_d[at] = dsum;
+  h.store(a.seg_h + at * a.N, 8 * q, a.N, a.wide_n);
+  if (q == 0) a.seg_d[at] = dsum.x;
 }
 
 // A CTA walks one segment of CH channels of one sequence; LPC lanes share a
-// channel, four states each. Tiles of TT steps are staged: d and d x of every
+// channel, eight states each. Tiles of TT steps are staged: d and d x of every
 // (step, channel) and B, C in float32, while the next tile's raw rows are already
 // under way to registers. The lanes' parts of y are summed by an exchange of four
 // steps at a time, and the gate and the output are done by whole rows again.
 template <typename T, int LPC>
 __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(ScanArgs a) {
-  using S = ScanShape<LPC>;
-  __shared__ float2 sdx[S::TT][S::CH];
+  using S = FwdShape<LPC>;
+  using St = States<8>;
+  __shared__ float4 sdx[S::TT][S::CH];  // d, d, d x, d x: pairs as the packed arithmetic reads them
   __shared__ __align__(16) float sbc[S::TT][2 * S::NP];
   __shared__ __align__(16) float sy[S::TT][S::CH + 8];
   const int cb = blockIdx.x % a.cblocks, seg = blockIdx.x / a.cblocks % a.nseg, b = blockIdx.x / a.cblocks / a.nseg;
@@ -281,75 +378,79 @@ __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(ScanArgs a) {
   const int t_begin = seg * a.seg_len, t_end = min(t_begin + a.seg_len, a.T), t_live = min(t_end, len);
   const int64_t hc = ((int64_t)b * a.C + c) * a.N;
   const bool mine = c < a.C;
-  Quad A2 = load_quad(a.A + (int64_t)min(c, a.C - 1) * a.N, 4 * q, a.N, a.wide_n);
-  A2.lo = mul2(A2.lo, splat(kL2E));
-  A2.hi = mul2(A2.hi, splat(kL2E));
-  Quad h{f2{0.f, 0.f}, f2{0.f, 0.f}};
-  if (mine && a.h0) h = load_quad(a.h0 + hc, 4 * q, a.N, a.wide_n);
-  if (mine) h = scan_carry(a, b, c, 4 * q, h, A2, 0, seg, 1);
+  St A2 = St::load(a.A + (int64_t)min(c, a.C - 1) * a.N, 8 * q, a.N, a.wide_n);
+  A2.scale(kL2E);
+  St h = St::zero();
+  if (mine && a.h0) h = St::load(a.h0 + hc, 8 * q, a.N, a.wide_n);
+  if (mine) h = scan_carry(a, b, c, 8 * q, h, A2, 0, seg, 1);
 
-  const int row = threadIdx.x / S::VPR, vc = threadIdx.x % S::VPR * 8;
-  const bool stager = row < S::TT;
-  constexpr int kBC = (S::TT * 2 * LPC + kScanThreads - 1) / kScanThreads;
-  Eight<T> rx, rd, rz;
+  const int row0 = threadIdx.x / S::kPairs, cp = c0 + threadIdx.x % S::kPairs * 2;
+  const bool plain = scan_plain(a, c0 + S::CH);
+  const f2 bias = param_pair(a.bias, cp, a.C), D = param_pair(a.D, cp, a.C);
+  const RowSource<T, S> px{static_cast<const T*>(a.x) + b * a.x_sb, a.x_st};
+  const RowSource<T, S> pd{static_cast<const T*>(a.dt) + b * a.dt_sb, a.dt_st};
+  const RowSource<T, S> pz{static_cast<const T*>(a.z) + (a.z ? b * a.z_sb : 0), a.z_st};
+  constexpr int kQ = S::NP / 4, kBC = (S::TT * 2 * kQ + kScanThreads - 1) / kScanThreads;
+  Vec<T, 2> rx[S::kRows], rd[S::kRows], rz[S::kRows];
   Vec<T, 4> rbc[kBC];
   auto fetch = [&](int t0) {
-    const int t = t0 + row;
-    const bool live = stager && t < t_live;
-    rx.load(static_cast<const T*>(a.x) + b * a.x_sb + (int64_t)t * a.x_st + c0, vc, a.C - c0, live, a.wide);
-    rd.load(static_cast<const T*>(a.dt) + b * a.dt_sb + (int64_t)t * a.dt_st + c0, vc, a.C - c0, live, a.wide);
-    if (a.z)
-      rz.load(static_cast<const T*>(a.z) + b * a.z_sb + (int64_t)t * a.z_st + c0, vc, a.C - c0, live, a.wide);
+    px.fetch(rx, t0, row0, cp, a, t_live, plain);
+    pd.fetch(rd, t0, row0, cp, a, t_live, plain);
+    if (a.z) pz.fetch(rz, t0, row0, cp, a, t_live, plain);
 #pragma unroll
     for (int k = 0; k < kBC; ++k) {
-      const int i = k * kScanThreads + threadIdx.x, tb = t0 + i / (2 * LPC), n = i % LPC * 4;
-      const bool on = i < S::TT * 2 * LPC && tb < t_live;
-      const T* p = i % (2 * LPC) < LPC ? static_cast<const T*>(a.Bm) + b * a.b_sb + (int64_t)tb * a.b_st
-                                       : static_cast<const T*>(a.Cm) + b * a.c_sb + (int64_t)tb * a.c_st;
+      const int i = k * kScanThreads + threadIdx.x, tb = t0 + i / (2 * kQ), n = i % kQ * 4;
+      const bool on = i < S::TT * 2 * kQ && tb < t_live;
+      const T* p = i % (2 * kQ) < kQ ? static_cast<const T*>(a.Bm) + b * a.b_sb + (int64_t)tb * a.b_st
+                                     : static_cast<const T*>(a.Cm) + b * a.c_sb + (int64_t)tb * a.c_st;
       rbc[k] = load_bc(p, n, a.N, on, a.wide_bc);
     }
   };
   const int nck = (a.T + kScanCkpt - 1) / kScanCkpt;
+  float* ckpt = a.ckpt && mine ? a.ckpt + ((int64_t)b * nck * a.C + c) * a.N : nullptr;
+  T* out = static_cast<T*>(a.out) + (int64_t)b * a.T * a.C;
   if (t_begin < t_live) fetch(t_begin);
   for (int t0 = t_begin; t0 < t_live; t0 += S::TT) {
-    const Eight<T> cx = rx, cz = rz;
-    if (stager) {
-      float f[8], d[8];
-      rd.get(d);
-      rx.get(f);
-      const bool live = t0 + row < t_live;
+    Vec<T, 2> cx[S::kRows], cz[S::kRows];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        d[i] = live ? scan_delta(d[i] + (a.bias && c0 + vc + i < a.C ? a.bias[c0 + vc + i] : 0.f), a.softplus) : 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; i += 2)
-        *reinterpret_cast<float4*>(&sdx[row][vc + i]) = make_float4(d[i], d[i] * f[i], d[i + 1], d[i + 1] * f[i + 1]);
+    for (int k = 0; k < S::kRows; ++k) {
+      const int r = row0 + k * S::kStep;
+      cx[k] = rx[k];
+      cz[k] = rz[k];
+      f2 d = scan_delta(add2(pair_of(rd[k]), bias), a.softplus);
+      if (t0 + r >= t_live) d = f2{0.f, 0.f};
+      const f2 w = mul2(d, pair_of(rx[k]));
+      sdx[r][cp - c0] = make_float4(d.x, d.x, w.x, w.x);
+      sdx[r][cp - c0 + 1] = make_float4(d.y, d.y, w.y, w.y);
     }
 #pragma unroll
     for (int k = 0; k < kBC; ++k) {
       const int i = k * kScanThreads + threadIdx.x;
       float f[4];
       rbc[k].get(f);
-      if (i < S::TT * 2 * LPC)
-        *reinterpret_cast<float4*>(&sbc[i / (2 * LPC)][i % (2 * LPC) * 4]) = make_float4(f[0], f[1], f[2], f[3]);
+      if (i < S::TT * 2 * kQ)
+        *reinterpret_cast<float4*>(&sbc[i / (2 * kQ)][i % (2 * kQ) * 4]) = make_float4(f[0], f[1], f[2], f[3]);
     }
     __syncthreads();
     if (t0 + S::TT < t_live) fetch(t0 + S::TT);
 #pragma unroll 2
     for (int j = 0; j < S::TT; j += 4) {
-      if (j % kScanCkpt == 0 && a.ckpt && mine && t0 + j < t_live)
-        store_quad(a.ckpt + (((int64_t)b * nck + (t0 + j) / kScanCkpt) * a.C + c) * a.N, 4 * q, a.N, a.wide_n, h);
+      if (j % kScanCkpt == 0 && ckpt && t0 + j < t_live)
+        h.store(ckpt + (int64_t)((t0 + j) / kScanCkpt) * a.C * a.N, 8 * q, a.N, a.wide_n);
       float y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 s = sdx[j + i][ch];
-        const Quad Bt = quad(*reinterpret_cast<const float4*>(&sbc[j + i][4 * q]));
-        const Quad Ct = quad(*reinterpret_cast<const float4*>(&sbc[j + i][S::NP + 4 * q]));
-        const Quad e = decay(A2, splat(s.x));
-        h.lo = fma2(e.lo, h.lo, mul2(Bt.lo, splat(s.y)));
-        h.hi = fma2(e.hi, h.hi, mul2(Bt.hi, splat(s.y)));
-        const f2 p = fma2(h.hi, Ct.hi, mul2(h.lo, Ct.lo));
-        y[i] = p.x + p.y;
+        const float4 s = sdx[j + i][ch];
+        const f2 d{s.x, s.y}, w{s.z, s.w};
+        const St Bt = St::shared(&sbc[j + i][8 * q]), Ct = St::shared(&sbc[j + i][S::NP + 8 * q]);
+        f2 v[2];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          h.p[n] = fma2(ex2x2(mul2(A2.p[n], d)), h.p[n], mul2(Bt.p[n], w));
+          v[n % 2] = n < 2 ? mul2(h.p[n], Ct.p[n]) : fma2(h.p[n], Ct.p[n], v[n % 2]);
+        }
+        const f2 u = add2(v[0], v[1]);
+        y[i] = u.x + u.y;
       }
       reduce_scatter<4, LPC, 1>(y);
       if constexpr (LPC <= 4) {
@@ -360,26 +461,32 @@ __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(ScanArgs a) {
       }
     }
     __syncthreads();
-    if (stager && t0 + row < t_live) {
-      float f[8], y[8], z[8];
-      cx.get(f);
-      cz.get(z);
-      Eight<T> o;
+    const bool whole = plain && t0 + S::TT <= t_live;
+    T* tile = out + (int64_t)t0 * a.C;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        y[i] = fmaf(a.D && c0 + vc + i < a.C ? a.D[c0 + vc + i] : 0.f, f[i], sy[row][vc + i]);
-        if (a.z) y[i] *= z[i] * sigmoid1(z[i]);
-        o.e[i] = Pair<T>::from_float(y[i]);
+    for (int k = 0; k < S::kRows; ++k) {
+      const int r = row0 + k * S::kStep;
+      const float2 v = *reinterpret_cast<const float2*>(&sy[r][cp - c0]);
+      f2 y = fma2(D, pair_of(cx[k]), f2{v.x, v.y});
+      if (a.z) {
+        const f2 z = pair_of(cz[k]);
+        y = mul2(y, mul2(z, sigmoid2(z)));
       }
-      o.store(static_cast<T*>(a.out) + ((int64_t)b * a.T + t0 + row) * a.C + c0, vc, a.C - c0, a.wide);
+      if (whole) {
+        Vec<T, 2> o;
+        o.set({y.x, y.y});
+        o.store(tile + (r * (uint32_t)a.C + cp));
+      } else if (t0 + r < t_live) {
+        store_pair(tile + (int64_t)r * a.C, cp, a.C, a.pairs, y);
+      }
     }
   }
   // the rows past the sequence's length
   for (int i = threadIdx.x; i < (t_end - max(t_begin, t_live)) * S::CH; i += kScanThreads) {
     const int t = max(t_begin, t_live) + i / S::CH, k = c0 + i % S::CH;
-    if (k < a.C) static_cast<T*>(a.out)[((int64_t)b * a.T + t) * a.C + k] = Pair<T>::from_float(0.f);
+    if (k < a.C) out[(int64_t)t * a.C + k] = Pair<T>::from_float(0.f);
   }
-  if (a.h_last && mine && seg == a.nseg - 1) store_quad(a.h_last + hc, 4 * q, a.N, a.wide_n, h);
+  if (a.h_last && mine && seg == a.nseg - 1) h.store(a.h_last + hc, 8 * q, a.N, a.wide_n);
 }
 
 __device__ __forceinline__ void copy16(void* dst, const void* src, bool on) {
@@ -387,158 +494,245 @@ __device__ __forceinline__ void copy16(void* dst, const void* src, bool on) {
                : "memory");
 }
 
-// Shared memory of the backward kernel (see there), in bytes from the start.
-template <typename T, int LPC>
-struct ScanBwdSmem {
-  using S = ScanShape<LPC>;
-  static constexpr int M = LPC < 4 ? LPC : 4;     // groups x sub-chunks of a tile
-  static constexpr int kCells = 8 * M * S::CH;    // (step, channel) pairs of a tile, <= 1024
-  static constexpr int kRaw = kCells * 16;                        // after the slots, float4 [kCells]: T [2][4][kCells]
-  static constexpr int kBC = kRaw + 8 * kCells * (int)sizeof(T);  // float [8 subs][2 NP]
-  static constexpr int kSub = 8 * 2 * S::NP * 4 * 5;              // bytes a sub-chunk: its B, C, and a partial row a warp
-  // float [subs][4 warps][8][2 NP], then float4 [3][groups][threads]: A log2 e, adjoint, gA
-  static constexpr int bytes(int groups) { return kBC + M / groups * kSub + 3 * groups * kScanThreads * 16; }
+// D += A B for one m16n8k8 tile of tf32 factors with float32 sums.
+__device__ __forceinline__ void mma_tf32(float (&d)[4], float a0, float a1, float a2, float a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)),
+        "r"(b0), "r"(b1));
+}
+// Sums over a warp's channels with the tensor core. The lanes of a channel sit
+// 32 / LPC apart, so the four lanes of a tile's k group are channels of one state
+// quad (LPC = 16: two channels of two quads), and a column is one lane group. A pair
+// of values is a B operand as it lies in its two registers; the A operand is a 0/1
+// matrix that adds value r of four into row 2 r (LPC = 16: the second quad's into row
+// 2 r + 1). Two A operands serve both accumulators, gB's and gC's, because the rows
+// from 8 on may hold anything: they get value r in row 2 r + 9. Shuffles take 28
+// instructions a step for these sums, this 20.
+//
+// A term enters as the sum of two tf32 values, its upper 11 bits and the rest, which
+// keeps 21 bits and more of it (rounded once to 11 bits, a sum that cancels would lose
+// more than the result's own rounding to bfloat16 does). A term that is infinite or
+// NaN makes the neighbouring rows of its tile NaN.
+template <int LPC>
+struct ChannelSums {
+  float sel[8];  // two A operands: for the values 0, 1 and for 2, 3
+
+  __device__ __forceinline__ void init() {
+    const int row = threadIdx.x % 32 / 4, odd = threadIdx.x / 2 % 2;  // LPC = 16: the quad of the lane's k
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      sel[r] = row == (LPC == 16 ? r / 2 * 2 + odd : r) ? 1.f : 0.f;
+      asm volatile("" : "+f"(sel[r]));  // stays in its register: rebuilding an operand costs more than its product
+    }
+  }
+  // adds the four values of a step to a tile
+  __device__ __forceinline__ void add(float (&d)[4], f2 v, f2 w) const {
+    const f2 vh{__uint_as_float(__float_as_uint(v.x) & 0xffffe000u), __uint_as_float(__float_as_uint(v.y) & 0xffffe000u)};
+    const f2 wh{__uint_as_float(__float_as_uint(w.x) & 0xffffe000u), __uint_as_float(__float_as_uint(w.y) & 0xffffe000u)};
+    const f2 vl = sub2(v, vh), wl = sub2(w, wh);
+    mma_tf32(d, sel[0], sel[1], sel[2], sel[3], __float_as_uint(vh.x), __float_as_uint(vh.y));
+    mma_tf32(d, sel[4], sel[5], sel[6], sel[7], __float_as_uint(wh.x), __float_as_uint(wh.y));
+    mma_tf32(d, sel[0], sel[1], sel[2], sel[3], __float_as_uint(vl.x), __float_as_uint(vl.y));
+    mma_tf32(d, sel[4], sel[5], sel[6], sel[7], __float_as_uint(wl.x), __float_as_uint(wl.y));
+  }
+  // to[B: 0 .. NP, C: NP .. 2 NP): the warp's sums of a step
+  __device__ __forceinline__ void store(const float (&dB)[4], const float (&dC)[4], float* to) const {
+    constexpr int NP = 4 * LPC;
+    const int row = threadIdx.x % 32 / 4, j = threadIdx.x % 4;
+    if constexpr (LPC == 16) {  // columns 2 j and 2 j + 1: the quads' pairs
+      to += row / 2 + 4 * (4 * j + row % 2);
+      to[0] = dB[0];
+      to[8] = dB[1];
+      to[NP] = dC[0];
+      to[NP + 8] = dC[1];
+    } else {  // even rows hold gB's values, odd ones (from row 9 on) gC's
+      to += (row % 2) * NP + row / 2;
+      const float u0 = row % 2 ? dC[2] : dB[0], u1 = row % 2 ? dC[3] : dB[1];
+      if constexpr (LPC == 8) {  // columns: quads
+        to[4 * (2 * j)] = u0;
+        to[4 * (2 * j + 1)] = u1;
+      } else {  // columns: 8 / LPC lane groups of each quad
+        float u = u0 + u1;
+#pragma unroll
+        for (int m = 1; m < 4 / LPC; m *= 2) u += __shfl_xor_sync(kFull, u, m);
+        if (j % (4 / LPC) == 0) to[4 * (j / (4 / LPC))] = u;
+      }
+    }
+  }
 };
 
-// A CTA walks one segment of `groups` x CH channels of one sequence backwards, in
-// tiles of 8 * (M / groups) steps. Per sub-chunk of 8 steps and group of CH
-// channels, a thread runs its channel's four states forward from the kept state,
-// with a_t and p_t = a_t h_{t-1} in registers, and then back with the adjoint. The
-// sums over states (for gx, gdt, gz) are exchanged among the channel's lanes; the
-// sums over channels (gB, gC) gather in registers over the groups, are exchanged
-// once for all of them, then added over the warps and left as one partial row of
-// the CTA's channels.
+// Shared memory of the backward kernel (see there), in bytes from the start.
+constexpr int kScanBwdThreads = 128;
+constexpr int kScanBwdPer = 2;  // channels of a thread
 template <typename T, int LPC>
-__global__ void __launch_bounds__(kScanThreads, LPC <= 4 ? 3 : 2) scan_bwd_kernel(ScanArgs a) {
-  using S = ScanShape<LPC>;
+struct ScanBwdSmem {
+  using S = ScanShape<LPC, 4, kScanBwdThreads, LPC == 1 ? 8 : 16, kScanBwdPer>;
+  static constexpr int kWarps = kScanBwdThreads / 32;
+  static constexpr int TS = S::TT;              // steps of a tile
+  static constexpr int kCells = TS * S::CH;     // (step, channel) pairs of a tile
+  static constexpr int kPitch = S::CH + 8;
+  static constexpr int kGy = kCells * 16;       // after d, d, d x, d x (float4 [kCells]): gy, gy (float2 [kCells])
+  static constexpr int kRaw = kGy + kCells * 8;                      // T [2][4][kCells]
+  static constexpr int kBC = kRaw + 8 * kCells * (int)sizeof(T);     // float [TS][2 NP]
+  static constexpr int kRes = kBC + TS * 2 * S::NP * 4;              // float [3][TS][kPitch]
+  static constexpr int kPart = kRes + 3 * TS * kPitch * 4;           // float [TS][warps][2 NP]
+  static constexpr int kBytes = kPart + TS * kWarps * 2 * S::NP * 4;
+};
+
+// A CTA walks one segment of CH channels of one sequence backwards, in tiles of TS
+// steps. Per sub-chunk of 8 steps a thread runs four states of its two channels
+// forward from the kept states, with p_t = a_t h_{t-1} in registers, and then back
+// with the adjoint (a_t again from the exponential unit, which has the time: held in
+// registers it would cost a quarter of the resident warps). The sums over states (for gx, gdt, gz) are exchanged among the
+// channel's lanes, the sums over channels (gB, gC) go through the tensor core, are
+// added over the warps and left as one partial row of the CTA's channels.
+template <typename T, int LPC>
+__global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a) {
   using L = ScanBwdSmem<T, LPC>;
+  using S = typename L::S;
+  using St = States<4>;
+  constexpr int NP = S::NP, CH = S::CH, TS = L::TS, kCells = L::kCells, kThr = kScanBwdThreads, kLane = 32 / LPC;
+  constexpr int kPer = kScanBwdPer;
   extern __shared__ __align__(16) char smem[];
-  constexpr int NP = S::NP, CH = S::CH, M = L::M, kCells = L::kCells;
-  const int G = a.groups, subs = M / G, TS = 8 * subs, CHB = CH * G;
-  float4* slot = reinterpret_cast<float4*>(smem);
-  T* raw = reinterpret_cast<T*>(smem + L::kRaw);
+  float4* slot = reinterpret_cast<float4*>(smem);             // d, d, d x, d x of a cell
+  float2* sgy = reinterpret_cast<float2*>(smem + L::kGy);     // gy, gy
+  T* raw = reinterpret_cast<T*>(smem + L::kRaw);              // x, dt, gout, z of this tile and the next
   float* sbc = reinterpret_cast<float*>(smem + L::kBC);
-  float* part = sbc + TS * 2 * NP;
-  float4* sgrp = reinterpret_cast<float4*>(part + subs * 4 * 8 * 2 * NP);
-  const int tid = threadIdx.x, q = tid % LPC, ch = tid / LPC, warp = tid / 32;
+  float* res = reinterpret_cast<float*>(smem + L::kRes);      // sum g B, sum A g p log2(e), sum C h of a cell
+  float* part = reinterpret_cast<float*>(smem + L::kPart);
+  const int tid = threadIdx.x, warp = tid / 32, q = tid % 32 / kLane, ch = warp * kLane * kPer + tid % kLane;
   const int cb = blockIdx.x % a.cblocks, seg = blockIdx.x / a.cblocks % a.nseg, b = blockIdx.x / a.cblocks / a.nseg;
-  const int c0 = cb * CHB;
+  const int c0 = cb * CH, c = c0 + ch;  // and c + kLane
   const int len = scan_length(a, b);
   const int t_begin = seg * a.seg_len, t_end = min(t_begin + a.seg_len, a.T), t_live = min(t_end, len);
   const int nck = (a.T + kScanCkpt - 1) / kScanCkpt;
 
-  for (int k = 0; k < G; ++k) {
-    const int c = c0 + k * CH + ch;
-    Quad A2{f2{0.f, 0.f}, f2{0.f, 0.f}}, g = A2;
-    sgrp[(2 * G + k) * kScanThreads + tid] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c < a.C) {
-      A2 = load_quad(a.A + (int64_t)c * a.N, 4 * q, a.N, a.wide_n);
-      A2.lo = mul2(A2.lo, splat(kL2E));
-      A2.hi = mul2(A2.hi, splat(kL2E));
-      if (a.gh_last) g = load_quad(a.gh_last + ((int64_t)b * a.C + c) * a.N, 4 * q, a.N, a.wide_n);
-      g = scan_carry(a, b, c, 4 * q, g, A2, a.nseg - 1, seg, -1);
+  St A2[kPer], g[kPer], gA[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int k = c + u * kLane;
+    A2[u] = g[u] = gA[u] = St::zero();
+    if (k < a.C) {
+      A2[u] = St::load(a.A + (int64_t)k * a.N, 4 * q, a.N, a.wide_n);
+      A2[u].scale(kL2E);
+      if (a.gh_last) g[u] = St::load(a.gh_last + ((int64_t)b * a.C + k) * a.N, 4 * q, a.N, a.wide_n);
+      g[u] = scan_carry(a, b, k, 4 * q, g[u], A2[u], a.nseg - 1, seg, -1);
     }
-    sgrp[k * kScanThreads + tid] = quad4(A2);
-    sgrp[(G + k) * kScanThreads + tid] = quad4(g);
   }
 
   // rows past the length: zero gradients
-  for (int i = tid; i < (t_end - max(t_begin, t_live)) * CHB; i += kScanThreads) {
-    const int t = max(t_begin, t_live) + i / CHB, c = c0 + i % CHB;
-    if (c < a.C) {
-      const int64_t at = ((int64_t)b * a.T + t) * a.C + c;
+  for (int i = tid; i < (t_end - max(t_begin, t_live)) * CH; i += kThr) {
+    const int t = max(t_begin, t_live) + i / CH, k = c0 + i % CH;
+    if (k < a.C) {
+      const int64_t at = ((int64_t)b * a.T + t) * a.C + k;
       static_cast<T*>(a.gx)[at] = Pair<T>::from_float(0.f);
       static_cast<T*>(a.gdt)[at] = Pair<T>::from_float(0.f);
       if (a.gz) static_cast<T*>(a.gz)[at] = Pair<T>::from_float(0.f);
     }
   }
   float* pbc = a.part_bc + ((int64_t)cb * a.B + b) * a.T * 2 * a.N;
-  for (int i = tid; i < (t_end - max(t_begin, t_live)) * 2 * a.N; i += kScanThreads)
+  for (int i = tid; i < (t_end - max(t_begin, t_live)) * 2 * a.N; i += kThr)
     pbc[(int64_t)max(t_begin, t_live) * 2 * a.N + i] = 0.f;
 
-  // a thread's cells in the staging and in the row-wise end: two adjacent channels
-  // (always the same ones) of every row_step-th row
-  const int pairs = CHB / 2, cp = tid % pairs * 2, row0 = tid / pairs, row_step = kScanThreads / pairs;
-  float Dp[2], bp[2], gD[2] = {0.f, 0.f}, gb[2] = {0.f, 0.f};
+  const int row0 = tid / S::kPairs, cl = tid % S::kPairs * 2, cp = c0 + cl;
+  const bool plain = scan_plain(a, c0 + CH);
+  const f2 bias = param_pair(a.bias, cp, a.C), D = param_pair(a.D, cp, a.C);
+  f2 gD{0.f, 0.f}, gb{0.f, 0.f};
+
+  // Raw rows come by asynchronous copies of 16 bytes, one thread always the same
+  // word of its tensors' tiles; rows without that alignment by plain loads.
+  constexpr int E = 16 / (int)sizeof(T), kWords = kCells / E, kCopies = (4 * kWords + kThr - 1) / kThr;
+  const T* src[kCopies];
+  int64_t back[kCopies];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int c = c0 + cp + i;
-    Dp[i] = a.D && c < a.C ? a.D[c] : 0.f;
-    bp[i] = a.bias && c < a.C ? a.bias[c] : 0.f;
+  for (int j = 0; j < kCopies; ++j) {
+    const int i = j * kThr + tid, k = i / kWords, cell = i % kWords * E;
+    const T* p = static_cast<const T*>(k == 0 ? a.x : k == 1 ? a.dt : k == 2 ? a.gout : a.z);
+    const int64_t sb = k == 0 ? a.x_sb : k == 1 ? a.dt_sb : k == 2 ? a.g_sb : a.z_sb;
+    const int64_t st = k == 0 ? a.x_st : k == 1 ? a.dt_st : k == 2 ? a.g_st : a.z_st;
+    src[j] = k < 4 && p && c0 + cell % CH < a.C ? p + b * sb + cell / CH * st + c0 + cell % CH : nullptr;
+    back[j] = st;
   }
-  const T* src[4] = {static_cast<const T*>(a.x) + b * a.x_sb, static_cast<const T*>(a.dt) + b * a.dt_sb,
-                     static_cast<const T*>(a.gout) + b * a.g_sb,
-                     a.z ? static_cast<const T*>(a.z) + b * a.z_sb : nullptr};
-  const int64_t pitch[4] = {a.x_st, a.dt_st, a.g_st, a.z_st};
   auto fetch = [&](int t0, int stage) {
+    T* dst = raw + stage * 4 * kCells;
+    if (a.wide) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (k == 3 && !a.z) break;
-      T* dst = raw + (stage * 4 + k) * kCells;
-      if (a.wide) {
-        constexpr int E = 16 / (int)sizeof(T);
-        for (int i = tid * E; i < kCells; i += kScanThreads * E) {
-          const int t = t0 + i / CHB, c = c0 + i % CHB;
-          const bool on = t < t_live && c < a.C;
-          copy16(dst + i, on ? src[k] + t * pitch[k] + c : src[k], on);
-        }
-      } else {
-        for (int i = tid; i < kCells; i += kScanThreads) {
-          const int t = t0 + i / CHB, c = c0 + i % CHB;
-          dst[i] = t < t_live && c < a.C ? src[k][t * pitch[k] + c] : Pair<T>::from_float(0.f);
+      for (int j = 0; j < kCopies; ++j) {
+        const int i = j * kThr + tid;
+        if (kCopies * kThr > 4 * kWords && i >= 4 * kWords) break;
+        const bool on = src[j] != nullptr && t0 + i % kWords * E / CH < t_live;
+        copy16(dst + i * E, on ? static_cast<const void*>(src[j] + t0 * back[j]) : a.A, on);
+      }
+    } else {
+      for (int k = 0; k < (a.z ? 4 : 3); ++k) {
+        const T* p = static_cast<const T*>(k == 0 ? a.x : k == 1 ? a.dt : k == 2 ? a.gout : a.z) +
+                     b * (k == 0 ? a.x_sb : k == 1 ? a.dt_sb : k == 2 ? a.g_sb : a.z_sb);
+        const int64_t st = k == 0 ? a.x_st : k == 1 ? a.dt_st : k == 2 ? a.g_st : a.z_st;
+#pragma unroll 4
+        for (int i = tid; i < kCells; i += kThr) {
+          const int t = t0 + i / CH, k0 = c0 + i % CH;
+          dst[k * kCells + i] = t < t_live && k0 < a.C ? p[t * st + k0] : Pair<T>::from_float(0.f);
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  constexpr int kBC = (8 * M * 2 * LPC + kScanThreads - 1) / kScanThreads;
+  constexpr int kBC = (TS * 2 * LPC + kThr - 1) / kThr;
   Vec<T, 4> rbc[kBC];
   auto fetch_bc = [&](int t0) {
 #pragma unroll
     for (int k = 0; k < kBC; ++k) {
-      const int i = k * kScanThreads + tid, t = t0 + i / (2 * LPC), n = i % LPC * 4;
+      const int i = k * kThr + tid, t = t0 + i / (2 * LPC), n = i % LPC * 4;
       const bool on = i < TS * 2 * LPC && t < t_live;
       const T* p = i % (2 * LPC) < LPC ? static_cast<const T*>(a.Bm) + b * a.b_sb + (int64_t)t * a.b_st
                                        : static_cast<const T*>(a.Cm) + b * a.c_sb + (int64_t)t * a.c_st;
       rbc[k] = load_bc(p, n, a.N, on, a.wide_bc);
     }
   };
-  auto kept = [&](int t, int k) {  // the state before step t (a multiple of 8) of group k
-    const int c = c0 + k * CH + ch;
-    if (c >= a.C || t >= t_live || t < t_begin) return Quad{f2{0.f, 0.f}, f2{0.f, 0.f}};
-    return load_quad(a.ckpt + (((int64_t)b * nck + t / kScanCkpt) * a.C + c) * a.N, 4 * q, a.N, a.wide_n);
+  auto kept = [&](int t, int u) {  // the state before step t, a multiple of 8, of the thread's channel u
+    if (t >= t_live || t < t_begin) return St::zero();
+    const int64_t row = ((int64_t)b * nck + t / kScanCkpt) * a.C + min(c + u * kLane, a.C - 1);
+    return St::load(a.ckpt + row * a.N, 4 * q, a.N, a.wide_n);
   };
 
   const int tiles = t_live > t_begin ? (t_live - t_begin + TS - 1) / TS : 0;
+  ChannelSums<LPC> sums;
+  sums.init();
   if (tiles > 0) {
     fetch(t_begin + (tiles - 1) * TS, 0);
     fetch_bc(t_begin + (tiles - 1) * TS);
   }
-  Quad next = kept(t_begin + (tiles - 1) * TS + (subs - 1) * 8, 0);
+  St next[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) next[u] = kept(t_begin + tiles * TS - 8, u);
   int stage = 0;
   for (int tile = tiles - 1; tile >= 0; --tile, stage ^= 1) {
     const int t0 = t_begin + tile * TS;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     const T* cur = raw + stage * 4 * kCells;
-    for (int r = row0; r < TS; r += row_step) {
-      const int at = r * CHB + cp;
-      const bool live = t0 + r < t_live;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float x = Pair<T>::scalar(cur[at + i]);
-        const float d = live ? scan_delta(Pair<T>::scalar(cur[kCells + at + i]) + bp[i], a.softplus) : 0.f;
-        float gy = Pair<T>::scalar(cur[2 * kCells + at + i]);
-        if (a.z) {
-          const float z = Pair<T>::scalar(cur[3 * kCells + at + i]);
-          gy *= z * sigmoid1(z);
-        }
-        slot[at + i] = make_float4(d, d * x, gy, 0.f);
+    for (int k = 0; k < S::kRows; ++k) {
+      const int r = row0 + k * S::kStep, at = r * CH + cl;
+      if (S::kIdle && r >= TS) break;
+      const f2 x = pair_of(Vec<T, 2>::load(cur + at));
+      f2 d = scan_delta(add2(pair_of(Vec<T, 2>::load(cur + kCells + at)), bias), a.softplus);
+      if (t0 + r >= t_live) d = f2{0.f, 0.f};
+      f2 gy = pair_of(Vec<T, 2>::load(cur + 2 * kCells + at));
+      if (a.z) {
+        const f2 z = pair_of(Vec<T, 2>::load(cur + 3 * kCells + at));
+        gy = mul2(gy, mul2(z, sigmoid2(z)));
       }
+      const f2 dx = mul2(d, x);
+      slot[at] = make_float4(d.x, d.x, dx.x, dx.x);
+      slot[at + 1] = make_float4(d.y, d.y, dx.y, dx.y);
+      *reinterpret_cast<float4*>(sgy + at) = make_float4(gy.x, gy.x, gy.y, gy.y);
     }
 #pragma unroll
     for (int k = 0; k < kBC; ++k) {
-      const int i = k * kScanThreads + tid;
+      const int i = k * kThr + tid;
       float f[4];
       rbc[k].get(f);
       if (i < TS * 2 * LPC)
@@ -550,178 +744,172 @@ __global__ void __launch_bounds__(kScanThreads, LPC <= 4 ? 3 : 2) scan_bwd_kerne
       fetch(t0 - TS, stage ^ 1);
       fetch_bc(t0 - TS);
     }
-    for (int sub = subs - 1; sub >= 0; --sub) {
-      f2 accB[8][2], accC[8][2];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) accB[i][0] = accB[i][1] = accC[i][0] = accC[i][1] = f2{0.f, 0.f};
+#pragma unroll 1
+    for (int sub = TS / 8 - 1; sub >= 0; --sub) {
       const float* bc = sbc + sub * 8 * 2 * NP + 4 * q;
-      for (int k = 0; k < G; ++k) {
-        float4* sl = slot + sub * 8 * CHB + k * CH + ch;
-        const Quad A2 = quad(sgrp[k * kScanThreads + tid]);
-        Quad h = next;
-        {  // the state that the next group or sub-chunk starts from
-          const int nk = k + 1 < G ? k + 1 : 0;
-          next = kept(t0 + (nk ? sub : sub - 1) * 8, nk);
+      const float4* sl = slot + sub * 8 * CH + ch;
+      const float2* sg = sgy + sub * 8 * CH + ch;
+      St p[8][kPer];
+      {
+        St h[kPer];
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+          h[u] = next[u];
+          next[u] = kept(t0 + (sub - 1) * 8, u);
         }
-        Quad e[8], p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float2 s = *reinterpret_cast<const float2*>(sl + i * CHB);
-          const Quad Bt = quad(*reinterpret_cast<const float4*>(bc + i * 2 * NP));
-          e[i] = decay(A2, splat(s.x));
-          p[i] = Quad{mul2(e[i].lo, h.lo), mul2(e[i].hi, h.hi)};
-          h.lo = fma2(Bt.lo, splat(s.y), p[i].lo);
-          h.hi = fma2(Bt.hi, splat(s.y), p[i].hi);
-        }
-        Quad g = quad(sgrp[(G + k) * kScanThreads + tid]);
-        Quad gA{f2{0.f, 0.f}, f2{0.f, 0.f}};
+          const St Bt = St::shared(bc + i * 2 * NP);
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {
-          float along[4], gd[4], y[4];
+          for (int u = 0; u < kPer; ++u) {
+            const float4 s = sl[i * CH + u * kLane];
+            const f2 d{s.x, s.y}, w{s.z, s.w};
 #pragma unroll
-          for (int ii = 3; ii >= 0; --ii) {
-            const int i = half * 4 + ii;
-            const float4 s = sl[i * CHB];
-            const Quad Bt = quad(*reinterpret_cast<const float4*>(bc + i * 2 * NP));
-            const Quad Ct = quad(*reinterpret_cast<const float4*>(bc + i * 2 * NP + NP));
-            const Quad hn{fma2(Bt.lo, splat(s.y), p[i].lo), fma2(Bt.hi, splat(s.y), p[i].hi)};
-            g.lo = fma2(Ct.lo, splat(s.z), g.lo);
-            g.hi = fma2(Ct.hi, splat(s.z), g.hi);
-            const f2 al = fma2(g.hi, Bt.hi, mul2(g.lo, Bt.lo));
-            const f2 yy = fma2(hn.hi, Ct.hi, mul2(hn.lo, Ct.lo));
-            accB[i][0] = fma2(g.lo, splat(s.y), accB[i][0]);
-            accB[i][1] = fma2(g.hi, splat(s.y), accB[i][1]);
-            accC[i][0] = fma2(hn.lo, splat(s.z), accC[i][0]);
-            accC[i][1] = fma2(hn.hi, splat(s.z), accC[i][1]);
-            const Quad w{mul2(g.lo, p[i].lo), mul2(g.hi, p[i].hi)};
-            const f2 dd = fma2(w.hi, A2.hi, mul2(w.lo, A2.lo));
-            gA.lo = fma2(w.lo, splat(s.x), gA.lo);
-            gA.hi = fma2(w.hi, splat(s.x), gA.hi);
-            g.lo = mul2(g.lo, e[i].lo);
-            g.hi = mul2(g.hi, e[i].hi);
-            along[ii] = al.x + al.y;
-            y[ii] = yy.x + yy.y;
-            gd[ii] = dd.x + dd.y;
-          }
-          reduce_scatter<4, LPC, 1>(along);
-          reduce_scatter<4, LPC, 1>(gd);
-          reduce_scatter<4, LPC, 1>(y);
-          __syncwarp();  // every lane has read the slots that are now reused
-          if constexpr (LPC <= 4) {
-#pragma unroll
-            for (int i = 0; i < 4 / LPC; ++i) {
-              float4* to = sl + (half * 4 + q * (4 / LPC) + i) * CHB;
-              to->y = along[i];
-              to->z = gd[i];
-              to->w = y[i];
-            }
-          } else {
-            if (q % (LPC / 4) == 0) {
-              float4* to = sl + (half * 4 + q / (LPC / 4)) * CHB;
-              to->y = along[0];
-              to->z = gd[0];
-              to->w = y[0];
+            for (int n = 0; n < 2; ++n) {
+              p[i][u].p[n] = mul2(ex2x2(mul2(A2[u].p[n], d)), h[u].p[n]);
+              h[u].p[n] = fma2(Bt.p[n], w, p[i][u].p[n]);
             }
           }
         }
-        sgrp[(G + k) * kScanThreads + tid] = quad4(g);
-        float4& tot = sgrp[(2 * G + k) * kScanThreads + tid];
-        tot = make_float4(tot.x + gA.lo.x, tot.y + gA.lo.y, tot.z + gA.hi.x, tot.w + gA.hi.y);
       }
-      // the warp's sums over its channels: value v = step * 8 + (0..3: B, 4..7: C)
-      constexpr int CL = 32 / LPC;
-      float v[64];
+      St gAs[kPer];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i * 8 + 0] = accB[i][0].x, v[i * 8 + 1] = accB[i][0].y, v[i * 8 + 2] = accB[i][1].x;
-        v[i * 8 + 3] = accB[i][1].y, v[i * 8 + 4] = accC[i][0].x, v[i * 8 + 5] = accC[i][0].y;
-        v[i * 8 + 6] = accC[i][1].x, v[i * 8 + 7] = accC[i][1].y;
+      for (int u = 0; u < kPer; ++u) gAs[u] = St::zero();
+#pragma unroll
+      for (int half = 1; half >= 0; --half) {
+        float along[kPer][4], gd[kPer][4], y[kPer][4];
+#pragma unroll
+        for (int ii = 3; ii >= 0; --ii) {
+          const int i = half * 4 + ii;
+          const St Bt = St::shared(bc + i * 2 * NP), Ct = St::shared(bc + i * 2 * NP + NP);
+          f2 sumB[2], sumC[2];
+#pragma unroll
+          for (int u = 0; u < kPer; ++u) {
+            const float4 s = sl[i * CH + u * kLane];
+            const float2 s2 = sg[i * CH + u * kLane];
+            const f2 d{s.x, s.y}, w{s.z, s.w}, gy{s2.x, s2.y};
+            f2 al, yy, dd;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const f2 hn = fma2(Bt.p[n], w, p[i][u].p[n]), gn = fma2(Ct.p[n], gy, g[u].p[n]);
+              const f2 v = mul2(gn, p[i][u].p[n]);
+              sumB[n] = u == 0 ? mul2(gn, w) : fma2(gn, w, sumB[n]);
+              sumC[n] = u == 0 ? mul2(hn, gy) : fma2(hn, gy, sumC[n]);
+              al = n == 0 ? mul2(gn, Bt.p[n]) : fma2(gn, Bt.p[n], al);
+              yy = n == 0 ? mul2(hn, Ct.p[n]) : fma2(hn, Ct.p[n], yy);
+              dd = n == 0 ? mul2(v, A2[u].p[n]) : fma2(v, A2[u].p[n], dd);
+              gAs[u].p[n] = fma2(v, d, gAs[u].p[n]);
+              g[u].p[n] = mul2(gn, ex2x2(mul2(A2[u].p[n], d)));
+            }
+            along[u][ii] = al.x + al.y;
+            y[u][ii] = yy.x + yy.y;
+            gd[u][ii] = dd.x + dd.y;
+          }
+          float tileB[4] = {0.f, 0.f, 0.f, 0.f}, tileC[4] = {0.f, 0.f, 0.f, 0.f};
+          sums.add(tileB, sumB[0], sumB[1]);
+          sums.add(tileC, sumC[0], sumC[1]);
+          sums.store(tileB, tileC, part + ((sub * 8 + i) * L::kWarps + warp) * 2 * NP);
+        }
+        constexpr int kOwn = LPC <= 4 ? 4 / LPC : 1, kSkip = LPC <= 4 ? 1 : LPC / 4;
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+          reduce_scatter<4, LPC, kLane>(along[u]);
+          reduce_scatter<4, LPC, kLane>(gd[u]);
+          reduce_scatter<4, LPC, kLane>(y[u]);
+          if (q % kSkip == 0) {
+            float* to = res + (sub * 8 + half * 4 + q / kSkip * kOwn) * L::kPitch + ch + u * kLane;
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i, to += L::kPitch) {
+              to[0] = along[u][i];
+              to[TS * L::kPitch] = gd[u][i];
+              to[2 * TS * L::kPitch] = y[u][i];
+            }
+          }
+        }
       }
-      reduce_scatter<64, CL, LPC>(v);
-      const int own = tid % 32 / LPC * (64 / CL);
-      float* pw = part + (sub * 4 + warp) * 8 * 2 * NP;
+      // gA: eight steps' sum at a time, which keeps the long sum's rounding small
 #pragma unroll
-      for (int i = 0; i < 64 / CL; ++i) {
-        const int k = own + i;
-        pw[k / 8 * 2 * NP + (k % 8 < 4 ? 0 : NP) + 4 * q + k % 4] = v[i];
+      for (int u = 0; u < kPer; ++u) {
+        gA[u].p[0] = add2(gA[u].p[0], gAs[u].p[0]);
+        gA[u].p[1] = add2(gA[u].p[1], gAs[u].p[1]);
       }
     }
     __syncthreads();
-    for (int r = row0; r < TS; r += row_step) {
-      const int at = r * CHB + cp, t = t0 + r;
-      if (t >= t_live) continue;
-      float fx[2], fd[2], fz[2];
+    const bool whole = plain && t0 + TS <= t_live;
+    const int64_t to = ((int64_t)b * a.T + t0) * a.C;
+    T *tx = static_cast<T*>(a.gx) + to, *td = static_cast<T*>(a.gdt) + to, *tz = static_cast<T*>(a.gz) + (a.gz ? to : 0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float4 s = slot[at + i];
-        const float x = Pair<T>::scalar(cur[at + i]), v = Pair<T>::scalar(cur[kCells + at + i]) + bp[i];
-        const float go = Pair<T>::scalar(cur[2 * kCells + at + i]);
-        float gy = go;
-        fz[i] = 0.f;
-        if (a.z) {
-          const float z = Pair<T>::scalar(cur[3 * kCells + at + i]), sz = sigmoid1(z);
-          gy = go * z * sz;
-          fz[i] = go * fmaf(Dp[i], x, s.w) * sz * fmaf(z, 1.f - sz, 1.f);
-        }
-        fx[i] = fmaf(s.x, s.y, Dp[i] * gy);
-        fd[i] = fmaf(x, s.y, s.z * 0.6931471805599453f) * scan_delta_slope(v, a.softplus);
-        gD[i] = fmaf(gy, x, gD[i]);
-        gb[i] += fd[i];
+    for (int k = 0; k < S::kRows; ++k) {
+      const int r = row0 + k * S::kStep, at = r * CH + cl;
+      if (S::kIdle && r >= TS) break;
+      const f2 d{slot[at].x, slot[at + 1].x};
+      const float* v = res + r * L::kPitch + cl;
+      const float2 al = *reinterpret_cast<const float2*>(v), ga = *reinterpret_cast<const float2*>(v + TS * L::kPitch);
+      const f2 along{al.x, al.y}, x = pair_of(Vec<T, 2>::load(cur + at));
+      const f2 go = pair_of(Vec<T, 2>::load(cur + 2 * kCells + at));
+      f2 gy = go, gz{0.f, 0.f};
+      if (a.z) {
+        const f2 z = pair_of(Vec<T, 2>::load(cur + 3 * kCells + at)), sz = sigmoid2(z);
+        const float2 yv = *reinterpret_cast<const float2*>(v + 2 * TS * L::kPitch);
+        const f2 gs = mul2(go, sz), y = fma2(D, x, f2{yv.x, yv.y});
+        gy = mul2(gs, z);
+        gz = mul2(mul2(gs, y), fma2(z, sub2(splat(1.f), sz), splat(1.f)));
       }
-      const int64_t to = ((int64_t)b * a.T + t) * a.C + c0 + cp;
-      if (a.wide) {
-        if (c0 + cp < a.C) {
-          Vec<T, 2> o;
-          o.set(fx);
-          o.store(static_cast<T*>(a.gx) + to);
-          o.set(fd);
-          o.store(static_cast<T*>(a.gdt) + to);
-          if (a.gz) {
-            o.set(fz);
-            o.store(static_cast<T*>(a.gz) + to);
-          }
+      f2 gdt = fma2(x, along, mul2(f2{ga.x, ga.y}, splat(0.6931471806f)));
+      if (a.softplus) gdt = mul2(gdt, sigmoid2(add2(pair_of(Vec<T, 2>::load(cur + kCells + at)), bias)));
+      const f2 gx = fma2(d, along, mul2(D, gy));
+      if (whole) {
+        const uint32_t off = r * (uint32_t)a.C + cp;
+        Vec<T, 2> o;
+        o.set({gx.x, gx.y});
+        o.store(tx + off);
+        o.set({gdt.x, gdt.y});
+        o.store(td + off);
+        if (a.gz) {
+          o.set({gz.x, gz.y});
+          o.store(tz + off);
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (c0 + cp + i < a.C) {
-            static_cast<T*>(a.gx)[to + i] = Pair<T>::from_float(fx[i]);
-            static_cast<T*>(a.gdt)[to + i] = Pair<T>::from_float(fd[i]);
-            if (a.gz) static_cast<T*>(a.gz)[to + i] = Pair<T>::from_float(fz[i]);
-          }
+      } else if (t0 + r < t_live) {
+        const int64_t off = (int64_t)r * a.C;
+        store_pair(tx + off, cp, a.C, a.pairs, gx);
+        store_pair(td + off, cp, a.C, a.pairs, gdt);
+        if (a.gz) store_pair(tz + off, cp, a.C, a.pairs, gz);
+      }
+      if (t0 + r < t_live) {
+        gD = fma2(gy, x, gD);
+        gb = add2(gb, gdt);
       }
     }
-    for (int i = tid; i < TS * 2 * NP; i += kScanThreads) {
+    for (int i = tid; i < TS * 2 * NP; i += kThr) {
       const int r = i / (2 * NP), j = i % (2 * NP), n = j < NP ? j : j - NP;
       if (t0 + r >= t_live || n >= a.N) continue;
-      const float* p = part + (r / 8 * 4 * 8 + r % 8) * 2 * NP + j;
-      pbc[(int64_t)(t0 + r) * 2 * a.N + (j < NP ? n : a.N + n)] =
-          (p[0] + p[8 * 2 * NP]) + (p[2 * 8 * 2 * NP] + p[3 * 8 * 2 * NP]);
+      const float* p = part + r * L::kWarps * 2 * NP + j;
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < L::kWarps; ++w) s += p[w * 2 * NP];
+      pbc[(int64_t)(t0 + r) * 2 * a.N + (j < NP ? n : a.N + n)] = s;
     }
   }
-  __syncthreads();
-  for (int k = 0; k < G; ++k) {
-    const int c = c0 + k * CH + ch;
-    if (c >= a.C) continue;
-    store_quad(a.part_a + (((int64_t)b * a.nseg + seg) * a.C + c) * a.N, 4 * q, a.N, a.wide_n,
-               quad(sgrp[(2 * G + k) * kScanThreads + tid]));
-    if (a.gh0 && seg == 0)
-      store_quad(a.gh0 + ((int64_t)b * a.C + c) * a.N, 4 * q, a.N, a.wide_n, quad(sgrp[(G + k) * kScanThreads + tid]));
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int k = c + u * kLane;
+    if (k >= a.C) continue;
+    gA[u].store(a.part_a + (((int64_t)b * a.nseg + seg) * a.C + k) * a.N, 4 * q, a.N, a.wide_n);
+    if (a.gh0 && seg == 0) g[u].store(a.gh0 + ((int64_t)b * a.C + k) * a.N, 4 * q, a.N, a.wide_n);
   }
   // gD and gbias over the rows of the thread's channels
   float* red = reinterpret_cast<float*>(slot);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    red[(row0 * 2 + 0) * CHB + cp + i] = gD[i];
-    red[(row0 * 2 + 1) * CHB + cp + i] = gb[i];
-  }
+  static_assert(kCells * 4 >= 4 * kThr, "the slots hold the channel sums");
   __syncthreads();
-  for (int i = tid; i < 2 * CHB; i += kScanThreads) {
-    const int c = c0 + i % CHB;
-    if (c >= a.C) continue;
+  *reinterpret_cast<float2*>(red + (row0 * 2 + 0) * CH + cl) = make_float2(gD.x, gD.y);
+  *reinterpret_cast<float2*>(red + (row0 * 2 + 1) * CH + cl) = make_float2(gb.x, gb.y);
+  __syncthreads();
+  for (int i = tid; i < 2 * CH; i += kThr) {
+    const int k = c0 + i % CH;
+    if (k >= a.C) continue;
     float s = 0.f;
-    for (int r = 0; r < row_step; ++r) s += red[(r * 2 + i / CHB) * CHB + i % CHB];
-    a.part_d[(((int64_t)b * a.nseg + seg) * 2 + i / CHB) * a.C + c] = s;
+    for (int r = 0; r < S::kStep; ++r) s += red[(r * 2 + i / CH) * CH + i % CH];
+    a.part_d[(((int64_t)b * a.nseg + seg) * 2 + i / CH) * a.C + k] = s;
   }
 }
 
@@ -747,7 +935,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(ScanArgs a) {
   const int b = (int)(i / a.C), c = (int)(i - (int64_t)b * a.C);
   const float x = Pair<T>::scalar(static_cast<const T*>(a.x)[b * a.x_sb + c]);
   const float d = scan_delta(
-      Pair<T>::scalar(static_cast<const T*>(a.dt)[b * a.dt_sb + c]) + (a.bias ? a.bias[c] : 0.f), a.softplus);
+      splat(Pair<T>::scalar(static_cast<const T*>(a.dt)[b * a.dt_sb + c]) + (a.bias ? a.bias[c] : 0.f)), a.softplus).x;
   const T* Bt = static_cast<const T*>(a.Bm) + b * a.b_sb;
   const T* Ct = static_cast<const T*>(a.Cm) + b * a.c_sb;
   float y = (a.D ? a.D[c] : 0.f) * x;
