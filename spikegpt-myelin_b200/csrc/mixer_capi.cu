@@ -242,6 +242,14 @@ void scan_layout(ScanArgs& a, const ScanPlan& p, const ScanWs& w, int dtype, std
 
 // --------------------------------------------------------------- 4-bit weights
 
+// The most shared memory a launch of the kernel takes: the widest tile of tokens.
+template <class E, int R, int NT>
+constexpr size_t q4_smem_max() {
+  constexpr int tokens = 8 * NT / Q4Type<E>::kTerms;
+  constexpr int a = kQ4Warps * q4_warp_bytes<E, R>(tokens), b = q4_sum_bytes<R, NT>();
+  return a > b ? a : b;
+}
+
 int q4_check(int dtype, int64_t M, int64_t N, int64_t K, int64_t G) {
   if (int rc = check_type(dtype)) return rc;
   if (int rc = check_sizes({M, N, K})) return rc;
@@ -673,14 +681,36 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
   a.groups = (int)((K + group - 1) / group);
   a.pitch = (int)((K + 31) / 32 * 16);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t my = (M + kQ4Tokens - 1) / kQ4Tokens;
-  if (my > 65535) return fail(WKV_ERR_INVALID_ARGUMENT, "too many tokens: %lld", (long long)M);
+  const int es = (int)dtype_size(dtype);
+  a.wide = vector_width(es, 16 / es, {x}, {x_stride, K}) == 16 / es;
   return with_type(dtype, [&](auto e) {
-    launch(K_Q4, st, [&] {
-      q4_matvec_kernel<decltype(e)>
-          <<<dim3((unsigned)((N + kQ4Threads / 32 - 1) / (kQ4Threads / 32)), (unsigned)my), kQ4Threads, 0, st>>>(a);
-    });
-    return launched("q4_matvec launch");
+    using E = decltype(e);
+    constexpr int kTerms = Q4Type<E>::kTerms;
+    a.tokens = (int)std::min<int64_t>(M, kTerms == 1 ? 16 : 8);  // what the rings' shared memory allows
+    const int tiles = (a.tokens * kTerms + 7) / 8;
+    const int64_t my = (M + a.tokens - 1) / a.tokens;
+    if (my > 65535) return fail(WKV_ERR_INVALID_ARGUMENT, "too many tokens: %lld", (long long)M);
+    auto go = [&](auto r, auto nt) {
+      constexpr int R = decltype(r)::value, NT = decltype(nt)::value;
+      // Warps along the inputs: at least three stages each where that leaves every SM a CTA.
+      const int64_t chunks = (K + kQ4Chunk - 1) / kQ4Chunk;
+      auto ctas = [&](int wk) { return (N + 16 * R * (kQ4Warps / wk) - 1) / (16 * R * (kQ4Warps / wk)); };
+      a.wk = kQ4Warps;
+      while (a.wk > 1 && chunks < 3 * a.wk && ctas(a.wk / 2) >= sm_count()) a.wk /= 2;
+      const int bytes = std::max(kQ4Warps * q4_warp_bytes<E, R>(a.tokens), q4_sum_bytes<R, NT>());
+      const cudaError_t err = allow_smem(q4_matvec_kernel<E, R, NT>, q4_smem_max<E, R, NT>());
+      if (err != cudaSuccess) return cuda_fail(err, "setting the q4_matvec kernel's shared memory size");
+      launch(K_Q4, st, [&] {
+        q4_matvec_kernel<E, R, NT><<<dim3((unsigned)ctas(a.wk), (unsigned)my), kQ4Warps * 32, bytes, st>>>(a);
+      });
+      return launched("q4_matvec launch");
+    };
+    // 32 rows a warp where that still gives two CTAs an SM: x is read and paired half as often
+    if (tiles == 2) return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
+    if constexpr (kTerms > 1)
+      if (tiles == 3) return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 3>{});
+    if (N >= 64 * sm_count()) return go(std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{});
+    return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
   });
 }
 
