@@ -132,7 +132,40 @@ int norm_check(int dtype, int64_t rows, int64_t C) {
   return WKV_OK;
 }
 
-int norm_grid(int64_t rows) { return (int)std::min<int64_t>(rows, 2 * sm_count()); }
+// Threads of a row and of a CTA (several rows' where they are short), and CTAs: about
+// what is resident at a time, so that every CTA walks several rows.
+struct NormPlan {
+  int span, threads, grid;
+};
+NormPlan norm_plan(int64_t rows, int64_t C) {
+  NormPlan p{32, 256, 0};
+  while (p.span * kNormValues < C) p.span *= 2;
+  p.threads = std::max(p.threads, p.span);
+  const int64_t teams = p.threads / p.span;
+  p.grid = (int)std::min<int64_t>((rows + teams - 1) / teams, (int64_t)sm_count() * 512 / p.threads);
+  return p;
+}
+
+// Calls f(element, V, threads): the widest words of x, y (and their gradients) that all
+// rows allow. The parameters are float32 [C]: words of four where x has words of 16 bytes.
+template <class F>
+int norm_dispatch(int dtype, int threads, std::initializer_list<const void*> ptrs,
+                  std::initializer_list<int64_t> pitches, F&& f) {
+  const int es = (int)dtype_size(dtype), v = vector_width(es, 16 / es, ptrs, pitches);
+  return with_type(dtype, [&](auto e) {
+    constexpr int kMost = 16 / (int)sizeof(e);
+    auto sized = [&](auto n) {
+      switch (threads) {
+        case 256: return f(e, n, std::integral_constant<int, 256>{});
+        case 512: return f(e, n, std::integral_constant<int, 512>{});
+        default: return f(e, n, std::integral_constant<int, 1024>{});
+      }
+    };
+    if (v == kMost) return sized(std::integral_constant<int, kMost>{});
+    if (v >= 2) return sized(std::integral_constant<int, 2>{});
+    return sized(std::integral_constant<int, 1>{});
+  });
+}
 
 // --------------------------------------------------------------------- scan
 
@@ -596,15 +629,25 @@ int layer_norm_forward(int dtype, const void* x, const float* weight, const floa
   a.x_s = x_stride;
   a.eps = eps;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return with_type(dtype, [&](auto e) {
-    launch(K_LN_FWD, st, [&] { layer_norm_fwd_kernel<decltype(e)><<<(unsigned)rows, kNormThreads, 0, st>>>(a); });
+  const NormPlan p = norm_plan(rows, C);
+  a.span = p.span;
+  return norm_dispatch(dtype, p.threads, {x, y, weight, bias}, {C, x_stride}, [&](auto e, auto v, auto n) {
+    using E = decltype(e);
+    constexpr int V = decltype(v)::value, kThr = decltype(n)::value;
+    constexpr bool kStaged = NormIo<E, V>::kStaged;
+    auto kernel = layer_norm_fwd_kernel<E, V, kThr>;
+    const cudaError_t err = allow_smem(kernel, kStaged ? norm_smem(false, true, sizeof(E), kThr, kThr, kThr * kNormValues) : 0);
+    if (err != cudaSuccess) return cuda_fail(err, "setting the layer_norm kernel's shared memory size");
+    launch(K_LN_FWD, st, [&] {
+      kernel<<<(unsigned)p.grid * 2, p.threads, norm_smem(false, kStaged, sizeof(E), p.span, p.threads, C), st>>>(a);
+    });
     return launched("layer_norm forward launch");
   });
 }
 
 size_t layer_norm_workspace_size(int dtype, int64_t rows, int64_t C) {
   if (norm_check(dtype, rows, C)) return 0;
-  return round_up((size_t)norm_grid(rows) * 2 * C * sizeof(float));
+  return round_up((size_t)norm_plan(rows, C).grid * 2 * C * sizeof(float));
 }
 
 int layer_norm_backward(int dtype, const void* grad_y, const void* x, const float* weight, const float* mean,
@@ -633,22 +676,30 @@ int layer_norm_backward(int dtype, const void* grad_y, const void* x, const floa
   a.x_s = x_stride;
   a.gy_s = g_stride;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int grid = norm_grid(rows);
+  const NormPlan p = norm_plan(rows, C);
+  a.span = p.span;
   if (rows > 0) {
-    const int rc = with_type(dtype, [&](auto e) {
-      using T = decltype(e);
-      const cudaError_t err = allow_smem(layer_norm_bwd_kernel<T>, 2 * kNormMaxC * sizeof(float));
-      if (err != cudaSuccess) return cuda_fail(err, "setting the layer_norm backward kernel's shared memory size");
-      launch(K_LN_BWD, st,
-             [&] { layer_norm_bwd_kernel<T><<<(unsigned)grid, kNormThreads, 2 * C * sizeof(float), st>>>(a); });
-      return launched("layer_norm backward launch");
-    });
+    const int rc =
+        norm_dispatch(dtype, p.threads, {grad_y, x, grad_x, weight}, {C, g_stride, x_stride}, [&](auto e, auto v, auto n) {
+          using E = decltype(e);
+          constexpr int V = decltype(v)::value, kThr = decltype(n)::value;
+          constexpr bool kStaged = NormIo<E, V>::kStaged;
+          auto kernel = layer_norm_bwd_kernel<E, V, kThr>;
+          const cudaError_t err =
+              allow_smem(kernel, (kThr == 256 ? 2 * kThr * kNormValues * sizeof(float) : 0) +
+                                     (kStaged ? norm_smem(true, true, sizeof(E), kThr, kThr, kThr * kNormValues) : 0));
+          if (err != cudaSuccess) return cuda_fail(err, "setting the layer_norm kernel's shared memory size");
+          launch(K_LN_BWD, st, [&] {
+            kernel<<<(unsigned)p.grid, p.threads, norm_smem(true, kStaged, sizeof(E), p.span, p.threads, C), st>>>(a);
+          });
+          return launched("layer_norm backward launch");
+        });
     if (rc) return rc;
   }
   if (!grad_weight && !grad_bias) return WKV_OK;
   ColSumArgs s{};
   s.in = a.partial;
-  s.rows = grid;
+  s.rows = p.grid;
   s.blocks = 2;
   s.C = C;
   s.out[0] = grad_weight;
