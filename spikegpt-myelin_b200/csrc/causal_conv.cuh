@@ -21,7 +21,8 @@
 namespace wkv {
 
 constexpr int kConvMaxTaps = 4;
-constexpr int kConvSteps = 32;
+constexpr int kConvSteps = 32;  // rows of a walk
+constexpr int kConvAhead = 4;   // rows under way
 constexpr int kConvThreads = 64;
 
 struct ConvArgs {
@@ -39,6 +40,7 @@ struct ConvArgs {
   int B, T, C;
   int chunks, cblocks;
   int silu;
+  int wide_w;  // the four taps of a channel can be read as one word
 };
 
 __device__ __forceinline__ int conv_length(const ConvArgs& a, int b) {
@@ -79,15 +81,29 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_fwd_kernel(ConvArgs 
   }
 #pragma unroll
   for (int i = 1; i < W; ++i) conv_row<T, V, W>(a, b, t0 - W + i, c, len).get(win[i]);
+  // kConvAhead rows are under way while as many are worked on
+  Vec<T, V> next[kConvAhead];
+  const T* x = static_cast<const T*>(a.x) + b * a.x_sb + c;
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kConvAhead; ++i)
+      next[i] = t + i < min(t1, len) ? Vec<T, V>::load(x + (t + i) * a.x_st) : Vec<T, V>::zero();
+  };
+  fetch(t0);
   T* y = static_cast<T*>(a.y) + ((int64_t)b * a.T + t0) * a.C + c;
-  for (int t = t0; t < t1; ++t, y += a.C) {
-    Vec<T, V> out = Vec<T, V>::zero();
-    if (t < len) {
+  for (int t = t0; t < t1; t += kConvAhead) {
+    Vec<T, V> cur[kConvAhead];
+#pragma unroll
+    for (int i = 0; i < kConvAhead; ++i) cur[i] = next[i];
+    fetch(t + kConvAhead);
+#pragma unroll
+    for (int k = 0; k < kConvAhead; ++k, y += a.C) {
+      if (t + k >= t1) break;
 #pragma unroll
       for (int i = 0; i + 1 < W; ++i)
 #pragma unroll
         for (int v = 0; v < V; ++v) win[i][v] = win[i + 1][v];
-      conv_row<T, V, W>(a, b, t, c, len).get(win[W - 1]);
+      cur[k].get(win[W - 1]);
       float f[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
@@ -96,9 +112,11 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_fwd_kernel(ConvArgs 
         for (int j = 0; j < W; ++j) u = fmaf(w[j][v], win[j][v], u);
         f[v] = a.silu ? u * sigmoid1(u) : u;
       }
+      Vec<T, V> out;
       out.set(f);
+      if (t + k >= len) out = Vec<T, V>::zero();
+      out.store(y);
     }
-    out.store(y);
   }
 }
 
@@ -128,53 +146,76 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_bwd_kernel(ConvArgs 
   for (int i = 1; i < W; ++i) conv_row<T, V, W>(a, b, t0 - W + i, c, len).get(win[i]);
   T* gx = static_cast<T*>(a.y) + (int64_t)b * a.T * a.C + c;
   const T* gy = static_cast<const T*>(a.gy) + b * a.gy_sb + c;
-  for (int t = t0; t < t1 + W - 1; ++t) {
+  const int t_end = t1 + W - 1;
+  Vec<T, V> nx[kConvAhead], ng[kConvAhead];
+  const T* x = static_cast<const T*>(a.x) + b * a.x_sb + c;
+  auto fetch = [&](int t) {
 #pragma unroll
-    for (int i = 0; i + 1 < W; ++i)
+    for (int i = 0; i < kConvAhead; ++i) {
+      const bool on = t + i < min(t_end, len);
+      nx[i] = on ? Vec<T, V>::load(x + (t + i) * a.x_st) : Vec<T, V>::zero();
+      ng[i] = on ? Vec<T, V>::load(gy + (t + i) * a.gy_st) : Vec<T, V>::zero();
+    }
+  };
+  fetch(t0);
+  for (int tt = t0; tt < t_end; tt += kConvAhead) {
+    Vec<T, V> cx[kConvAhead], cg[kConvAhead];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        win[i][v] = win[i + 1][v];
-        gu[i][v] = gu[i + 1][v];
-      }
-    if (t < len) {
-      conv_row<T, V, W>(a, b, t, c, len).get(win[W - 1]);
+    for (int i = 0; i < kConvAhead; ++i) {
+      cx[i] = nx[i];
+      cg[i] = ng[i];
+    }
+    fetch(tt + kConvAhead);
+#pragma unroll
+    for (int k = 0; k < kConvAhead; ++k) {
+      const int t = tt + k;
+      if (t >= t_end) break;
+#pragma unroll
+      for (int i = 0; i + 1 < W; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          win[i][v] = win[i + 1][v];
+          gu[i][v] = gu[i + 1][v];
+        }
+      cx[k].get(win[W - 1]);
       float g[V];
-      Vec<T, V>::load(gy + t * a.gy_st).get(g);
+      cg[k].get(g);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float u = bias[v];
-#pragma unroll
-        for (int j = 0; j < W; ++j) u = fmaf(w[j][v], win[j][v], u);
         if (a.silu) {
+          float u = bias[v];
+#pragma unroll
+          for (int j = 0; j < W; ++j) u = fmaf(w[j][v], win[j][v], u);
           const float s = sigmoid1(u);
           g[v] *= s * fmaf(u, 1.f - s, 1.f);
         }
+        if (t >= len) g[v] = 0.f;  // a window of infinities gives its row no gradient
         gu[W - 1][v] = g[v];
-        if (t < t1) {
+      }
+      if (t < min(t1, len)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
 #pragma unroll
           for (int j = 0; j < W; ++j) gw[j][v] = fmaf(g[v], win[j][v], gw[j][v]);
           gw[W][v] += g[v];
         }
       }
-    } else {
+      const int at = t - W + 1;  // the row whose gradient is complete now
+      if (at >= t0 || (chunk == 0 && a.window != nullptr && at < 0)) {
+        float f[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) gu[W - 1][v] = 0.f;
-    }
-    const int at = t - W + 1;  // the row whose gradient is complete now
-    if (at >= t0 || (chunk == 0 && a.window != nullptr && at < 0)) {
-      float f[V];
+        for (int v = 0; v < V; ++v) {
+          f[v] = 0.f;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        f[v] = 0.f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) f[v] = fmaf(w[j][v], gu[W - 1 - j][v], f[v]);
+          for (int j = 0; j < W; ++j) f[v] = fmaf(w[j][v], gu[W - 1 - j][v], f[v]);
+        }
+        Vec<T, V> out;
+        out.set(f);
+        if (at >= 0)
+          out.store(gx + (int64_t)at * a.C);
+        else
+          out.store(static_cast<T*>(a.window) + ((int64_t)b * (W - 1) + (W - 1 + at)) * a.C + c);
       }
-      Vec<T, V> out;
-      out.set(f);
-      if (at >= 0)
-        out.store(gx + (int64_t)at * a.C);
-      else
-        out.store(static_cast<T*>(a.window) + ((int64_t)b * (W - 1) + (W - 1 + at)) * a.C + c);
     }
   }
   float* part = a.partial + ((int64_t)b * a.chunks + chunk) * (W + 1) * a.C + c;
@@ -196,15 +237,24 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(ConvArgs
 #pragma unroll
   for (int i = 0; i < W - 1; ++i) row[i] = Vec<T, V>::load(window + (int64_t)i * a.C);
   row[W - 1] = Vec<T, V>::load(static_cast<const T*>(a.x) + b * a.x_sb + c);
-  float u[V];
+  float u[V], w[W][V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) u[v] = a.bias ? a.bias[c + v] : 0.f;
+  for (int v = 0; v < V; ++v) {
+    if (W == 4 && a.wide_w) {
+      const float4 f = *reinterpret_cast<const float4*>(a.w + (int64_t)(c + v) * 4);
+      w[0][v] = f.x, w[1 % W][v] = f.y, w[2 % W][v] = f.z, w[3 % W][v] = f.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[j][v] = a.w[(int64_t)(c + v) * W + j];
+    }
+    u[v] = a.bias ? a.bias[c + v] : 0.f;
+  }
 #pragma unroll
   for (int j = 0; j < W; ++j) {
     float f[V];
     row[j].get(f);
 #pragma unroll
-    for (int v = 0; v < V; ++v) u[v] = fmaf(a.w[(int64_t)(c + v) * W + j], f[v], u[v]);
+    for (int v = 0; v < V; ++v) u[v] = fmaf(w[j][v], f[v], u[v]);
     if (j > 0) row[j].store(window + (int64_t)(j - 1) * a.C);
   }
   if (a.silu) {

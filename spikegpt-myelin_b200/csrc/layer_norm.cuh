@@ -18,8 +18,7 @@
 //
 // Rows that are not 16-byte aligned (odd widths, odd pitches) move as words of V
 // values, neighbouring lanes' side by side, and are re-ordered into the same granules
-// through shared memory (where w and b lie as well): a row's result does not depend on
-// how it lies in memory.
+// through shared memory: a row's result does not depend on how it lies in memory.
 #pragma once
 
 #include "row_io.cuh"
@@ -48,6 +47,7 @@ struct NormArgs {
 template <typename T, int V>
 struct NormIo {
   static constexpr int kGran = 16 / (int)sizeof(T), kGrans = kNormValues / kGran, kWords = kNormValues / V;
+  static constexpr int kPairs = kNormValues / 2;
   static constexpr bool kStaged = V < kGran;
 
   struct Row {
@@ -83,43 +83,46 @@ struct NormIo {
           for (int v = 0; v < V; ++v) r.w[i * (kGran / V) + k].e[v] = g.e[k * V + v];
       }
   }
-  // Values of granule i of a gathered row.
-  static __device__ __forceinline__ void get(const Row& r, int i, float (&f)[kGran]) {
+  // The pairs of a gathered row, in granule order.
+  static __device__ __forceinline__ void get(const Row& r, f2 (&f)[kPairs]) {
+    if constexpr (V == 1) {
 #pragma unroll
-    for (int k = 0; k < kGran / V; ++k) {
-      float p[V];
-      r.w[i * (kGran / V) + k].get(p);
-#pragma unroll
-      for (int v = 0; v < V; ++v) f[k * V + v] = p[v];
-    }
-  }
-  // A parameter's granule: from shared memory where rows are staged (padded there), else
-  // from the parameter itself, whose C is then a multiple of the granule.
-  static __device__ __forceinline__ void param(const float* p, const float* staged, int c, float fill,
-                                               float (&f)[kGran]) {
-    const float* from = kStaged ? staged : p;
-    if (!kStaged && p == nullptr) {
-#pragma unroll
-      for (int v = 0; v < kGran; ++v) f[v] = fill;
+      for (int i = 0; i < kPairs; ++i) f[i] = f2{Pair<T>::scalar(r.w[2 * i].e[0]), Pair<T>::scalar(r.w[2 * i + 1].e[0])};
     } else {
 #pragma unroll
-      for (int v = 0; v < kGran; v += 4) {
-        const float4 u = *reinterpret_cast<const float4*>(from + c + v);
-        f[v] = u.x, f[v + 1] = u.y, f[v + 2] = u.z, f[v + 3] = u.w;
+      for (int i = 0; i < kWords; ++i) {
+        float p[V];
+        r.w[i].get(p);
+#pragma unroll
+        for (int v = 0; v < V; v += 2) f[(i * V + v) / 2] = f2{p[v], p[v + 1]};
       }
     }
   }
-  static __device__ __forceinline__ void stage_param(const float* p, float* to, int C, int span, float fill) {
-    for (int c = threadIdx.x; c < span * kNormValues; c += blockDim.x) to[c] = c < C ? (p ? p[c] : fill) : 0.f;
+  // A parameter's pairs, held for all the rows; zeros past C, `fill` without one.
+  static __device__ __forceinline__ void param(const float* p, int lane, int span, int C, float fill, f2 (&f)[kPairs]) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const int c = (i * 2 / kGran * span + lane) * kGran + i * 2 % kGran;
+      f[i] = f2{c < C ? (p ? p[c] : fill) : 0.f, c + 1 < C ? (p ? p[c + 1] : fill) : 0.f};
+    }
   }
-  // Writes a row given by granules.
-  static __device__ __forceinline__ void store(T* row, T* buf, int lane, int span, int C, bool live,
-                                               const float (&f)[kGrans][kGran]) {
+  static __device__ __forceinline__ bool inside(int i, int e, int lane, int span, int C) {
+    const int c = (i * 2 / kGran * span + lane) * kGran;
+    return kStaged ? c + i * 2 % kGran + e < C : c < C;
+  }
+  // Writes a row given by pairs.
+  static __device__ __forceinline__ void store(T* row, T* buf, int lane, int span, int C, bool live, const f2 (&f)[kPairs]) {
 #pragma unroll
     for (int i = 0; i < kGrans; ++i) {
       const int c = (i * span + lane) * kGran;
+      float p[kGran];
+#pragma unroll
+      for (int v = 0; v < kGran; v += 2) {
+        p[v] = f[(i * kGran + v) / 2].x;
+        p[v + 1] = f[(i * kGran + v) / 2].y;
+      }
       Vec<T, kGran> o;
-      o.set(f[i]);
+      o.set(p);
       if constexpr (kStaged)
         o.store(buf + c);
       else if (live && c < C)
@@ -136,11 +139,11 @@ struct NormIo {
   }
 };
 
-// Shared memory of the kernels, in bytes: staged parameters and rows, and the
-// backward's sums where a CTA has several teams.
+// Shared memory of the kernels, in bytes: the backward's sums where a CTA has several
+// teams, and staged rows.
 inline size_t norm_smem(bool backward, bool staged, size_t es, int span, int threads, int64_t C) {
   size_t n = backward && threads > span ? (2 * C * sizeof(float) + 15) / 16 * 16 : 0;
-  if (staged) n += (size_t)span * kNormValues * sizeof(float) * (backward ? 1 : 2) + threads * kNormValues * es * (backward ? 2 : 1);
+  if (staged) n += threads * kNormValues * es * (backward ? 2 : 1);
   return n;
 }
 
@@ -166,26 +169,22 @@ __device__ __forceinline__ float2 norm_sums(float u, float v, int span, float2 (
 }
 
 // kThr: the CTA's threads, 256, 512 (rows past 4096) or 1024 (past 8192, where 64
-// registers a thread make the backward spill: such rows are rare).
+// registers a thread make both kernels spill: such rows are rare).
 template <typename T, int V, int kThr>
 __global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_fwd_kernel(NormArgs a) {
   using Io = NormIo<T, V>;
-  constexpr int G = Io::kGran, kGrans = Io::kGrans;
+  constexpr int P = Io::kPairs;
   extern __shared__ __align__(16) char smem[];
   __shared__ float2 red[2][32];
   const int lane = threadIdx.x & (a.span - 1), teams = blockDim.x / a.span, team = threadIdx.x / a.span;
-  float* sw = reinterpret_cast<float*>(smem);
-  float* sb = sw + a.span * kNormValues;
-  T* buf = reinterpret_cast<T*>(sb + a.span * kNormValues) + team * a.span * kNormValues;
+  T* buf = reinterpret_cast<T*>(smem) + team * a.span * kNormValues;
   const int64_t first = (int64_t)blockIdx.x * teams, step = (int64_t)gridDim.x * teams;
   const float inv = 1.f / a.C;
   typename Io::Row row;
   row.load(static_cast<const T*>(a.x) + (first + team) * a.x_s, lane, a.span, a.C, first + team < a.rows);
-  if constexpr (Io::kStaged) {
-    Io::stage_param(a.w, sw, a.C, a.span, 1.f);
-    Io::stage_param(a.b, sb, a.C, a.span, 0.f);
-    __syncthreads();
-  }
+  f2 w[P], b[P];
+  Io::param(a.w, lane, a.span, a.C, 1.f, w);
+  Io::param(a.b, lane, a.span, a.C, 0.f, b);
   for (int64_t r0 = first; r0 < a.rows; r0 += step) {
     const int64_t r = r0 + team;
     if constexpr (Io::kStaged) {
@@ -193,35 +192,27 @@ __global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_fwd_kern
       Io::sync(a.span);
       Io::gather(row, buf, lane, a.span);
     }
-    float f[kGrans][G], s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kGrans; ++i) {
-      Io::get(row, i, f[i]);
-#pragma unroll
-      for (int v = 0; v < G; ++v) s += f[i][v];
-    }
+    f2 f[P], s{0.f, 0.f};
+    Io::get(row, f);
     row.load(static_cast<const T*>(a.x) + (r + step) * a.x_s, lane, a.span, a.C, r + step < a.rows);
-    const float mu = norm_sums(s, 0.f, a.span, red, 0).x * inv;
-    s = 0.f;
 #pragma unroll
-    for (int i = 0; i < kGrans; ++i)
+    for (int i = 0; i < P; ++i) s = add2(s, f[i]);
+    const float mu = norm_sums(s.x + s.y, 0.f, a.span, red, 0).x * inv;
+    s = f2{0.f, 0.f};
 #pragma unroll
-      for (int v = 0; v < G; ++v) {
-        f[i][v] -= mu;
-        if ((i * a.span + lane) * G + (Io::kStaged ? v : 0) < a.C) s = fmaf(f[i][v], f[i][v], s);
+    for (int i = 0; i < P; ++i) {
+      f[i] = sub2(f[i], splat(mu));
+      if constexpr (Io::kStaged) {  // the values past C are zeros less the mean
+        if (!Io::inside(i, 0, lane, a.span, a.C)) f[i].x = 0.f;
+        if (!Io::inside(i, 1, lane, a.span, a.C)) f[i].y = 0.f;
+      } else {
+        if (!Io::inside(i, 0, lane, a.span, a.C)) f[i] = f2{0.f, 0.f};
       }
-    const float rs = rsqrtf(norm_sums(s, 0.f, a.span, red, 1).x * inv + a.eps);
-#pragma unroll
-    for (int i = 0; i < kGrans; ++i) {
-      const int c = (i * a.span + lane) * G;
-      if (Io::kStaged || c < a.C) {
-        float w[G], b[G];
-        Io::param(a.w, sw, c, 1.f, w);
-        Io::param(a.b, sb, c, 0.f, b);
-#pragma unroll
-        for (int v = 0; v < G; ++v) f[i][v] = fmaf(f[i][v] * rs, w[v], b[v]);
-      }
+      s = fma2(f[i], f[i], s);
     }
+    const float rs = rsqrtf(norm_sums(s.x + s.y, 0.f, a.span, red, 1).x * inv + a.eps);
+#pragma unroll
+    for (int i = 0; i < P; ++i) f[i] = fma2(mul2(f[i], splat(rs)), w[i], b[i]);
     Io::store(static_cast<T*>(a.y) + r * a.C, buf, lane, a.span, a.C, r < a.rows, f);
     if constexpr (Io::kStaged) Io::sync(a.span);  // buf is rewritten
     if (r < a.rows && lane == 0) {
@@ -234,21 +225,20 @@ __global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_fwd_kern
 template <typename T, int V, int kThr>
 __global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_bwd_kernel(NormArgs a) {
   using Io = NormIo<T, V>;
-  constexpr int G = Io::kGran, kGrans = Io::kGrans;
-  extern __shared__ __align__(16) char smem[];  // [2][C] sums where a CTA has several teams, then what is staged
+  constexpr int P = Io::kPairs, G = Io::kGran;
+  extern __shared__ __align__(16) char smem[];  // [2][C] sums where a CTA has several teams, then staged rows
   __shared__ float2 red[2][32];
   const int lane = threadIdx.x & (a.span - 1), teams = blockDim.x / a.span, team = threadIdx.x / a.span;
   float* acc = reinterpret_cast<float*>(smem);
-  float* sw = reinterpret_cast<float*>(smem + (teams > 1 ? (2 * a.C * sizeof(float) + 15) / 16 * 16 : 0));
-  T* bx = reinterpret_cast<T*>(sw + a.span * kNormValues) + team * 2 * a.span * kNormValues;
+  T* bx = reinterpret_cast<T*>(smem + (teams > 1 ? (2 * a.C * sizeof(float) + 15) / 16 * 16 : 0)) +
+          team * 2 * a.span * kNormValues;
   T* bg = bx + a.span * kNormValues;
   const int64_t first = (int64_t)blockIdx.x * teams, step = (int64_t)gridDim.x * teams;
   const float inv = 1.f / a.C;
-  float gw[kGrans][G], gb[kGrans][G];
+  f2 gw[P], gb[P], w[P];
 #pragma unroll
-  for (int i = 0; i < kGrans; ++i)
-#pragma unroll
-    for (int v = 0; v < G; ++v) gw[i][v] = gb[i][v] = 0.f;
+  for (int i = 0; i < P; ++i) gw[i] = gb[i] = f2{0.f, 0.f};
+  Io::param(a.w, lane, a.span, a.C, 1.f, w);
   typename Io::Row nx, ng;
   float nmu = 0.f, nrs = 0.f;
   auto fetch = [&](int64_t r) {
@@ -259,61 +249,37 @@ __global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_bwd_kern
     nrs = live ? a.rstd[r] : 0.f;
   };
   fetch(first + team);
-  if constexpr (Io::kStaged) {
-    Io::stage_param(a.w, sw, a.C, a.span, 1.f);
-    __syncthreads();
-  }
   int slot = 0;
   for (int64_t r0 = first; r0 < a.rows; r0 += step, slot ^= 1) {
     const int64_t r = r0 + team;
-    typename Io::Row x = nx, g = ng;
-    const float mu = nmu, rs = nrs;
+    f2 h[P], g[P];
     if constexpr (Io::kStaged) {
-      Io::spread(x, bx, lane, a.span);
-      Io::spread(g, bg, lane, a.span);
+      Io::spread(nx, bx, lane, a.span);
+      Io::spread(ng, bg, lane, a.span);
       Io::sync(a.span);
+      Io::gather(nx, bx, lane, a.span);
+      Io::gather(ng, bg, lane, a.span);
     }
+    Io::get(nx, h);
+    Io::get(ng, g);
+    const f2 mu = splat(nmu), rs = splat(nrs);
     fetch(r + step);
-    if constexpr (Io::kStaged) {
-      Io::gather(x, bx, lane, a.span);
-      Io::gather(g, bg, lane, a.span);
+    f2 s1{0.f, 0.f}, s2{0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < P; ++i) {  // past C w and gy are zeros
+      h[i] = mul2(sub2(h[i], mu), rs);
+      gw[i] = fma2(g[i], h[i], gw[i]);
+      gb[i] = add2(gb[i], g[i]);
+      g[i] = mul2(g[i], w[i]);
+      s1 = add2(s1, g[i]);
+      s2 = fma2(g[i], h[i], s2);
     }
-    float s1 = 0.f, s2 = 0.f;
+    const float2 m = norm_sums(s1.x + s1.y, s2.x + s2.y, a.span, red, slot);
+    const f2 m1 = splat(m.x * inv), m2 = splat(-m.y * inv);
 #pragma unroll
-    for (int i = 0; i < kGrans; ++i) {
-      const int c = (i * a.span + lane) * G;
-      if (Io::kStaged || c < a.C) {  // what is staged past C has w = gy = 0
-        float xv[G], gv[G], w[G];
-        Io::get(x, i, xv);
-        Io::get(g, i, gv);
-        Io::param(a.w, sw, c, 1.f, w);
-#pragma unroll
-        for (int v = 0; v < G; ++v) {
-          const float h = (xv[v] - mu) * rs, gh = gv[v] * w[v];
-          s1 += gh;
-          s2 = fmaf(gh, h, s2);
-          gw[i][v] = fmaf(gv[v], h, gw[i][v]);
-          gb[i][v] += gv[v];
-        }
-      }
-    }
-    const float2 m = norm_sums(s1, s2, a.span, red, slot);
-    const float m1 = m.x * inv, m2 = m.y * inv;
-    float o[kGrans][G];
-#pragma unroll
-    for (int i = 0; i < kGrans; ++i) {
-      const int c = (i * a.span + lane) * G;
-      if (Io::kStaged || c < a.C) {
-        float xv[G], gv[G], w[G];
-        Io::get(x, i, xv);
-        Io::get(g, i, gv);
-        Io::param(a.w, sw, c, 1.f, w);
-#pragma unroll
-        for (int v = 0; v < G; ++v) o[i][v] = rs * (fmaf(gv[v], w[v], -m1) - (xv[v] - mu) * rs * m2);
-      }
-    }
+    for (int i = 0; i < P; ++i) g[i] = mul2(fma2(h[i], m2, sub2(g[i], m1)), rs);
     if constexpr (Io::kStaged) Io::sync(a.span);  // every lane has gathered from bx
-    Io::store(static_cast<T*>(a.y) + r * a.C, bx, lane, a.span, a.C, r < a.rows, o);
+    Io::store(static_cast<T*>(a.y) + r * a.C, bx, lane, a.span, a.C, r < a.rows, g);
     if constexpr (Io::kStaged) Io::sync(a.span);
   }
   float* part = a.partial + (int64_t)blockIdx.x * 2 * a.C;
@@ -321,13 +287,14 @@ __global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_bwd_kern
   for (int k = 0; k < teams; ++k) {
     if (team == k) {
 #pragma unroll
-      for (int i = 0; i < kGrans; ++i) {
-        const int c = (i * a.span + lane) * G;
+      for (int i = 0; i < P; ++i) {
+        const int c = (i * 2 / G * a.span + lane) * G + i * 2 % G;
+        const float vw[2] = {gw[i].x, gw[i].y}, vb[2] = {gb[i].x, gb[i].y};
 #pragma unroll
-        for (int v = 0; v < G; ++v)
-          if (c + v < a.C) {
-            to[c + v] = (k ? to[c + v] : 0.f) + gw[i][v];
-            to[a.C + c + v] = (k ? to[a.C + c + v] : 0.f) + gb[i][v];
+        for (int e = 0; e < 2; ++e)
+          if (c + e < a.C) {
+            to[c + e] = (k ? to[c + e] : 0.f) + vw[e];
+            to[a.C + c + e] = (k ? to[a.C + c + e] : 0.f) + vb[e];
           }
       }
     }

@@ -279,13 +279,14 @@ void scan_layout(ScanArgs& a, const ScanPlan& p, const ScanWs& w, int dtype, std
 template <class E, int R, int NT>
 constexpr size_t q4_smem_max() {
   constexpr int tokens = 8 * NT / Q4Type<E>::kTerms;
-  constexpr int a = kQ4Warps * q4_warp_bytes<E, R>(tokens), b = q4_sum_bytes<R, NT>();
+  constexpr int a = kQ4Warps * q4_warp_bytes<E, R, NT>(tokens), b = q4_sum_bytes<R, NT>();
   return a > b ? a : b;
 }
 
 int q4_check(int dtype, int64_t M, int64_t N, int64_t K, int64_t G) {
   if (int rc = check_type(dtype)) return rc;
   if (int rc = check_sizes({M, N, K})) return rc;
+  if (K > (1 << 21)) return fail(WKV_ERR_INVALID_ARGUMENT, "size out of range: %lld", (long long)K);
   if (G < 32 || G % 32 != 0 || G > kMaxDim)
     return fail(WKV_ERR_INVALID_ARGUMENT, "the group size must be a positive multiple of 32, got %lld", (long long)G);
   return WKV_OK;
@@ -386,6 +387,7 @@ int causal_conv_step(int dtype, const void* x, const float* weight, const float*
   ConvArgs a = conv_args(x, weight, bias, nullptr, nullptr, B, 1, C, x_stride_b, C, silu);
   a.y = y;
   a.window = window;
+  a.wide_w = aligned16(weight);
   const int V = vector_width(dtype_size(dtype), 4, {x, y, window}, {C, x_stride_b});
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return conv_dispatch(dtype, V, W, [&](auto e, auto v, auto w) {
@@ -603,12 +605,19 @@ int selective_scan_step(int dtype, const void* x, const void* dt, const float* A
   a.B = (int)B, a.T = 1, a.C = (int)C, a.N = (int)N;
   a.softplus = softplus;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return with_type(dtype, [&](auto e) {
+  const int es = (int)dtype_size(dtype), lanes = scan_lanes(N, 4);
+  a.wide_bc = N % 4 == 0 && vector_width(es, 4, {Bm, Cm}, {b_sb, c_sb}) == 4;
+  a.wide_n = N % 4 == 0 && vector_width(4, 4, {A, state}, {}) == 4;
+  auto go = [&](auto e, auto lanes_) {
+    constexpr int kLanesPer = decltype(lanes_)::value, kChannels = kScanStepThreads / kLanesPer;
+    a.cblocks = (int)((C + kChannels - 1) / kChannels);
     launch(K_SCAN_STEP, st, [&] {
-      scan_step_kernel<decltype(e)><<<(unsigned)((B * C + 127) / 128), 128, 0, st>>>(a);
+      scan_step_kernel<decltype(e), kLanesPer><<<(unsigned)(B * a.cblocks), kScanStepThreads, 0, st>>>(a);
     });
     return launched("selective_scan step launch");
-  });
+  };
+  return lanes == 16 ? with_type(dtype, [&](auto e) { return go(e, std::integral_constant<int, 16>{}); })
+                     : scan_dispatch(dtype, lanes, go);
 }
 
 int layer_norm_forward(int dtype, const void* x, const float* weight, const float* bias, void* y, float* mean,
@@ -734,6 +743,9 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int es = (int)dtype_size(dtype);
   a.wide = vector_width(es, 16 / es, {x}, {x_stride, K}) == 16 / es;
+  // floor(i / d) is the upper word of i * (floor(2^32 / d) + 1) while i * d < 2^32
+  const int64_t d = std::min(group, (K + 31) / 32 * 32) / 32;
+  a.group_magic = d > 1 ? (uint32_t)((1ull << 32) / d + 1) : 0;
   return with_type(dtype, [&](auto e) {
     using E = decltype(e);
     constexpr int kTerms = Q4Type<E>::kTerms;
@@ -748,7 +760,7 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
       auto ctas = [&](int wk) { return (N + 16 * R * (kQ4Warps / wk) - 1) / (16 * R * (kQ4Warps / wk)); };
       a.wk = kQ4Warps;
       while (a.wk > 1 && chunks < 3 * a.wk && ctas(a.wk / 2) >= sm_count()) a.wk /= 2;
-      const int bytes = std::max(kQ4Warps * q4_warp_bytes<E, R>(a.tokens), q4_sum_bytes<R, NT>());
+      const int bytes = std::max(kQ4Warps * q4_warp_bytes<E, R, NT>(a.tokens), q4_sum_bytes<R, NT>());
       const cudaError_t err = allow_smem(q4_matvec_kernel<E, R, NT>, q4_smem_max<E, R, NT>());
       if (err != cudaSuccess) return cuda_fail(err, "setting the q4_matvec kernel's shared memory size");
       launch(K_Q4, st, [&] {

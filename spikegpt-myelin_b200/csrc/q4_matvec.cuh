@@ -6,8 +6,7 @@
 //
 // Bound by the bytes of the weights while the tokens are few, so the weights are
 // read once for up to 16 tokens (8 in float32), by asynchronous copies kQ4Stages deep in a
-// ring of the warp's own: 16 R rows x 128 inputs a stage, with the tokens' 128 inputs
-// beside them. Decoding is a logical operation and a packed subtraction for two
+// ring of the warp's own: 16 R rows x 128 inputs a stage. Decoding is a logical operation and a packed subtraction for two
 // weights (and a shift for three of four): a nibble or-ed into the mantissa of a 16-bit
 // float stands for 2^m + q, and less 2^m + zero it is exact. The products go to
 // m16n8k16 tiles (A the weights, B the tokens), whose k order is free: the pairs that a
@@ -41,6 +40,7 @@ struct Q4Args {
   int tokens;  // of a CTA
   int wk;      // warps along the inputs
   int wide;    // rows of x are whole aligned 16-byte words
+  uint32_t group_magic;  // the upper word of its product with k / 32 is the group (0: k / 32 is)
 };
 
 // Columns that a token takes, and the 16-bit type the products run in.
@@ -88,19 +88,25 @@ struct Q4Math<__half> {
   }
 };
 
+// One tile of 16-bit tokens is read straight to registers a stage ahead (the rows of x
+// are short and stay in the L1 cache); more tokens, and float32 ones, are staged.
+template <typename T, int NT>
+__host__ __device__ constexpr bool q4_staged() {
+  return NT > 1 || sizeof(T) > 2;
+}
 // Bytes of a staged token's inputs: a shift of half the banks from token to token.
 template <typename T>
 __host__ __device__ constexpr int q4_token_bytes() {
   return kQ4Chunk * (int)sizeof(T) + 64;
 }
-template <typename T, int R>
+template <typename T, int R, int NT>
 __host__ __device__ constexpr int q4_stage_bytes(int tokens) {
-  return R * 16 * kQ4Row + tokens * q4_token_bytes<T>();
+  return R * 16 * kQ4Row + (q4_staged<T, NT>() ? tokens * q4_token_bytes<T>() : 0);
 }
 // A warp's ring and its scales and zeros (float, uint32_t) [2][16 R][4].
-template <typename T, int R>
+template <typename T, int R, int NT>
 __host__ __device__ constexpr int q4_warp_bytes(int tokens) {
-  return kQ4Stages * q4_stage_bytes<T, R>(tokens) + 2 * R * 16 * 4 * 8;
+  return kQ4Stages * q4_stage_bytes<T, R, NT>(tokens) + 2 * R * 16 * 4 * 8;
 }
 template <int R, int NT>
 constexpr int q4_sum_bytes() {
@@ -112,15 +118,17 @@ __device__ __forceinline__ void q4_copy(void* dst, const void* src, bool on) {
                : "memory");
 }
 
-// B operands of a column's eight inputs at p: word i holds inputs i and i + 4.
+// B operands of a column's eight inputs: word i holds inputs i and i + 4.
+__device__ __forceinline__ void q4_pairs(uint4 u, uint32_t (&b)[4]) {
+  b[0] = __byte_perm(u.x, u.z, 0x5410);
+  b[1] = __byte_perm(u.x, u.z, 0x7632);
+  b[2] = __byte_perm(u.y, u.w, 0x5410);
+  b[3] = __byte_perm(u.y, u.w, 0x7632);
+}
 template <typename T>
 __device__ __forceinline__ void q4_inputs(const T* p, int term, uint32_t (&b)[4]) {
   if constexpr (sizeof(T) == 2) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    b[0] = __byte_perm(u.x, u.z, 0x5410);
-    b[1] = __byte_perm(u.x, u.z, 0x7632);
-    b[2] = __byte_perm(u.y, u.w, 0x5410);
-    b[3] = __byte_perm(u.y, u.w, 0x7632);
+    q4_pairs(*reinterpret_cast<const uint4*>(p), b);
   } else {
     const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
     const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
@@ -148,53 +156,87 @@ __global__ void __launch_bounds__(kQ4Warps * 32) q4_matvec_kernel(Q4Args a) {
   const int rows = 16 * R, cta_rows = rows * (kQ4Warps / a.wk);
   const int n0 = blockIdx.x * cta_rows + wn * rows, m0 = blockIdx.y * a.tokens;
   const int tokens = min(a.tokens, a.M - m0);
-  const int stage_bytes = q4_stage_bytes<T, R>(a.tokens);
-  char* ring = smem + warp * q4_warp_bytes<T, R>(a.tokens);
+  const int stage_bytes = q4_stage_bytes<T, R, NT>(a.tokens);
+  char* ring = smem + warp * q4_warp_bytes<T, R, NT>(a.tokens);
   float2* sz = reinterpret_cast<float2*>(ring + kQ4Stages * stage_bytes);
   const int chunks = (a.K + kQ4Chunk - 1) / kQ4Chunk;
   const int mine = n0 < a.N && chunks > wk ? (chunks - wk + a.wk - 1) / a.wk : 0;
   const T* x = static_cast<const T*>(a.x) + m0 * a.x_s;
 
+  // where the lane reads: rows p * 8 + g, its quarter of each stage's inputs
+  const uint8_t* pq[2 * R];
+  const uint16_t* ps[2 * R];
+  const uint8_t* pz[2 * R];
+#pragma unroll
+  for (int p = 0; p < 2 * R; ++p) {
+    const int64_t row = min(n0 + p * 8 + g, a.N - 1);
+    pq[p] = a.q + row * a.pitch + wk * (kQ4Chunk / 2) + j * 16;
+    ps[p] = reinterpret_cast<const uint16_t*>(a.scale) + row * a.groups;
+    pz[p] = a.zero ? a.zero + row * a.groups : nullptr;
+  }
+  const int last32 = (a.K - 1) / 32;  // the row's last 32 inputs
   auto issue = [&](int i) {
     if (i < mine) {
       const int k0 = (wk + i * a.wk) * kQ4Chunk;
       char* to = ring + i % kQ4Stages * stage_bytes;
+      const bool on = k0 + j * 32 < a.K;
+      const int64_t at = (int64_t)i * a.wk * (kQ4Chunk / 2);
 #pragma unroll
-      for (int p = 0; p < 2 * R; ++p) {
-        const int row = p * 8 + g;
-        const bool on = k0 + j * 32 < a.K;
-        q4_copy(to + row * kQ4Row + j * 16,
-                a.q + (int64_t)min(n0 + row, a.N - 1) * a.pitch + (on ? k0 / 2 + j * 16 : 0), on);
-      }
-      char* tx = to + rows * kQ4Row;
-      constexpr int kWords = kQ4Chunk * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
-      if (a.wide) {
-        for (int p = lane; p < tokens * kWords; p += 32) {
-          const int k = k0 + p % kWords * E;
-          const bool on = k < a.K;
-          q4_copy(tx + p / kWords * kTok + p % kWords * 16, x + p / kWords * a.x_s + (on ? k : 0), on);
-        }
-      } else {
-        for (int p = lane; p < tokens * kQ4Chunk; p += 32) {
-          const int k = k0 + p % kQ4Chunk;
-          reinterpret_cast<T*>(tx + p / kQ4Chunk * kTok)[p % kQ4Chunk] =
-              k < a.K ? x[p / kQ4Chunk * a.x_s + k] : Pair<T>::from_float(0.f);
+      for (int p = 0; p < 2 * R; ++p)
+        q4_copy(to + (p * 8 + g) * kQ4Row + j * 16, on ? pq[p] + at : a.q, on);
+      if constexpr (q4_staged<T, NT>()) {
+        char* tx = to + rows * kQ4Row;
+        constexpr int kWords = kQ4Chunk * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
+        if (a.wide) {
+          for (int p = lane; p < tokens * kWords; p += 32) {
+            const int k = k0 + p % kWords * E;
+            q4_copy(tx + p / kWords * kTok + p % kWords * 16, x + p / kWords * a.x_s + (k < a.K ? k : 0), k < a.K);
+          }
+        } else {
+          for (int p = lane; p < tokens * kQ4Chunk; p += 32) {
+            const int k = k0 + p % kQ4Chunk;
+            reinterpret_cast<T*>(tx + p / kQ4Chunk * kTok)[p % kQ4Chunk] =
+                k < a.K ? x[p / kQ4Chunk * a.x_s + k] : Pair<T>::from_float(0.f);
+          }
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // scales and zeros of the next stage: 32 inputs of a row each
+  // scales and zeros of the next stage, 32 inputs of a row each, and unstaged tokens
   uint16_t fs[2 * R];
   uint8_t fz[2 * R];
+  uint4 fx[4];
+  const bool token = g < tokens;  // the lane's column is a token (one tile of 16-bit tokens)
+  const T* px = x + (token ? g * a.x_s : 0) + wk * kQ4Chunk + j * 8;
   auto fetch = [&](int i) {
     if (i >= mine) return;
-    const int k = (wk + i * a.wk) * kQ4Chunk + j * 32, group = k < a.K ? k / a.G : 0;
+    const int k32 = min((wk + i * a.wk) * 4 + j, last32), group = a.group_magic ? __umulhi(k32, a.group_magic) : k32;
 #pragma unroll
     for (int p = 0; p < 2 * R; ++p) {
-      const int64_t at = (int64_t)min(n0 + p * 8 + g, a.N - 1) * a.groups + group;
-      fs[p] = reinterpret_cast<const uint16_t*>(a.scale)[at];
-      fz[p] = a.zero ? a.zero[at] : 8;
+      fs[p] = ps[p][group];
+      fz[p] = a.zero ? pz[p][group] : 8;
+    }
+    if constexpr (!q4_staged<T, NT>()) {
+      const T* from = px + (int64_t)i * a.wk * kQ4Chunk;
+      const int k0 = (wk + i * a.wk) * kQ4Chunk + j * 8;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int k = k0 + w * 32;
+        fx[w] = make_uint4(0, 0, 0, 0);
+        if (token && k < a.K) {
+          if (a.wide) {
+            fx[w] = *reinterpret_cast<const uint4*>(from + w * 32);
+          } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(from + w * 32);
+            uint32_t u[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              u[n] = (k + 2 * n < a.K ? h[2 * n] : 0u) | (k + 2 * n + 1 < a.K ? (uint32_t)h[2 * n + 1] << 16 : 0u);
+            fx[w] = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        }
+      }
     }
   };
   auto keep = [&](int i) {
@@ -218,6 +260,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32) q4_matvec_kernel(Q4Args a) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kQ4Stages - 2) : "memory");
     __syncwarp();  // the stage and its scales are there, and every lane is done with the stage before
     issue(i + kQ4Stages - 1);
+    const uint4 cx[4] = {fx[0], fx[1], fx[2], fx[3]};
     fetch(i + 1);
     const char* from = ring + i % kQ4Stages * stage_bytes;
     const float2* sc = sz + (i & 1) * rows * 4;
@@ -227,7 +270,9 @@ __global__ void __launch_bounds__(kQ4Warps * 32) q4_matvec_kernel(Q4Args a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int column = t * 8 + g;
-        if (column < tokens * kTerms)
+        if constexpr (!q4_staged<T, NT>())
+          q4_pairs(cx[w], b[t]);
+        else if (column < tokens * kTerms)
           q4_inputs(reinterpret_cast<const T*>(from + rows * kQ4Row + column / kTerms * kTok) + w * 32 + j * 8,
                     column % kTerms, b[t]);
         else

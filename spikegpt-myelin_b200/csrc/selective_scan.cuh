@@ -927,29 +927,47 @@ __global__ void __launch_bounds__(256) scan_reduce_kernel(const float* part, int
   to[row * N + (j < N ? j : j - N)] = Pair<T>::from_float(s);
 }
 
-// One token: x, dt, z [B][C] and B, C [B][N]; the state is updated in place.
-template <typename T>
-__global__ void __launch_bounds__(128) scan_step_kernel(ScanArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
-  if (i >= (int64_t)a.B * a.C) return;
-  const int b = (int)(i / a.C), c = (int)(i - (int64_t)b * a.C);
+// One token: x, dt, z [B][C] and B, C [B][N]; the state is updated in place. LPC
+// lanes share a channel, four states each, so a warp reads and writes 512 contiguous
+// bytes of the state, which is nearly all the traffic there is.
+constexpr int kScanStepThreads = 128;
+template <typename T, int LPC>
+__global__ void __launch_bounds__(kScanStepThreads) scan_step_kernel(ScanArgs a) {
+  constexpr int kChannels = kScanStepThreads / LPC;
+  const int q = threadIdx.x % LPC, b = blockIdx.x / a.cblocks;
+  const int c0 = blockIdx.x % a.cblocks * kChannels + threadIdx.x / LPC;
+  const bool mine = c0 < a.C;
+  const int c = mine ? c0 : a.C - 1;
+  float* hp = a.h_last + ((int64_t)b * a.C + c) * a.N;
+  States<4> h = States<4>::load(hp, 4 * q, a.N, a.wide_n);
+  States<4> A2 = States<4>::load(a.A + (int64_t)c * a.N, 4 * q, a.N, a.wide_n);
+  const Vec<T, 4> rB = load_bc(static_cast<const T*>(a.Bm) + b * a.b_sb, 4 * q, a.N, true, a.wide_bc);
+  const Vec<T, 4> rC = load_bc(static_cast<const T*>(a.Cm) + b * a.c_sb, 4 * q, a.N, true, a.wide_bc);
   const float x = Pair<T>::scalar(static_cast<const T*>(a.x)[b * a.x_sb + c]);
-  const float d = scan_delta(
-      splat(Pair<T>::scalar(static_cast<const T*>(a.dt)[b * a.dt_sb + c]) + (a.bias ? a.bias[c] : 0.f)), a.softplus).x;
-  const T* Bt = static_cast<const T*>(a.Bm) + b * a.b_sb;
-  const T* Ct = static_cast<const T*>(a.Cm) + b * a.c_sb;
-  float y = (a.D ? a.D[c] : 0.f) * x;
-  float* h = a.h_last + i * a.N;
-  for (int n = 0; n < a.N; ++n) {
-    const float v = fmaf(ex2(d * a.A[(int64_t)c * a.N + n] * kL2E), h[n], d * x * Pair<T>::scalar(Bt[n]));
-    h[n] = v;
-    y = fmaf(v, Pair<T>::scalar(Ct[n]), y);
+  const float raw = Pair<T>::scalar(static_cast<const T*>(a.dt)[b * a.dt_sb + c]);
+  const float z = a.z ? Pair<T>::scalar(static_cast<const T*>(a.z)[b * a.z_sb + c]) : 0.f;
+  const float D = a.D ? a.D[c] : 0.f, bias = a.bias ? a.bias[c] : 0.f;
+  const f2 d = scan_delta(splat(raw + bias), a.softplus), w = mul2(d, splat(x));
+  float fB[4], fC[4];
+  rB.get(fB);
+  rC.get(fC);
+  A2.scale(kL2E);
+  f2 y{0.f, 0.f};
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    h.p[n] = fma2(ex2x2(mul2(A2.p[n], d)), h.p[n], mul2(f2{fB[2 * n], fB[2 * n + 1]}, w));
+    y = fma2(h.p[n], f2{fC[2 * n], fC[2 * n + 1]}, y);
   }
-  if (a.z) {
-    const float z = Pair<T>::scalar(static_cast<const T*>(a.z)[b * a.z_sb + c]);
-    y *= z * sigmoid1(z);
+  float s = y.x + y.y;
+#pragma unroll
+  for (int o = 1; o < LPC; o *= 2) s += __shfl_xor_sync(kFull, s, o);
+  if (!mine) return;
+  h.store(hp, 4 * q, a.N, a.wide_n);
+  if (q == 0) {
+    s = fmaf(D, x, s);
+    if (a.z) s *= z * sigmoid1(z);
+    static_cast<T*>(a.out)[(int64_t)b * a.C + c] = Pair<T>::from_float(s);
   }
-  static_cast<T*>(a.out)[i] = Pair<T>::from_float(y);
 }
 
 }  // namespace wkv
