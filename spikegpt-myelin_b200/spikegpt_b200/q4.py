@@ -9,15 +9,12 @@ are float32. No gradient: it serves generation.
 
 from __future__ import annotations
 
-from contextlib import nullcontext
-
 import torch
 from torch import Tensor
 
-from . import _capi
-from ._mixer import code_of, need_cuda, need_shape, no_grad_only, on_device, parameter, ptr, rows, stream
+from . import _native
 
-_FEW = 64  # tokens of one call into the library
+_op = _native.op_if_built("q4_linear")
 
 
 def packed_pitch(in_features: int) -> int:
@@ -67,67 +64,10 @@ def _check_group(group_size: int) -> None:
         raise ValueError(f"group_size must be a positive multiple of 32; got {group_size}")
 
 
-def _matvec(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, bias: Tensor | None,
-            group_size: int) -> Tensor:
-    m, k = x.shape
-    n = packed.shape[0]
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    code, fn = code_of("x", x), _capi.lib().q4_matvec
-    for at in range(0, m, _FEW):
-        part = x[at : at + _FEW] if m > _FEW else x
-        to = y[at : at + _FEW] if m > _FEW else y
-        _capi.check(
-            fn(code, part.data_ptr(), packed.data_ptr(), scales.data_ptr(), ptr(zeros), ptr(bias), to.data_ptr(),
-               part.shape[0], n, k, group_size, x.stride(0), stream(x)),
-            "q4_matvec",
-        )
-    return y
-
-
-@torch.library.custom_op("spikegpt_b200::q4_linear", mutates_args=(), device_types="cuda")
-def _op(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, bias: Tensor | None,
-        group_size: int) -> Tensor:
-    with on_device(x) or nullcontext():
-        return _matvec(rows(x), packed, scales, zeros, bias, group_size)
-
-
-@_op.register_fake
-def _(x, packed, scales, zeros, bias, group_size):
-    return x.new_empty((x.shape[0], packed.shape[0]))
-
-
 def q4_linear(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None = None, bias: Tensor | None = None, *,
               group_size: int = 64) -> Tensor:
     """``x @ W.T + bias`` for x [..., K] (CUDA, float32 / bfloat16 / float16) and the
     weight W [N, K] that ``quantize_q4`` packed with the same ``group_size``; in x's
     dtype. Made for up to 64 tokens a call (more run in turns that read the weight
     again)."""
-    if x.ndim < 1:
-        raise ValueError("x must have at least one dimension")
-    _check_group(group_size)
-    k = x.shape[-1]
-    if packed.ndim != 2 or packed.dtype != torch.uint8 or packed.shape[1] != packed_pitch(k):
-        raise ValueError(f"packed must be uint8 [N, {packed_pitch(k)}] for {k} inputs; "
-                         f"got {packed.dtype} {list(packed.shape)}")
-    n = packed.shape[0]
-    need_shape("scales", scales, (n, -(-k // group_size)))
-    need_shape("zeros", zeros, (n, -(-k // group_size)))
-    need_shape("bias", bias, (n,))
-    if scales.dtype != torch.bfloat16 or (zeros is not None and zeros.dtype != torch.uint8):
-        raise ValueError("scales must be bfloat16 and zeros uint8")
-    code_of("x", x)
-    need_cuda("q4_linear", x, packed, scales, zeros, bias)
-    if not (packed.is_contiguous() and scales.is_contiguous() and (zeros is None or zeros.is_contiguous())):
-        raise ValueError("packed, scales and zeros must be contiguous")
-    no_grad_only("q4_linear", x, bias)
-    bias = parameter(bias)
-    flat = rows(x if x.ndim == 2 else x.reshape(-1, k))
-    if torch.compiler.is_compiling():
-        y = torch.ops.spikegpt_b200.q4_linear(flat, packed, scales, zeros, bias, group_size)
-    else:
-        guard = on_device(x)
-        if guard is not None:
-            with guard:
-                return q4_linear(x, packed, scales, zeros, bias, group_size=group_size)
-        y = _matvec(flat, packed, scales, zeros, bias, group_size)
-    return y if x.ndim == 2 else y.view(*x.shape[:-1], n)
+    return (_op or _native.op("q4_linear"))(x, packed, scales, zeros, bias, group_size)
