@@ -147,25 +147,27 @@ inline size_t norm_smem(bool backward, bool staged, size_t es, int span, int thr
   return n;
 }
 
-// The sums of u and v over the threads of a row (teams of `span` threads); `slot`
-// alternates between calls.
+// The sum of u (and of v: kTwo) over the threads of a row (teams of `span` threads);
+// `slot` alternates between calls.
+template <bool kTwo>
 __device__ __forceinline__ float2 norm_sums(float u, float v, int span, float2 (*red)[32], int slot) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     u += __shfl_xor_sync(kFull, u, o);
-    v += __shfl_xor_sync(kFull, v, o);
+    if (kTwo) v += __shfl_xor_sync(kFull, v, o);
   }
   if (span == 32) return make_float2(u, v);
   if ((threadIdx.x & 31) == 0) red[slot][threadIdx.x >> 5] = make_float2(u, v);
   __syncthreads();
-  const int warps = span >> 5, first = (threadIdx.x >> 5) / warps * warps;
-  float2 s = make_float2(0.f, 0.f);
-  for (int i = 0; i < warps; ++i) {
-    const float2 r = red[slot][first + i];
-    s.x += r.x;
-    s.y += r.y;
+  const int warps = span >> 5;  // lane i takes warp i's (the team's warps in turn, as often as they fit)
+  const float2 r = red[slot][((threadIdx.x >> 5) & ~(warps - 1)) + (threadIdx.x & (warps - 1))];
+  u = r.x;
+  v = r.y;
+  for (int o = warps >> 1; o > 0; o >>= 1) {
+    u += __shfl_xor_sync(kFull, u, o);
+    if (kTwo) v += __shfl_xor_sync(kFull, v, o);
   }
-  return s;
+  return make_float2(u, v);
 }
 
 // kThr: the CTA's threads, 256, 512 (rows past 4096) or 1024 (past 8192, where 64
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_fwd_kern
     row.load(static_cast<const T*>(a.x) + (r + step) * a.x_s, lane, a.span, a.C, r + step < a.rows);
 #pragma unroll
     for (int i = 0; i < P; ++i) s = add2(s, f[i]);
-    const float mu = norm_sums(s.x + s.y, 0.f, a.span, red, 0).x * inv;
+    const float mu = norm_sums<false>(s.x + s.y, 0.f, a.span, red, 0).x * inv;
     s = f2{0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_fwd_kern
       }
       s = fma2(f[i], f[i], s);
     }
-    const float rs = rsqrtf(norm_sums(s.x + s.y, 0.f, a.span, red, 1).x * inv + a.eps);
+    const float rs = rsqrtf(norm_sums<false>(s.x + s.y, 0.f, a.span, red, 1).x * inv + a.eps);
 #pragma unroll
     for (int i = 0; i < P; ++i) f[i] = fma2(mul2(f[i], splat(rs)), w[i], b[i]);
     Io::store(static_cast<T*>(a.y) + r * a.C, buf, lane, a.span, a.C, r < a.rows, f);
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_bwd_kern
       s1 = add2(s1, g[i]);
       s2 = fma2(g[i], h[i], s2);
     }
-    const float2 m = norm_sums(s1.x + s1.y, s2.x + s2.y, a.span, red, slot);
+    const float2 m = norm_sums<true>(s1.x + s1.y, s2.x + s2.y, a.span, red, slot);
     const f2 m1 = splat(m.x * inv), m2 = splat(-m.y * inv);
 #pragma unroll
     for (int i = 0; i < P; ++i) g[i] = mul2(fma2(h[i], m2, sub2(g[i], m1)), rs);

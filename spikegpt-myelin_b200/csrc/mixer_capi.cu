@@ -276,10 +276,10 @@ void scan_layout(ScanArgs& a, const ScanPlan& p, const ScanWs& w, int dtype, std
 // --------------------------------------------------------------- 4-bit weights
 
 // The most shared memory a launch of the kernel takes: the widest tile of tokens.
-template <class E, int R, int NT>
+template <class E, int R, int NT, int GW>
 constexpr size_t q4_smem_max() {
   constexpr int tokens = 8 * NT / Q4Type<E>::kTerms;
-  constexpr int a = kQ4Warps * q4_warp_bytes<E, R, NT>(tokens), b = q4_sum_bytes<R, NT>();
+  constexpr int a = kQ4MaxWarps * q4_warp_bytes<E, R, NT, GW>(tokens), b = q4_sum_bytes<R, NT>(kQ4MaxWarps);
   return a > b ? a : b;
 }
 
@@ -612,7 +612,8 @@ int selective_scan_step(int dtype, const void* x, const void* dt, const float* A
     constexpr int kLanesPer = decltype(lanes_)::value, kChannels = kScanStepThreads / kLanesPer;
     a.cblocks = (int)((C + kChannels - 1) / kChannels);
     launch(K_SCAN_STEP, st, [&] {
-      scan_step_kernel<decltype(e), kLanesPer><<<(unsigned)(B * a.cblocks), kScanStepThreads, 0, st>>>(a);
+      scan_step_kernel<decltype(e), kLanesPer>
+          <<<(unsigned)((B + kLanesPer - 1) / kLanesPer * a.cblocks), kScanStepThreads, 0, st>>>(a);
     });
     return launched("selective_scan step launch");
   };
@@ -742,7 +743,7 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
   a.pitch = (int)((K + 31) / 32 * 16);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int es = (int)dtype_size(dtype);
-  a.wide = vector_width(es, 16 / es, {x}, {x_stride, K}) == 16 / es;
+  const bool wide = vector_width(es, 16 / es, {x}, {x_stride, K}) == 16 / es;
   // floor(i / d) is the upper word of i * (floor(2^32 / d) + 1) while i * d < 2^32
   const int64_t d = std::min(group, (K + 31) / 32 * 32) / 32;
   a.group_magic = d > 1 ? (uint32_t)((1ull << 32) / d + 1) : 0;
@@ -753,20 +754,29 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
     const int tiles = (a.tokens * kTerms + 7) / 8;
     const int64_t my = (M + a.tokens - 1) / a.tokens;
     if (my > 65535) return fail(WKV_ERR_INVALID_ARGUMENT, "too many tokens: %lld", (long long)M);
-    auto go = [&](auto r, auto nt) {
-      constexpr int R = decltype(r)::value, NT = decltype(nt)::value;
-      // Warps along the inputs: at least three stages each where that leaves every SM a CTA.
+    auto launch_one = [&](auto r, auto nt, auto gw) {
+      constexpr int R = decltype(r)::value, NT = decltype(nt)::value, GW = decltype(gw)::value;
+      // Four warps a CTA where the rows alone make two such CTAs an SM, else eight; all of
+      // them along the inputs as long as each has three stages or rows are short of SMs.
       const int64_t chunks = (K + kQ4Chunk - 1) / kQ4Chunk;
-      auto ctas = [&](int wk) { return (N + 16 * R * (kQ4Warps / wk) - 1) / (16 * R * (kQ4Warps / wk)); };
-      a.wk = kQ4Warps;
+      const int warps = N >= 16 * R * 2 * sm_count() ? 4 : 8;
+      auto ctas = [&](int wk) { return (N + 16 * R * (warps / wk) - 1) / (16 * R * (warps / wk)); };
+      a.wk = warps;
       while (a.wk > 1 && chunks < 3 * a.wk && ctas(a.wk / 2) >= sm_count()) a.wk /= 2;
-      const int bytes = std::max(kQ4Warps * q4_warp_bytes<E, R, NT>(a.tokens), q4_sum_bytes<R, NT>());
-      const cudaError_t err = allow_smem(q4_matvec_kernel<E, R, NT>, q4_smem_max<E, R, NT>());
+      const int bytes = std::max(warps * q4_warp_bytes<E, R, NT, GW>(a.tokens), q4_sum_bytes<R, NT>(warps));
+      auto kernel = wide ? q4_matvec_kernel<E, R, NT, GW, true> : q4_matvec_kernel<E, R, NT, GW, false>;
+      const cudaError_t err = allow_smem(kernel, q4_smem_max<E, R, NT, GW>());
       if (err != cudaSuccess) return cuda_fail(err, "setting the q4_matvec kernel's shared memory size");
       launch(K_Q4, st, [&] {
-        q4_matvec_kernel<E, R, NT><<<dim3((unsigned)ctas(a.wk), (unsigned)my), kQ4Warps * 32, bytes, st>>>(a);
+        kernel<<<dim3((unsigned)ctas(a.wk), (unsigned)my), warps * 32, bytes, st>>>(a);
       });
       return launched("q4_matvec launch");
+    };
+    // Inputs scaled at a time: 128, 64 or 32, that always lie in one group.
+    auto go = [&](auto r, auto nt) {
+      if (a.groups == 1 || group % 128 == 0) return launch_one(r, nt, std::integral_constant<int, 4>{});
+      if (group % 64 == 0) return launch_one(r, nt, std::integral_constant<int, 2>{});
+      return launch_one(r, nt, std::integral_constant<int, 1>{});
     };
     // 32 rows a warp where that still gives two CTAs an SM: x is read and paired half as often
     if (tiles == 2) return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});

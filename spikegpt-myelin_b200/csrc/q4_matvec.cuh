@@ -11,22 +11,24 @@
 // float stands for 2^m + q, and less 2^m + zero it is exact. The products go to
 // m16n8k16 tiles (A the weights, B the tokens), whose k order is free: the pairs that a
 // word of eight nibbles gives, (0, 4), (1, 5), (2, 6), (3, 7), are taken as they come
-// and x is paired the same way. Four lanes' words make 32 inputs, always of one group,
-// whose sums are scaled in float32. float32 tokens enter as three bfloat16 terms
+// and x is paired the same way. Four lanes' words make 32 inputs (64 or 128 where the
+// group allows), always of one group, whose sums are scaled in float32. float32 tokens enter as three bfloat16 terms
 // (8 + 8 + 8 bits, exact) in three columns that are added at the end.
 //
-// The warps of a CTA are `wk` along the inputs (every wk-th 128 of them) by 8 / wk
-// along the rows; the sums along the inputs meet in shared memory in warp order.
+// The warps of a CTA are `wk` along the inputs (every wk-th 128 of them) by the
+// others along the rows; the sums along the inputs meet in shared memory in warp order.
 #pragma once
 
 #include "row_io.cuh"
 
 namespace wkv {
 
-constexpr int kQ4Warps = 8;
+constexpr int kQ4MaxWarps = 8;  // of a CTA: 4 or 8
 constexpr int kQ4Chunk = 128;  // inputs of a stage
 constexpr int kQ4Stages = 4;
-constexpr int kQ4Row = 80;  // bytes of a staged row of weights: 64 and a shift of the banks
+// Bytes of a staged row of weights, 64 and a shift: lanes read 4 GW bytes of eight rows
+// side by side, and no two rows of an access may meet in a bank.
+__host__ __device__ constexpr int q4_row_bytes(int GW) { return GW == 4 ? 64 : GW == 2 ? 96 : 80; }
 
 struct Q4Args {
   const void* x;  // [M][K]
@@ -39,7 +41,6 @@ struct Q4Args {
   int M, N, K, G, groups, pitch;
   int tokens;  // of a CTA
   int wk;      // warps along the inputs
-  int wide;    // rows of x are whole aligned 16-byte words
   uint32_t group_magic;  // the upper word of its product with k / 32 is the group (0: k / 32 is)
 };
 
@@ -55,6 +56,7 @@ struct Q4Type<float> {
   static constexpr int kTerms = 3;
 };
 
+// Packed arithmetic of the 16-bit type: kBase or-ed to a nibble is 2^m + nibble.
 template <typename H>
 struct Q4Math;
 template <>
@@ -66,10 +68,10 @@ struct Q4Math<__nv_bfloat16> {
     return d;
   }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                                             uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
 template <>
@@ -81,12 +83,19 @@ struct Q4Math<__half> {
     return d;
   }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                                             uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
+
+// (a & mask) | base: one operation with both constants in registers.
+__device__ __forceinline__ uint32_t q4_nibbles(uint32_t a, uint32_t mask, uint32_t base) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(mask), "r"(base));
+  return d;
+}
 
 // One tile of 16-bit tokens is read straight to registers a stage ahead (the rows of x
 // are short and stay in the L1 cache); more tokens, and float32 ones, are staged.
@@ -99,18 +108,18 @@ template <typename T>
 __host__ __device__ constexpr int q4_token_bytes() {
   return kQ4Chunk * (int)sizeof(T) + 64;
 }
-template <typename T, int R, int NT>
+template <typename T, int R, int NT, int GW>
 __host__ __device__ constexpr int q4_stage_bytes(int tokens) {
-  return R * 16 * kQ4Row + (q4_staged<T, NT>() ? tokens * q4_token_bytes<T>() : 0);
+  return R * 16 * q4_row_bytes(GW) + (q4_staged<T, NT>() ? tokens * q4_token_bytes<T>() : 0);
 }
-// A warp's ring and its scales and zeros (float, uint32_t) [2][16 R][4].
-template <typename T, int R, int NT>
+// A warp's ring and its scales and zeros (float, uint32_t) [2][16 R][4 / GW].
+template <typename T, int R, int NT, int GW>
 __host__ __device__ constexpr int q4_warp_bytes(int tokens) {
-  return kQ4Stages * q4_stage_bytes<T, R, NT>(tokens) + 2 * R * 16 * 4 * 8;
+  return kQ4Stages * q4_stage_bytes<T, R, NT, GW>(tokens) + 2 * R * 16 * (4 / GW) * 8;
 }
 template <int R, int NT>
-constexpr int q4_sum_bytes() {
-  return kQ4Warps * R * 16 * (8 * NT + 1) * 4;
+constexpr int q4_sum_bytes(int warps) {
+  return warps * R * 16 * (8 * NT + 1) * 4;
 }
 
 __device__ __forceinline__ void q4_copy(void* dst, const void* src, bool on) {
@@ -145,49 +154,48 @@ __device__ __forceinline__ void q4_inputs(const T* p, int term, uint32_t (&b)[4]
   }
 }
 
-template <typename T, int R, int NT>
-__global__ void __launch_bounds__(kQ4Warps * 32) q4_matvec_kernel(Q4Args a) {
+// GW: words of eight weights that a lane takes side by side, 1, 2 or 4: the four lanes'
+// 32, 64 or 128 inputs lie in one group, and are scaled at a time.
+// kWide: rows of x are whole aligned 16-byte words.
+template <typename T, int R, int NT, int GW, bool kWide>
+__global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a) {
   using H = typename Q4Type<T>::half;
   using Math = Q4Math<H>;
-  constexpr int kTerms = Q4Type<T>::kTerms, kTok = q4_token_bytes<T>();
+  constexpr int kTerms = Q4Type<T>::kTerms, kTok = q4_token_bytes<T>(), kRow = q4_row_bytes(GW);
+  constexpr int kSpans = 4 / GW, kEntries = 16 * R * kSpans, kPer = (kEntries + 31) / 32;
+  constexpr bool kStaged = q4_staged<T, NT>();
   extern __shared__ __align__(16) char smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
   const int wk = warp % a.wk, wn = warp / a.wk;
-  const int rows = 16 * R, cta_rows = rows * (kQ4Warps / a.wk);
+  constexpr int rows = 16 * R;
+  const int cta_rows = rows * ((int)blockDim.x / 32 / a.wk);
   const int n0 = blockIdx.x * cta_rows + wn * rows, m0 = blockIdx.y * a.tokens;
   const int tokens = min(a.tokens, a.M - m0);
-  const int stage_bytes = q4_stage_bytes<T, R, NT>(a.tokens);
-  char* ring = smem + warp * q4_warp_bytes<T, R, NT>(a.tokens);
+  const int stage_bytes = q4_stage_bytes<T, R, NT, GW>(a.tokens);
+  char* ring = smem + warp * q4_warp_bytes<T, R, NT, GW>(a.tokens);
   float2* sz = reinterpret_cast<float2*>(ring + kQ4Stages * stage_bytes);
   const int chunks = (a.K + kQ4Chunk - 1) / kQ4Chunk;
   const int mine = n0 < a.N && chunks > wk ? (chunks - wk + a.wk - 1) / a.wk : 0;
   const T* x = static_cast<const T*>(a.x) + m0 * a.x_s;
 
-  // where the lane reads: rows p * 8 + g, its quarter of each stage's inputs
+  // What the lane copies: its quarter of each stage's inputs of rows p * 8 + g. Rows past N
+  // stand in for the last one; inputs past K are zeros.
   const uint8_t* pq[2 * R];
-  const uint16_t* ps[2 * R];
-  const uint8_t* pz[2 * R];
 #pragma unroll
-  for (int p = 0; p < 2 * R; ++p) {
-    const int64_t row = min(n0 + p * 8 + g, a.N - 1);
-    pq[p] = a.q + row * a.pitch + wk * (kQ4Chunk / 2) + j * 16;
-    ps[p] = reinterpret_cast<const uint16_t*>(a.scale) + row * a.groups;
-    pz[p] = a.zero ? a.zero + row * a.groups : nullptr;
-  }
-  const int last32 = (a.K - 1) / 32;  // the row's last 32 inputs
+  for (int p = 0; p < 2 * R; ++p) pq[p] = a.q + (int64_t)min(n0 + p * 8 + g, a.N - 1) * a.pitch;
+  int copy_k = wk * kQ4Chunk + j * 32, copy_stage = 0;
   auto issue = [&](int i) {
     if (i < mine) {
-      const int k0 = (wk + i * a.wk) * kQ4Chunk;
-      char* to = ring + i % kQ4Stages * stage_bytes;
-      const bool on = k0 + j * 32 < a.K;
-      const int64_t at = (int64_t)i * a.wk * (kQ4Chunk / 2);
+      char* to = ring + copy_stage * stage_bytes;
+      const bool on = copy_k < a.K;
+      const int off = on ? copy_k >> 1 : 0;
 #pragma unroll
-      for (int p = 0; p < 2 * R; ++p)
-        q4_copy(to + (p * 8 + g) * kQ4Row + j * 16, on ? pq[p] + at : a.q, on);
-      if constexpr (q4_staged<T, NT>()) {
-        char* tx = to + rows * kQ4Row;
+      for (int p = 0; p < 2 * R; ++p) q4_copy(to + (p * 8 + g) * kRow + j * 16, pq[p] + off, on);
+      if constexpr (kStaged) {
+        char* tx = to + rows * kRow;
+        const int k0 = copy_k - j * 32;
         constexpr int kWords = kQ4Chunk * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
-        if (a.wide) {
+        if constexpr (kWide) {
           for (int p = lane; p < tokens * kWords; p += 32) {
             const int k = k0 + p % kWords * E;
             q4_copy(tx + p / kWords * kTok + p % kWords * 16, x + p / kWords * a.x_s + (k < a.K ? k : 0), k < a.K);
@@ -200,51 +208,55 @@ __global__ void __launch_bounds__(kQ4Warps * 32) q4_matvec_kernel(Q4Args a) {
           }
         }
       }
+      copy_k += a.wk * kQ4Chunk;
+      copy_stage = copy_stage + 1 == kQ4Stages ? 0 : copy_stage + 1;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // scales and zeros of the next stage, 32 inputs of a row each, and unstaged tokens
-  uint16_t fs[2 * R];
-  uint8_t fz[2 * R];
+  // The next stage's scales and zeros, kPer (row, span) pairs a lane, and unstaged tokens.
+  uint16_t fs[kPer];
+  uint8_t fz[kPer];
   uint4 fx[4];
-  const bool token = g < tokens;  // the lane's column is a token (one tile of 16-bit tokens)
-  const T* px = x + (token ? g * a.x_s : 0) + wk * kQ4Chunk + j * 8;
-  auto fetch = [&](int i) {
-    if (i >= mine) return;
-    const int k32 = min((wk + i * a.wk) * 4 + j, last32), group = a.group_magic ? __umulhi(k32, a.group_magic) : k32;
+  const T* px = x + (g < tokens ? g * a.x_s : 0);  // columns past the tokens are not written
+  int fetch_k = wk * kQ4Chunk;
+  auto fetch = [&]() {  // past the last stage: of inputs that exist, and are not used
 #pragma unroll
-    for (int p = 0; p < 2 * R; ++p) {
-      fs[p] = ps[p][group];
-      fz[p] = a.zero ? pz[p][group] : 8;
+    for (int p = 0; p < kPer; ++p) {
+      const int entry = p * 32 + lane, row = min(n0 + entry / kSpans % rows, a.N - 1);
+      const int k32 = (min(fetch_k + entry % kSpans * (32 * GW), a.K - 1)) >> 5;
+      const int64_t at = (int64_t)row * a.groups + (a.group_magic ? __umulhi(k32, a.group_magic) : k32);
+      fs[p] = reinterpret_cast<const uint16_t*>(a.scale)[at];
+      fz[p] = a.zero ? a.zero[at] : 8;
     }
-    if constexpr (!q4_staged<T, NT>()) {
-      const T* from = px + (int64_t)i * a.wk * kQ4Chunk;
-      const int k0 = (wk + i * a.wk) * kQ4Chunk + j * 8;
+    if constexpr (!kStaged) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const int k = k0 + w * 32;
-        fx[w] = make_uint4(0, 0, 0, 0);
-        if (token && k < a.K) {
-          if (a.wide) {
-            fx[w] = *reinterpret_cast<const uint4*>(from + w * 32);
-          } else {
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(from + w * 32);
-            uint32_t u[4];
+        const int k = fetch_k + j * 8 * GW + w / GW * (32 * GW) + w % GW * 8;
+        if constexpr (kWide) {
+          fx[w] = *reinterpret_cast<const uint4*>(px + min(k, a.K - 8));
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(px) + k;
+          uint32_t u[4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-              u[n] = (k + 2 * n < a.K ? h[2 * n] : 0u) | (k + 2 * n + 1 < a.K ? (uint32_t)h[2 * n + 1] << 16 : 0u);
-            fx[w] = make_uint4(u[0], u[1], u[2], u[3]);
-          }
+          for (int n = 0; n < 4; ++n)
+            u[n] = (k + 2 * n < a.K ? h[2 * n] : 0u) | (k + 2 * n + 1 < a.K ? (uint32_t)h[2 * n + 1] << 16 : 0u);
+          fx[w] = make_uint4(u[0], u[1], u[2], u[3]);
         }
       }
+      if (kWide && fetch_k + kQ4Chunk > a.K) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          if (fetch_k + j * 8 * GW + w / GW * (32 * GW) + w % GW * 8 >= a.K) fx[w] = make_uint4(0, 0, 0, 0);
+      }
     }
+    fetch_k += a.wk * kQ4Chunk;
   };
   auto keep = [&](int i) {
-    if (i >= mine) return;
 #pragma unroll
-    for (int p = 0; p < 2 * R; ++p)
-      sz[((i & 1) * rows + p * 8 + g) * 4 + j] =
-          make_float2(__uint_as_float((uint32_t)fs[p] << 16), __uint_as_float(Math::kBase + fz[p] * 0x10001u));
+    for (int p = 0; p < kPer; ++p)
+      if (kEntries % 32 == 0 || lane < kEntries)
+        sz[(i & 1) * kEntries + p * 32 + lane] =
+            make_float2(__uint_as_float((uint32_t)fs[p] << 16), __uint_as_float(Math::kBase + fz[p] * 0x10001u));
   };
 
   float acc[R][NT][4];
@@ -252,53 +264,74 @@ __global__ void __launch_bounds__(kQ4Warps * 32) q4_matvec_kernel(Q4Args a) {
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[r][t][0] = acc[r][t][1] = acc[r][t][2] = acc[r][t][3] = 0.f;
-  fetch(0);
+  const float none[4] = {0.f, 0.f, 0.f, 0.f};
+  uint32_t mask = 0x000f000fu, base = Math::kBase;
+  asm volatile("" : "+r"(mask), "+r"(base));  // in registers: an instruction holds one constant
+  if (mine > 0) fetch();
 #pragma unroll
   for (int i = 0; i < kQ4Stages - 1; ++i) issue(i);
-  keep(0);
+  if (mine > 0) keep(0);
+  int stage = 0;
   for (int i = 0; i < mine; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kQ4Stages - 2) : "memory");
     __syncwarp();  // the stage and its scales are there, and every lane is done with the stage before
     issue(i + kQ4Stages - 1);
-    const uint4 cx[4] = {fx[0], fx[1], fx[2], fx[3]};
-    fetch(i + 1);
-    const char* from = ring + i % kQ4Stages * stage_bytes;
-    const float2* sc = sz + (i & 1) * rows * 4;
+    uint32_t bx[4][4];  // the unstaged tokens' operands: their words are free for the next stage's
+    if constexpr (!kStaged)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      uint32_t b[NT][4];
+      for (int w = 0; w < 4; ++w) q4_pairs(fx[w], bx[w]);
+    fetch();
+    const char* from = ring + stage * stage_bytes + g * kRow + j * 4 * GW;
+    const char* tx = ring + stage * stage_bytes + rows * kRow + j * 8 * GW * sizeof(T);
+    const float2* sc = sz + (i & 1) * kEntries + g * kSpans;
+    stage = stage + 1 == kQ4Stages ? 0 : stage + 1;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int column = t * 8 + g;
-        if constexpr (!q4_staged<T, NT>())
-          q4_pairs(cx[w], b[t]);
-        else if (column < tokens * kTerms)
-          q4_inputs(reinterpret_cast<const T*>(from + rows * kQ4Row + column / kTerms * kTok) + w * 32 + j * 8,
-                    column % kTerms, b[t]);
-        else
-          b[t][0] = b[t][1] = b[t][2] = b[t][3] = 0;
-      }
+    for (int span = 0; span < kSpans; ++span) {
+      uint32_t b[GW][NT][4];
+#pragma unroll
+      for (int w = 0; w < GW; ++w)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int column = t * 8 + g;
+          if constexpr (!kStaged) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) b[w][t][n] = bx[span * GW + w][n];
+          } else if (column < tokens * kTerms)
+            q4_inputs(reinterpret_cast<const T*>(tx + column / kTerms * kTok) + span * 32 * GW + w * 8, column % kTerms,
+                      b[w][t]);
+          else
+            b[w][t][0] = b[w][t][1] = b[w][t][2] = b[w][t][3] = 0;
+        }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int row = r * 16 + g;
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(from + row * kQ4Row + w * 16 + j * 4);
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(from + (row + 8) * kQ4Row + w * 16 + j * 4);
-        const float2 su = sc[row * 4 + w], sv = sc[(row + 8) * 4 + w];
-        uint32_t p[4], q[4];
+        using Words = Vec<uint32_t, GW>;
+        const Words u = Words::load(reinterpret_cast<const uint32_t*>(from + r * 16 * kRow + span * 16 * GW));
+        const Words v = Words::load(reinterpret_cast<const uint32_t*>(from + (r * 16 + 8) * kRow + span * 16 * GW));
+        const float2 su = sc[r * 16 * kSpans + span], sv = sc[(r * 16 + 8) * kSpans + span];
+        float d[NT][4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          p[n] = Math::sub((u >> (4 * n) & 0x000f000fu) | Math::kBase, __float_as_uint(su.y));
-          q[n] = Math::sub((v >> (4 * n) & 0x000f000fu) | Math::kBase, __float_as_uint(sv.y));
+        for (int w = 0; w < GW; ++w) {
+          uint32_t p[4], q[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            p[n] = Math::sub(q4_nibbles(u.e[w] >> (4 * n), mask, base), __float_as_uint(su.y));
+            q[n] = Math::sub(q4_nibbles(v.e[w] >> (4 * n), mask, base), __float_as_uint(sv.y));
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (w == 0)
+              Math::mma(d[t], p[0], q[0], p[1], q[1], b[w][t][0], b[w][t][1], none);
+            else
+              Math::mma(d[t], p[0], q[0], p[1], q[1], b[w][t][0], b[w][t][1], d[t]);
+            Math::mma(d[t], p[2], q[2], p[3], q[3], b[w][t][2], b[w][t][3], d[t]);
+          }
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          Math::mma(d, p[0], q[0], p[1], q[1], b[t][0], b[t][1]);
-          Math::mma(d, p[2], q[2], p[3], q[3], b[t][2], b[t][3]);
-          acc[r][t][0] = fmaf(su.x, d[0], acc[r][t][0]);
-          acc[r][t][1] = fmaf(su.x, d[1], acc[r][t][1]);
-          acc[r][t][2] = fmaf(sv.x, d[2], acc[r][t][2]);
-          acc[r][t][3] = fmaf(sv.x, d[3], acc[r][t][3]);
+          acc[r][t][0] = fmaf(su.x, d[t][0], acc[r][t][0]);
+          acc[r][t][1] = fmaf(su.x, d[t][1], acc[r][t][1]);
+          acc[r][t][2] = fmaf(sv.x, d[t][2], acc[r][t][2]);
+          acc[r][t][3] = fmaf(sv.x, d[t][3], acc[r][t][3]);
         }
       }
     }
@@ -316,16 +349,16 @@ __global__ void __launch_bounds__(kQ4Warps * 32) q4_matvec_kernel(Q4Args a) {
       for (int i = 0; i < 4; ++i)
         sum[(warp * rows + r * 16 + g + i / 2 * 8) * kPitch + t * 8 + j * 2 + i % 2] = acc[r][t][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < cta_rows * tokens; i += kQ4Warps * 32) {
-    const int row = i % cta_rows, token = i / cta_rows, n = blockIdx.x * cta_rows + row;
+  for (int i = threadIdx.x; i < cta_rows * tokens; i += blockDim.x) {
+    const int row = i % cta_rows, t = i / cta_rows, n = blockIdx.x * cta_rows + row;
     if (n >= a.N) continue;
     float s = 0.f;
     for (int k = 0; k < a.wk; ++k)
 #pragma unroll
-      for (int t = 0; t < kTerms; ++t)
-        s += sum[((row / rows * a.wk + k) * rows + row % rows) * kPitch + token * kTerms + t];
+      for (int e = 0; e < kTerms; ++e)
+        s += sum[((row / rows * a.wk + k) * rows + row % rows) * kPitch + t * kTerms + e];
     if (a.bias) s += a.bias[n];
-    static_cast<T*>(a.y)[(int64_t)(m0 + token) * a.N + n] = Pair<T>::from_float(s);
+    static_cast<T*>(a.y)[(int64_t)(m0 + t) * a.N + n] = Pair<T>::from_float(s);
   }
 }
 

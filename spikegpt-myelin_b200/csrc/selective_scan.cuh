@@ -929,45 +929,69 @@ __global__ void __launch_bounds__(256) scan_reduce_kernel(const float* part, int
 
 // One token: x, dt, z [B][C] and B, C [B][N]; the state is updated in place. LPC
 // lanes share a channel, four states each, so a warp reads and writes 512 contiguous
-// bytes of the state, which is nearly all the traffic there is.
+// bytes of the state, which is nearly all the traffic there is. The lanes take LPC
+// sequences together: each works out one sequence's step (its softplus and its gate)
+// and hands it to the others.
 constexpr int kScanStepThreads = 128;
 template <typename T, int LPC>
 __global__ void __launch_bounds__(kScanStepThreads) scan_step_kernel(ScanArgs a) {
   constexpr int kChannels = kScanStepThreads / LPC;
-  const int q = threadIdx.x % LPC, b = blockIdx.x / a.cblocks;
+  const int q = threadIdx.x % LPC, b0 = blockIdx.x / a.cblocks * LPC;
   const int c0 = blockIdx.x % a.cblocks * kChannels + threadIdx.x / LPC;
   const bool mine = c0 < a.C;
-  const int c = mine ? c0 : a.C - 1;
-  float* hp = a.h_last + ((int64_t)b * a.C + c) * a.N;
-  States<4> h = States<4>::load(hp, 4 * q, a.N, a.wide_n);
+  const int c = mine ? c0 : a.C - 1, own = min(b0 + q, a.B - 1), rows = min(LPC, a.B - b0);
+  float* hp = a.h_last + ((int64_t)b0 * a.C + c) * a.N;
+  const int64_t pitch = (int64_t)a.C * a.N;
+  constexpr int kAhead = LPC < 4 ? LPC : 4;  // sequences whose states are under way at a time
   States<4> A2 = States<4>::load(a.A + (int64_t)c * a.N, 4 * q, a.N, a.wide_n);
-  const Vec<T, 4> rB = load_bc(static_cast<const T*>(a.Bm) + b * a.b_sb, 4 * q, a.N, true, a.wide_bc);
-  const Vec<T, 4> rC = load_bc(static_cast<const T*>(a.Cm) + b * a.c_sb, 4 * q, a.N, true, a.wide_bc);
-  const float x = Pair<T>::scalar(static_cast<const T*>(a.x)[b * a.x_sb + c]);
-  const float raw = Pair<T>::scalar(static_cast<const T*>(a.dt)[b * a.dt_sb + c]);
-  const float z = a.z ? Pair<T>::scalar(static_cast<const T*>(a.z)[b * a.z_sb + c]) : 0.f;
+  const float x = Pair<T>::scalar(static_cast<const T*>(a.x)[own * a.x_sb + c]);
+  const float raw = Pair<T>::scalar(static_cast<const T*>(a.dt)[own * a.dt_sb + c]);
+  const float z = a.z ? Pair<T>::scalar(static_cast<const T*>(a.z)[own * a.z_sb + c]) : 0.f;
   const float D = a.D ? a.D[c] : 0.f, bias = a.bias ? a.bias[c] : 0.f;
-  const f2 d = scan_delta(splat(raw + bias), a.softplus), w = mul2(d, splat(x));
-  float fB[4], fC[4];
-  rB.get(fB);
-  rC.get(fC);
+  float y[LPC];
+  f2 d, w;
   A2.scale(kL2E);
-  f2 y{0.f, 0.f};
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    h.p[n] = fma2(ex2x2(mul2(A2.p[n], d)), h.p[n], mul2(f2{fB[2 * n], fB[2 * n + 1]}, w));
-    y = fma2(h.p[n], f2{fC[2 * n], fC[2 * n + 1]}, y);
-  }
-  float s = y.x + y.y;
+  for (int r0 = 0; r0 < LPC; r0 += kAhead) {
+    States<4> h[kAhead];
+    Vec<T, 4> rB[kAhead], rC[kAhead];
 #pragma unroll
-  for (int o = 1; o < LPC; o *= 2) s += __shfl_xor_sync(kFull, s, o);
-  if (!mine) return;
-  h.store(hp, 4 * q, a.N, a.wide_n);
-  if (q == 0) {
-    s = fmaf(D, x, s);
-    if (a.z) s *= z * sigmoid1(z);
-    static_cast<T*>(a.out)[(int64_t)b * a.C + c] = Pair<T>::from_float(s);
+    for (int i = 0; i < kAhead; ++i) {
+      const int r = r0 + i;
+      h[i] = States<4>::zero();
+      rB[i] = rC[i] = Vec<T, 4>::zero();
+      if (r < rows) {
+        h[i] = States<4>::load(hp + r * pitch, 4 * q, a.N, a.wide_n);
+        rB[i] = load_bc(static_cast<const T*>(a.Bm) + (b0 + r) * a.b_sb, 4 * q, a.N, true, a.wide_bc);
+        rC[i] = load_bc(static_cast<const T*>(a.Cm) + (b0 + r) * a.c_sb, 4 * q, a.N, true, a.wide_bc);
+      }
+    }
+    if (r0 == 0) {
+      d = scan_delta(splat(raw + bias), a.softplus);
+      w = mul2(d, splat(x));
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int r = r0 + i;
+      const f2 dr = splat(__shfl_sync(kFull, d.x, r, LPC)), wr = splat(__shfl_sync(kFull, w.x, r, LPC));
+      float fB[4], fC[4];
+      rB[i].get(fB);
+      rC[i].get(fC);
+      f2 v{0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        h[i].p[n] = fma2(ex2x2(mul2(A2.p[n], dr)), h[i].p[n], mul2(f2{fB[2 * n], fB[2 * n + 1]}, wr));
+        v = fma2(h[i].p[n], f2{fC[2 * n], fC[2 * n + 1]}, v);
+      }
+      y[r] = v.x + v.y;
+      if (mine && r < rows) h[i].store(hp + r * pitch, 4 * q, a.N, a.wide_n);
+    }
   }
+  reduce_scatter<LPC, LPC, 1>(y);
+  if (!mine || q >= rows) return;
+  float s = fmaf(D, x, y[0]);
+  if (a.z) s *= z * sigmoid1(z);
+  static_cast<T*>(a.out)[(int64_t)own * a.C + c] = Pair<T>::from_float(s);
 }
 
 }  // namespace wkv
