@@ -23,7 +23,7 @@ using namespace wkv_host;
 
 constexpr int64_t kMaxDim = 1ll << 30;
 constexpr int kScanMaxSegments = 64;
-constexpr int kScanMinSegment = 64;
+constexpr int kScanMinSegment = 32;
 
 // Calls f with a value of the dtype's element type.
 template <class F>
@@ -226,7 +226,7 @@ ScanPlan scan_forward_plan(int64_t B, int64_t T, int64_t C, int64_t N) {
   return scan_plan(B, T, C, kScanThreads / scan_lanes(N, 8), 6 * sm_count());
 }
 ScanPlan scan_backward_plan(int64_t B, int64_t T, int64_t C, int64_t N) {
-  return scan_plan(B, T, C, kScanBwdPer * kScanBwdThreads / scan_lanes(N, 4), 2 * sm_count());
+  return scan_plan(B, T, C, kScanBwdPer * kScanBwdThreads / scan_lanes(N, 4), 3 * sm_count());
 }
 
 struct ScanWs {

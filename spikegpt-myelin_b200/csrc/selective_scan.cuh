@@ -494,74 +494,54 @@ __device__ __forceinline__ void copy16(void* dst, const void* src, bool on) {
                : "memory");
 }
 
-// D += A B for one m16n8k8 tile of tf32 factors with float32 sums.
+// D = A B + C for one m16n8k8 tile of tf32 factors with float32 sums.
 __device__ __forceinline__ void mma_tf32(float (&d)[4], float a0, float a1, float a2, float a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                                         uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)),
-        "r"(b0), "r"(b1));
+        "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-// Sums over a warp's channels with the tensor core. The lanes of a channel sit
-// 32 / LPC apart, so the four lanes of a tile's k group are channels of one state
-// quad (LPC = 16: two channels of two quads), and a column is one lane group. A pair
-// of values is a B operand as it lies in its two registers; the A operand is a 0/1
-// matrix that adds value r of four into row 2 r (LPC = 16: the second quad's into row
-// 2 r + 1). Two A operands serve both accumulators, gB's and gC's, because the rows
-// from 8 on may hold anything: they get value r in row 2 r + 9. Shuffles take 28
-// instructions a step for these sums, this 20.
+// Sums over the lanes of a channel with the tensor core, where at least four lanes
+// share one. The four lanes of a tile's k group belong to one channel and a column is
+// a lane group: a channel, or a half or quarter of one. A pair of values is a B
+// operand as it lies in its two registers; the A operand is a 0/1 matrix that adds
+// value r of four into row 2 r. Two A operands serve all tiles, because the rows from
+// 8 on may hold anything: they get value r in row 2 r + 9, from where the odd lane
+// groups read it. A step's three sums of two channels take 16 instructions this way,
+// by shuffles 36.
 //
 // A term enters as the sum of two tf32 values, its upper 11 bits and the rest, which
 // keeps 21 bits and more of it (rounded once to 11 bits, a sum that cancels would lose
 // more than the result's own rounding to bfloat16 does). A term that is infinite or
 // NaN makes the neighbouring rows of its tile NaN.
-template <int LPC>
-struct ChannelSums {
+struct StateSums {
   float sel[8];  // two A operands: for the values 0, 1 and for 2, 3
 
   __device__ __forceinline__ void init() {
-    const int row = threadIdx.x % 32 / 4, odd = threadIdx.x / 2 % 2;  // LPC = 16: the quad of the lane's k
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      sel[r] = row == (LPC == 16 ? r / 2 * 2 + odd : r) ? 1.f : 0.f;
+      sel[r] = threadIdx.x % 32 / 4 == r ? 1.f : 0.f;
       asm volatile("" : "+f"(sel[r]));  // stays in its register: rebuilding an operand costs more than its product
     }
   }
-  // adds the four values of a step to a tile
-  __device__ __forceinline__ void add(float (&d)[4], f2 v, f2 w) const {
+  // the tile of four values
+  __device__ __forceinline__ void sum(float (&d)[4], f2 v, f2 w) const {
     const f2 vh{__uint_as_float(__float_as_uint(v.x) & 0xffffe000u), __uint_as_float(__float_as_uint(v.y) & 0xffffe000u)};
     const f2 wh{__uint_as_float(__float_as_uint(w.x) & 0xffffe000u), __uint_as_float(__float_as_uint(w.y) & 0xffffe000u)};
     const f2 vl = sub2(v, vh), wl = sub2(w, wh);
-    mma_tf32(d, sel[0], sel[1], sel[2], sel[3], __float_as_uint(vh.x), __float_as_uint(vh.y));
-    mma_tf32(d, sel[4], sel[5], sel[6], sel[7], __float_as_uint(wh.x), __float_as_uint(wh.y));
-    mma_tf32(d, sel[0], sel[1], sel[2], sel[3], __float_as_uint(vl.x), __float_as_uint(vl.y));
-    mma_tf32(d, sel[4], sel[5], sel[6], sel[7], __float_as_uint(wl.x), __float_as_uint(wl.y));
-  }
-  // to[B: 0 .. NP, C: NP .. 2 NP): the warp's sums of a step
-  __device__ __forceinline__ void store(const float (&dB)[4], const float (&dC)[4], float* to) const {
-    constexpr int NP = 4 * LPC;
-    const int row = threadIdx.x % 32 / 4, j = threadIdx.x % 4;
-    if constexpr (LPC == 16) {  // columns 2 j and 2 j + 1: the quads' pairs
-      to += row / 2 + 4 * (4 * j + row % 2);
-      to[0] = dB[0];
-      to[8] = dB[1];
-      to[NP] = dC[0];
-      to[NP + 8] = dC[1];
-    } else {  // even rows hold gB's values, odd ones (from row 9 on) gC's
-      to += (row % 2) * NP + row / 2;
-      const float u0 = row % 2 ? dC[2] : dB[0], u1 = row % 2 ? dC[3] : dB[1];
-      if constexpr (LPC == 8) {  // columns: quads
-        to[4 * (2 * j)] = u0;
-        to[4 * (2 * j + 1)] = u1;
-      } else {  // columns: 8 / LPC lane groups of each quad
-        float u = u0 + u1;
-#pragma unroll
-        for (int m = 1; m < 4 / LPC; m *= 2) u += __shfl_xor_sync(kFull, u, m);
-        if (j % (4 / LPC) == 0) to[4 * (j / (4 / LPC))] = u;
-      }
-    }
+    const float none[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_tf32(d, sel[0], sel[1], sel[2], sel[3], __float_as_uint(vh.x), __float_as_uint(vh.y), none);
+    mma_tf32(d, sel[4], sel[5], sel[6], sel[7], __float_as_uint(wh.x), __float_as_uint(wh.y), d);
+    mma_tf32(d, sel[0], sel[1], sel[2], sel[3], __float_as_uint(vl.x), __float_as_uint(vl.y), d);
+    mma_tf32(d, sel[4], sel[5], sel[6], sel[7], __float_as_uint(wl.x), __float_as_uint(wl.y), d);
   }
 };
+// The lane's pair of columns of value (lane / 8) of two tiles: the even lane groups'
+// from tile a, the odd ones' from tile b.
+__device__ __forceinline__ f2 tile_pair(const float (&a)[4], const float (&b)[4]) {
+  return threadIdx.x & 4 ? f2{b[2], b[3]} : f2{a[0], a[1]};
+}
 
 // Shared memory of the backward kernel (see there), in bytes from the start.
 constexpr int kScanBwdThreads = 128;
@@ -585,9 +565,9 @@ struct ScanBwdSmem {
 // steps. Per sub-chunk of 8 steps a thread runs four states of its two channels
 // forward from the kept states, with p_t = a_t h_{t-1} in registers, and then back
 // with the adjoint (a_t again from the exponential unit, which has the time: held in
-// registers it would cost a quarter of the resident warps). The sums over states (for gx, gdt, gz) are exchanged among the
-// channel's lanes, the sums over channels (gB, gC) go through the tensor core, are
-// added over the warps and left as one partial row of the CTA's channels.
+// registers it would cost a quarter of the resident warps). The sums over states (for
+// gx, gdt, gz) go through the tensor core, the sums over channels (gB, gC) are
+// exchanged among the lanes, added over the warps and left as one partial row of the CTA's channels.
 template <typename T, int LPC>
 __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a) {
   using L = ScanBwdSmem<T, LPC>;
@@ -602,7 +582,7 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
   float* sbc = reinterpret_cast<float*>(smem + L::kBC);
   float* res = reinterpret_cast<float*>(smem + L::kRes);      // sum g B, sum A g p log2(e), sum C h of a cell
   float* part = reinterpret_cast<float*>(smem + L::kPart);
-  const int tid = threadIdx.x, warp = tid / 32, q = tid % 32 / kLane, ch = warp * kLane * kPer + tid % kLane;
+  const int tid = threadIdx.x, warp = tid / 32, q = tid % LPC, ch = warp * kLane * kPer + tid % 32 / LPC;
   const int cb = blockIdx.x % a.cblocks, seg = blockIdx.x / a.cblocks % a.nseg, b = blockIdx.x / a.cblocks / a.nseg;
   const int c0 = cb * CH, c = c0 + ch;  // and c + kLane
   const int len = scan_length(a, b);
@@ -698,7 +678,7 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
   };
 
   const int tiles = t_live > t_begin ? (t_live - t_begin + TS - 1) / TS : 0;
-  ChannelSums<LPC> sums;
+  StateSums sums;
   sums.init();
   if (tiles > 0) {
     fetch(t_begin + (tiles - 1) * TS, 0);
@@ -776,13 +756,14 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
 #pragma unroll
       for (int u = 0; u < kPer; ++u) gAs[u] = St::zero();
 #pragma unroll
-      for (int half = 1; half >= 0; --half) {
-        float along[kPer][4], gd[kPer][4], y[kPer][4];
+      for (int two = 3; two >= 0; --two) {  // two steps at a time
+        f2 along[2], gd[2], y[2];           // of the thread's two channels
 #pragma unroll
-        for (int ii = 3; ii >= 0; --ii) {
-          const int i = half * 4 + ii;
+        for (int ii = 1; ii >= 0; --ii) {
+          const int i = two * 2 + ii;
           const St Bt = St::shared(bc + i * 2 * NP), Ct = St::shared(bc + i * 2 * NP + NP);
           f2 sumB[2], sumC[2];
+          float ra[kPer], rg[kPer], ry[kPer];
 #pragma unroll
           for (int u = 0; u < kPer; ++u) {
             const float4 s = sl[i * CH + u * kLane];
@@ -801,30 +782,64 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
               gAs[u].p[n] = fma2(v, d, gAs[u].p[n]);
               g[u].p[n] = mul2(gn, ex2x2(mul2(A2[u].p[n], d)));
             }
-            along[u][ii] = al.x + al.y;
-            y[u][ii] = yy.x + yy.y;
-            gd[u][ii] = dd.x + dd.y;
+            ra[u] = al.x + al.y;
+            ry[u] = yy.x + yy.y;
+            rg[u] = dd.x + dd.y;
           }
-          float tileB[4] = {0.f, 0.f, 0.f, 0.f}, tileC[4] = {0.f, 0.f, 0.f, 0.f};
-          sums.add(tileB, sumB[0], sumB[1]);
-          sums.add(tileC, sumC[0], sumC[1]);
-          sums.store(tileB, tileC, part + ((sub * 8 + i) * L::kWarps + warp) * 2 * NP);
-        }
-        constexpr int kOwn = LPC <= 4 ? 4 / LPC : 1, kSkip = LPC <= 4 ? 1 : LPC / 4;
+          along[ii] = f2{ra[0], ra[1]};
+          gd[ii] = f2{rg[0], rg[1]};
+          y[ii] = f2{ry[0], ry[1]};
+          // over the warp's channels: lane group l keeps sum l of (B: 0..3, C: 4..7) of its quad
+          float v[8] = {sumB[0].x, sumB[0].y, sumB[1].x, sumB[1].y, sumC[0].x, sumC[0].y, sumC[1].x, sumC[1].y};
+          reduce_scatter<8, kLane, LPC>(v);
+          constexpr int kOwn = kLane < 8 ? 8 / kLane : 1, kSkip = kLane < 8 ? 1 : kLane / 8;
+          const int l = tid % 32 / LPC;
+          if (l % kSkip == 0) {
+            float* pw = part + ((sub * 8 + i) * L::kWarps + warp) * 2 * NP + 4 * q;
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) {
-          reduce_scatter<4, LPC, kLane>(along[u]);
-          reduce_scatter<4, LPC, kLane>(gd[u]);
-          reduce_scatter<4, LPC, kLane>(y[u]);
-          if (q % kSkip == 0) {
-            float* to = res + (sub * 8 + half * 4 + q / kSkip * kOwn) * L::kPitch + ch + u * kLane;
-#pragma unroll
-            for (int i = 0; i < kOwn; ++i, to += L::kPitch) {
-              to[0] = along[u][i];
-              to[TS * L::kPitch] = gd[u][i];
-              to[2 * TS * L::kPitch] = y[u][i];
+            for (int k = 0; k < kOwn; ++k) {
+              const int at = l / kSkip * kOwn + k;
+              pw[at < 4 ? at : NP + at - 4] = v[k];
             }
           }
+        }
+        float* to = res + (sub * 8 + two * 2) * L::kPitch;  // step two * 2; the other is a row on
+        if constexpr (LPC >= 4) {
+          float t0_[4], t1_[4], ty[4];
+          sums.sum(t0_, along[0], gd[0]);
+          sums.sum(t1_, along[1], gd[1]);
+          sums.sum(ty, y[0], y[1]);
+          f2 s = tile_pair(t0_, t1_), r = tile_pair(ty, ty);
+          // value (lane / 8): along of channel 0, of channel 1, gd of each; y of each at step 0, at step 1
+          const int k = tid % 32 / 8, step = tid / 4 % 2, col = tid % 4 * 2, c8 = warp * kLane * kPer + k % 2 * kLane;
+          float* ps = to + k / 2 * TS * L::kPitch + step * L::kPitch + c8;
+          float* pr = to + 2 * TS * L::kPitch + k / 2 * L::kPitch + c8;
+          if constexpr (LPC == 4) {  // a column is a channel
+            *reinterpret_cast<float2*>(ps + col) = make_float2(s.x, s.y);
+            if (step == 0) *reinterpret_cast<float2*>(pr + col) = make_float2(r.x, r.y);
+          } else {
+            float su = s.x + s.y, ru = r.x + r.y;  // two columns a channel, or four
+            if constexpr (LPC == 16) {
+              su += __shfl_xor_sync(kFull, su, 1);
+              ru += __shfl_xor_sync(kFull, ru, 1);
+            }
+            if (LPC == 8 || tid % 2 == 0) {
+              ps[col / (LPC / 4)] = su;
+              if (step == 0) pr[col / (LPC / 4)] = ru;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) {
+              float v[3] = {u ? along[ii].y : along[ii].x, u ? gd[ii].y : gd[ii].x, u ? y[ii].y : y[ii].x};
+#pragma unroll
+              for (int k = 0; k < 3; ++k) {
+                if constexpr (LPC == 2) v[k] += __shfl_xor_sync(kFull, v[k], 1);
+                if (q == 0) to[k * TS * L::kPitch + ii * L::kPitch + ch + u * kLane] = v[k];
+              }
+            }
         }
       }
       // gA: eight steps' sum at a time, which keeps the long sum's rounding small
@@ -880,14 +895,19 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
         gb = add2(gb, gdt);
       }
     }
-    for (int i = tid; i < TS * 2 * NP; i += kThr) {
-      const int r = i / (2 * NP), j = i % (2 * NP), n = j < NP ? j : j - NP;
-      if (t0 + r >= t_live || n >= a.N) continue;
-      const float* p = part + r * L::kWarps * 2 * NP + j;
-      float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < L::kWarps; ++w) s += p[w * 2 * NP];
-      pbc[(int64_t)(t0 + r) * 2 * a.N + (j < NP ? n : a.N + n)] = s;
+    for (int k = 0; k < (TS * 2 * LPC + kThr - 1) / kThr; ++k) {
+      const int i = k * kThr + tid, r = i / (2 * LPC), j = i % (2 * LPC) * 4, n = j < NP ? j : j - NP;
+      if (i >= TS * 2 * LPC || t0 + r >= t_live) break;
+      const float* p = part + r * L::kWarps * 2 * NP + j;
+      States<4> s = States<4>::shared(p);
+#pragma unroll
+      for (int w = 1; w < L::kWarps; ++w) {
+        const States<4> o = States<4>::shared(p + w * 2 * NP);
+        s.p[0] = add2(s.p[0], o.p[0]);
+        s.p[1] = add2(s.p[1], o.p[1]);
+      }
+      s.store(pbc + (int64_t)(t0 + r) * 2 * a.N + (j < NP ? 0 : a.N), n, a.N, a.wide_n);
     }
   }
 #pragma unroll
