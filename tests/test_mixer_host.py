@@ -95,3 +95,21 @@ def test_size_queries():
         assert lib.selective_scan_state_size(b, t, c, n) == _kept_bytes(b, t, c, n)
     assert lib.causal_conv_workspace_size(2, 100, 64, 5) == 0  # an invalid width
     assert lib.layer_norm_workspace_size(0, 0, 64) == 0
+
+
+def test_selective_model_builds_and_quantizes_on_the_cpu():
+    from spikegpt_b200.selective_model import Q4Linear, SelectiveConfig, SelectiveLM
+
+    with pytest.raises(ValueError):
+        SelectiveLM(SelectiveConfig(n_state=65))
+    with pytest.raises(ValueError):
+        SelectiveLM(SelectiveConfig(taps=5))
+    model = SelectiveLM(SelectiveConfig(vocab_size=33, n_layer=2, n_embd=24, n_state=4))
+    assert model.blocks[0].in_proj.weight.shape == (96, 24) and model.blocks[0].A_log.shape == (48, 4)
+    head = model.head.weight.detach().clone()
+    model.quantize_(32)
+    assert isinstance(model.head, Q4Linear) and model.head.weight().shape == head.shape
+    assert (model.head.weight() - head).abs().max() <= 0.1 * head.abs().max()
+    again = SelectiveLM(SelectiveConfig(vocab_size=33, n_layer=2, n_embd=24, n_state=4)).quantize_(32)
+    again.load_state_dict(model.state_dict())
+    assert torch.equal(again.head.weight(), model.head.weight())
