@@ -524,7 +524,7 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], float a0, float a1, floa
 // A term enters as the sum of two tf32 values, its upper 11 bits and the rest, which
 // keeps 21 bits and more of it (rounded once to 11 bits, a sum that cancels would lose
 // more than the result's own rounding to bfloat16 does). A term that is infinite or
-// NaN makes the neighbouring rows of its tile NaN.
+// NaN makes all rows of its tile NaN: the caller then adds by shuffles instead.
 struct StateSums {
   float sel[8];  // two A operands: for the values 0, 1 and for 2, 3
 
@@ -568,7 +568,8 @@ struct ScanBwdSmem {
   static constexpr int kBC = kRaw + 8 * kCells * (int)sizeof(T);     // float [TS][2 NP]
   static constexpr int kRes = kBC + TS * 2 * S::NP * 4;              // float [3][TS][kPitch]
   static constexpr int kPart = kRes + 3 * TS * kPitch * 4;           // float [TS][warps][2 NP]
-  static constexpr int kBytes = kPart + TS * kWarps * 2 * S::NP * 4;
+  static constexpr int kHeld = kPart + TS * kWarps * 2 * S::NP * 4;  // float [threads][4 kPer]
+  static constexpr int kBytes = kHeld + (LPC >= 4 ? kScanBwdThreads * 4 * kScanBwdPer * 4 : 0);
 };
 
 // A CTA walks one segment of CH channels of one sequence backwards, in tiles of TS
@@ -763,8 +764,13 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
         }
       }
       St gAs[kPer];
+      f2 check{0.f, 0.f};
+      float* held = reinterpret_cast<float*>(smem + L::kHeld) + tid * 4 * kPer;  // the adjoint as these steps get it
 #pragma unroll
-      for (int u = 0; u < kPer; ++u) gAs[u] = St::zero();
+      for (int u = 0; u < kPer; ++u) {
+        gAs[u] = St::zero();
+        if constexpr (LPC >= 4) g[u].store(held + u * 4, 0, 4, 1);
+      }
 #pragma unroll
       for (int two = 3; two >= 0; --two) {  // two steps at a time
         f2 along[2], gd[2], y[2];           // of the thread's two channels
@@ -822,6 +828,7 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
           f2 s = tile_pair(t0_, t1_), r = tile_pair(ty, ty);
           // value (lane / 8): along of channel 0, of channel 1, gd of each; y of each at step 0, at step 1
           const int k = tid % 32 / 8, step = tid / 4 % 2, col = tid % 4 * 2, c8 = warp * kLane * kPer + k % 2 * kLane;
+          check = add2(check, mul2(add2(s, r), splat(0.f)));  // NaN if one of them is not finite
           float* ps = to + k / 2 * TS * L::kPitch + step * L::kPitch + c8;
           float* pr = to + 2 * TS * L::kPitch + k / 2 * L::kPitch + c8;
           if constexpr (LPC == 4) {  // a column is a channel
@@ -850,6 +857,57 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
                 if (q == 0) to[k * TS * L::kPitch + ii * L::kPitch + ch + u * kLane] = v[k];
               }
             }
+        }
+      }
+      if constexpr (LPC >= 4) {
+        if (__any_sync(kFull, check.x + check.y != 0.f)) {
+          // A value is not finite: these sums once more, each channel's for itself, so that
+          // it stays in its channel. Not for speed: the loops are rolled.
+          __syncwarp();
+          St h[kPer], back[kPer], q8[8][kPer];
+#pragma unroll
+          for (int u = 0; u < kPer; ++u) {
+            h[u] = kept(t0 + sub * 8, u);
+            back[u] = St::shared(held + u * 4);
+          }
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            const St Bt = St::shared(bc + i * 2 * NP);
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) {
+              const float4 s = sl[i * CH + u * kLane];
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                q8[i][u].p[n] = mul2(decay2(A2[u].p[n], f2{s.x, s.y}), h[u].p[n]);
+                h[u].p[n] = fma2(Bt.p[n], f2{s.z, s.w}, q8[i][u].p[n]);
+              }
+            }
+          }
+#pragma unroll 1
+          for (int i = 7; i >= 0; --i) {
+            const St Bt = St::shared(bc + i * 2 * NP), Ct = St::shared(bc + i * 2 * NP + NP);
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) {
+              const float4 s = sl[i * CH + u * kLane];
+              const float2 s2 = sg[i * CH + u * kLane];
+              f2 v[3] = {f2{0.f, 0.f}, f2{0.f, 0.f}, f2{0.f, 0.f}};
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const f2 hn = fma2(Bt.p[n], f2{s.z, s.w}, q8[i][u].p[n]), gn = fma2(Ct.p[n], f2{s2.x, s2.y}, back[u].p[n]);
+                v[0] = fma2(gn, Bt.p[n], v[0]);
+                v[1] = fma2(mul2(gn, q8[i][u].p[n]), A2[u].p[n], v[1]);
+                v[2] = fma2(hn, Ct.p[n], v[2]);
+                back[u].p[n] = mul2(gn, decay2(A2[u].p[n], f2{s.x, s.y}));
+              }
+#pragma unroll
+              for (int e = 0; e < 3; ++e) {
+                float w = v[e].x + v[e].y;
+#pragma unroll
+                for (int o = LPC / 2; o > 0; o >>= 1) w += __shfl_xor_sync(kFull, w, o);
+                if (q == 0) res[(e * TS + sub * 8 + i) * L::kPitch + ch + u * kLane] = w;
+              }
+            }
+          }
         }
       }
       // gA: eight steps' sum at a time, which keeps the long sum's rounding small

@@ -144,6 +144,35 @@ def test_scan_reads_slices_of_wider_projections_in_place(cuda):
         assert all(torch.equal(p, q) for p, q in zip(got, ref))
 
 
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("where", ["x", "dt", "z", "gradient"])
+@pytest.mark.parametrize("n", [3, 8, 16, 24, 64])
+def test_scan_infinities_stay_in_their_channel(cuda, n, where, value):
+    """A value that is not finite reaches its own sequence's channel and the sums over
+    channels, and no other channel's outputs and gradients."""
+    b, t, c, hit = 2, 45, 70, 21
+    ins, _, g = scan_inputs(b, t, c, n, torch.float32, cuda, seed=9)
+    refs = {k: wide(v) for k, v in ins.items()}
+    rout, _ = scan_ref(*[refs[k] for k in ORDER])
+    want = dict(zip(ORDER, _grads(rout, g.double(), [refs[k] for k in ORDER])))
+    spoilt = {k: v.clone() for k, v in ins.items()}
+    g = g.clone()
+    (g if where == "gradient" else spoilt[where])[1, 30, hit] = value
+    leaves = [spoilt[k].requires_grad_() for k in ORDER]
+    out = sg.selective_scan(*leaves)
+    got = dict(zip(ORDER, _grads(out, g, leaves)))
+    others = torch.arange(c, device=cuda) != hit
+    check("out", out[..., others], rout[..., others])
+    check("out of the other sequence", out[0], rout[0])
+    for k in ("x", "dt", "z"):
+        check(f"gradient of {k}", got[k][..., others], want[k][..., others])
+        check(f"gradient of {k} in the other sequence", got[k][0], want[k][0])
+    for k in ("A", "D", "dt_bias"):
+        check(f"gradient of {k}", got[k][others], want[k][others])
+    for k in ("B", "C"):
+        check(f"gradient of {k} in the other sequence", got[k][0], want[k][0])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_scan_split_sequence_and_empty_sequence(cuda, dtype):
     ins, h0, _ = scan_inputs(2, 90, 41, 16, dtype, cuda, seed=11)
