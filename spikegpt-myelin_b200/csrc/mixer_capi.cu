@@ -67,7 +67,7 @@ int vector_width(size_t es, int most, std::initializer_list<const void*> ptrs, s
 int launch_column_sums(ColSumArgs a, cudaStream_t st) {
   const int64_t width = a.C * a.blocks;
   if (width == 0) return WKV_OK;
-  launch(K_COL_SUM, st, [&] { column_sum_kernel<<<(unsigned)((width + 31) / 32), dim3(32, 32), 0, st>>>(a); });
+  launch(K_COL_SUM, st, [&] { column_sum_kernel<<<(unsigned)((width + 31) / 32), 1024, 0, st>>>(a); });
   return launched("column sum launch");
 }
 
@@ -174,7 +174,7 @@ int scan_check(int dtype, int64_t B, int64_t T, int64_t C, int64_t N) {
   if (int rc = check_sizes({B, T, C, N})) return rc;
   if (N < 1 || N > kScanMaxN)
     return fail(WKV_ERR_INVALID_ARGUMENT, "the state size must be 1..%d, got %lld", kScanMaxN, (long long)N);
-  if (T > (1 << 23) || (B > 0 && (C + 7) / 8 * kScanMaxSegments > INT_MAX / B))
+  if (T > (1 << 23) || (B > 0 && ((C + 7) / 8 * kScanMaxSegments > INT_MAX / B || T > INT_MAX / B)))
     return fail(WKV_ERR_INVALID_ARGUMENT, "sizes out of range B=%lld T=%lld C=%lld", (long long)B, (long long)T,
                 (long long)C);
   return WKV_OK;
@@ -552,34 +552,37 @@ int selective_scan_backward(int dtype, const void* grad_out, const void* x, cons
     rc = lanes == 16 ? with_type(dtype, [&](auto e) { return main(e, std::integral_constant<int, 16>{}); })
                      : scan_dispatch(dtype, lanes, main);
     if (rc) return rc;
-    const int64_t cells = B * T * 2 * N;
-    if (cells > 0) {
-      rc = with_type(dtype, [&](auto e) {
-        launch(K_SCAN_RED, st, [&] {
-          scan_reduce_kernel<decltype(e)><<<(unsigned)((cells + 255) / 256), 256, 0, st>>>(ws.bc, p.cblocks, B * T,
-                                                                                          (int)N, grad_B, grad_C);
-        });
-        return launched("selective_scan reduction launch");
-      });
-      if (rc) return rc;
-    }
   }
-  ColSumArgs s{};
-  s.in = ws.a;
-  s.rows = (int)(B * p.nseg);
-  s.blocks = 1;
-  s.C = C * N;
-  s.out[0] = grad_A;
-  s.step[0] = 1;
-  if (int rc = launch_column_sums(s, st)) return rc;
-  if (!grad_D && !grad_dt_bias) return WKV_OK;
-  s.in = ws.d;
-  s.blocks = 2;
-  s.C = C;
-  s.out[0] = grad_D;
-  s.out[1] = grad_dt_bias;
-  s.step[1] = 1;
-  return launch_column_sums(s, st);
+  const int64_t cells = B * T * 2 * N;
+  ScanReduceArgs r{};
+  r.bc = ws.bc;
+  r.slices = p.cblocks;
+  r.N = (int)N;
+  r.rows = B * T;
+  r.gB = grad_B;
+  r.gC = grad_C;
+  r.bc_blocks = (cells + kScanReduceThreads - 1) / kScanReduceThreads;
+  r.a_blocks = (C * N + 31) / 32;
+  r.a.in = ws.a;
+  r.a.out[0] = grad_A;
+  r.a.step[0] = 1;
+  r.a.C = C * N;
+  r.a.blocks = 1;
+  r.d.in = ws.d;
+  r.d.out[0] = grad_D;
+  r.d.out[1] = grad_dt_bias;
+  r.d.step[0] = r.d.step[1] = 1;
+  r.d.C = C;
+  r.d.blocks = 2;
+  r.a.rows = r.d.rows = (int)(B * p.nseg);
+  const int64_t d_blocks = grad_D || grad_dt_bias ? (2 * C + 31) / 32 : 0;
+  return with_type(dtype, [&](auto e) {
+    launch(K_SCAN_RED, st, [&] {
+      scan_reduce_kernel<decltype(e)>
+          <<<(unsigned)(r.bc_blocks + r.a_blocks + d_blocks), kScanReduceThreads, 0, st>>>(r);
+    });
+    return launched("selective_scan reduction launch");
+  });
 }
 
 int selective_scan_step(int dtype, const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,

@@ -98,24 +98,25 @@ __device__ __forceinline__ uint32_t q4_nibbles(uint32_t a, uint32_t mask, uint32
 }
 
 // One tile of 16-bit tokens is read straight to registers a stage ahead (the rows of x
-// are short and stay in the L1 cache); more tokens, and float32 ones, are staged.
+// are short and stay in the L1 cache); more tokens are staged in the ring. float32 ones
+// come to registers a stage ahead too, and the warp splits each value once, into a
+// buffer of the terms' rows.
 template <typename T, int NT>
 __host__ __device__ constexpr bool q4_staged() {
-  return NT > 1 || sizeof(T) > 2;
+  return NT > 1 && sizeof(T) == 2;
 }
-// Bytes of a staged token's inputs: a shift of half the banks from token to token.
-template <typename T>
-__host__ __device__ constexpr int q4_token_bytes() {
-  return kQ4Chunk * (int)sizeof(T) + 64;
-}
+// Bytes of a column's inputs of a stage: a shift of half the banks from one to the next.
+constexpr int kQ4ColumnBytes = kQ4Chunk * 2 + 64;
 template <typename T, int R, int NT, int GW>
 __host__ __device__ constexpr int q4_stage_bytes(int tokens) {
-  return R * 16 * q4_row_bytes(GW) + (q4_staged<T, NT>() ? tokens * q4_token_bytes<T>() : 0);
+  return R * 16 * q4_row_bytes(GW) + (q4_staged<T, NT>() ? tokens * kQ4ColumnBytes : 0);
 }
-// A warp's ring and its scales and zeros (float, uint32_t) [2][16 R][4 / GW].
+// A warp's ring, its scales and zeros (float, uint32_t) [2][16 R][4 / GW] and float32
+// tokens' terms.
 template <typename T, int R, int NT, int GW>
 __host__ __device__ constexpr int q4_warp_bytes(int tokens) {
-  return kQ4Stages * q4_stage_bytes<T, R, NT, GW>(tokens) + 2 * R * 16 * (4 / GW) * 8;
+  return kQ4Stages * q4_stage_bytes<T, R, NT, GW>(tokens) + 2 * R * 16 * (4 / GW) * 8 +
+         (sizeof(T) > 2 ? 3 * tokens * kQ4ColumnBytes : 0);
 }
 template <int R, int NT>
 constexpr int q4_sum_bytes(int warps) {
@@ -134,24 +135,22 @@ __device__ __forceinline__ void q4_pairs(uint4 u, uint32_t (&b)[4]) {
   b[2] = __byte_perm(u.y, u.w, 0x5410);
   b[3] = __byte_perm(u.y, u.w, 0x7632);
 }
-template <typename T>
-__device__ __forceinline__ void q4_inputs(const T* p, int term, uint32_t (&b)[4]) {
-  if constexpr (sizeof(T) == 2) {
-    q4_pairs(*reinterpret_cast<const uint4*>(p), b);
-  } else {
-    const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
-    const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-    uint32_t t[8];
+// Four float32 values as three bfloat16 terms of 8 bits each (the upper half of a
+// float32 is its value cut to bfloat16), exactly; term e's four words side by side.
+__device__ __forceinline__ void q4_split(float4 v, uint2 (&t)[3]) {
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  uint32_t u[3][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {  // the upper half of a float32 is its value cut to bfloat16
-      const float h = __uint_as_float(__float_as_uint(f[i]) & 0xffff0000u);
-      const float r = h == f[i] ? 0.f : f[i] - h;  // an infinity stays in the first term
-      const float r2 = r - __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-      t[i] = __float_as_uint(term == 0 ? f[i] : term == 1 ? r : r2);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = __byte_perm(t[i], t[i + 4], 0x7632);
+  for (int i = 0; i < 4; ++i) {
+    const float h = __uint_as_float(__float_as_uint(f[i]) & 0xffff0000u);
+    const float r = h == f[i] ? 0.f : f[i] - h;  // an infinity stays in the first term
+    u[0][i] = __float_as_uint(f[i]);
+    u[1][i] = __float_as_uint(r);
+    u[2][i] = __float_as_uint(r - __uint_as_float(__float_as_uint(r) & 0xffff0000u));
   }
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    t[e] = make_uint2(__byte_perm(u[e][0], u[e][1], 0x7632), __byte_perm(u[e][2], u[e][3], 0x7632));
 }
 
 // GW: words of eight weights that a lane takes side by side, 1, 2 or 4: the four lanes'
@@ -161,9 +160,10 @@ template <typename T, int R, int NT, int GW, bool kWide>
 __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a) {
   using H = typename Q4Type<T>::half;
   using Math = Q4Math<H>;
-  constexpr int kTerms = Q4Type<T>::kTerms, kTok = q4_token_bytes<T>(), kRow = q4_row_bytes(GW);
+  constexpr int kTerms = Q4Type<T>::kTerms, kTok = kQ4ColumnBytes, kRow = q4_row_bytes(GW);
   constexpr int kSpans = 4 / GW, kEntries = 16 * R * kSpans, kPer = (kEntries + 31) / 32;
-  constexpr bool kStaged = q4_staged<T, NT>();
+  constexpr bool kStaged = q4_staged<T, NT>(), kSplit = kTerms > 1;
+  constexpr int kSplitTokens = kSplit ? 8 * NT / kTerms : 1;
   extern __shared__ __align__(16) char smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
   const int wk = warp % a.wk, wn = warp / a.wk;
@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
   const int stage_bytes = q4_stage_bytes<T, R, NT, GW>(a.tokens);
   char* ring = smem + warp * q4_warp_bytes<T, R, NT, GW>(a.tokens);
   float2* sz = reinterpret_cast<float2*>(ring + kQ4Stages * stage_bytes);
+  char* terms = reinterpret_cast<char*>(sz + 2 * kEntries);
   const int chunks = (a.K + kQ4Chunk - 1) / kQ4Chunk;
   const int mine = n0 < a.N && chunks > wk ? (chunks - wk + a.wk - 1) / a.wk : 0;
   const T* x = static_cast<const T*>(a.x) + m0 * a.x_s;
@@ -217,6 +218,7 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
   uint16_t fs[kPer];
   uint8_t fz[kPer];
   uint4 fx[4];
+  float4 fy[kSplitTokens];
   const T* px = x + (g < tokens ? g * a.x_s : 0);  // columns past the tokens are not written
   int fetch_k = wk * kQ4Chunk;
   auto fetch = [&]() {  // past the last stage: of inputs that exist, and are not used
@@ -228,7 +230,20 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
       fs[p] = reinterpret_cast<const uint16_t*>(a.scale)[at];
       fz[p] = a.zero ? a.zero[at] : 8;
     }
-    if constexpr (!kStaged) {
+    if constexpr (kSplit) {
+      const int k = fetch_k + lane * 4;
+#pragma unroll
+      for (int t = 0; t < kSplitTokens; ++t) {
+        fy[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (t < tokens && k < a.K) {
+          const float* p = reinterpret_cast<const float*>(x) + t * a.x_s + k;
+          if constexpr (kWide)
+            fy[t] = *reinterpret_cast<const float4*>(p);
+          else
+            fy[t] = make_float4(p[0], k + 1 < a.K ? p[1] : 0.f, k + 2 < a.K ? p[2] : 0.f, k + 3 < a.K ? p[3] : 0.f);
+        }
+      }
+    } else if constexpr (!kStaged) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int k = fetch_k + j * 8 * GW + w / GW * (32 * GW) + w % GW * 8;
@@ -277,12 +292,23 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
     __syncwarp();  // the stage and its scales are there, and every lane is done with the stage before
     issue(i + kQ4Stages - 1);
     uint32_t bx[4][4];  // the unstaged tokens' operands: their words are free for the next stage's
-    if constexpr (!kStaged)
+    if constexpr (kSplit) {
+#pragma unroll
+      for (int t = 0; t < kSplitTokens; ++t)
+        if (t < tokens) {
+          uint2 u[3];
+          q4_split(fy[t], u);
+#pragma unroll
+          for (int e = 0; e < 3; ++e) *reinterpret_cast<uint2*>(terms + (3 * t + e) * kTok + lane * 8) = u[e];
+        }
+      __syncwarp();
+    } else if constexpr (!kStaged) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) q4_pairs(fx[w], bx[w]);
+    }
     fetch();
     const char* from = ring + stage * stage_bytes + g * kRow + j * 4 * GW;
-    const char* tx = ring + stage * stage_bytes + rows * kRow + j * 8 * GW * sizeof(T);
+    const char* tx = (kSplit ? terms : ring + stage * stage_bytes + rows * kRow) + j * 8 * GW * 2;
     const float2* sc = sz + (i & 1) * kEntries + g * kSpans;
     stage = stage + 1 == kQ4Stages ? 0 : stage + 1;
 #pragma unroll
@@ -293,12 +319,11 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const int column = t * 8 + g;
-          if constexpr (!kStaged) {
+          if constexpr (!kStaged && !kSplit) {
 #pragma unroll
             for (int n = 0; n < 4; ++n) b[w][t][n] = bx[span * GW + w][n];
           } else if (column < tokens * kTerms)
-            q4_inputs(reinterpret_cast<const T*>(tx + column / kTerms * kTok) + span * 32 * GW + w * 8, column % kTerms,
-                      b[w][t]);
+            q4_pairs(*reinterpret_cast<const uint4*>(tx + column * kTok + (span * 32 * GW + w * 8) * 2), b[w][t]);
           else
             b[w][t][0] = b[w][t][1] = b[w][t][2] = b[w][t][3] = 0;
         }

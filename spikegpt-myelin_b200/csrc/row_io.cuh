@@ -83,9 +83,10 @@ struct Vec {
 // 1 / (1 + e^-v); 0 and 1 at the infinities.
 __device__ __forceinline__ float sigmoid1(float v) { return rcp(1.f + ex2(-v * kL2E)); }
 
-// Column sums of `rows` float32 rows of `blocks` groups of C columns, in row
-// order within each of 32 strides and then over the strides in order, so the
-// result does not depend on timing. Group k goes to out[k][c * step[k]].
+// Column sums of `rows` float32 rows of `blocks` groups of C columns, in row order
+// within each of kRows strides and then over the strides in order, so the result does
+// not depend on timing. Group k goes to out[k][c * step[k]]. A CTA of 32 kRows threads
+// sums 32 columns; neighbouring lanes read neighbouring columns.
 constexpr int kSumGroups = 6;
 struct ColSumArgs {
   const float* in;
@@ -95,25 +96,29 @@ struct ColSumArgs {
   int64_t C;
 };
 
-__global__ void __launch_bounds__(1024) column_sum_kernel(ColSumArgs a) {
-  __shared__ float red[32][33];
-  const int64_t width = a.C * a.blocks;
-  const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.x;
+template <int kRows>
+__device__ __forceinline__ void column_sums(const ColSumArgs& a, int64_t block) {
+  __shared__ float red[kRows][33];
+  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
+  const int64_t width = a.C * a.blocks, col = block * 32 + x;
   float s = 0.f;
   if (col < width) {
     const float* p = a.in + col;
-    for (int r = threadIdx.y; r < a.rows; r += 32) s += p[(int64_t)r * width];
+#pragma unroll 4
+    for (int r = y; r < a.rows; r += kRows) s += p[(int64_t)r * width];
   }
-  red[threadIdx.y][threadIdx.x] = s;
+  red[y][x] = s;
   __syncthreads();
-  if (threadIdx.y == 0 && col < width) {
+  if (y == 0 && col < width) {
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) t += red[i][threadIdx.x];
+    for (int i = 0; i < kRows; ++i) t += red[i][x];
     const int k = (int)(col / a.C);
     const int64_t c = col - (int64_t)k * a.C;
     if (a.out[k]) a.out[k][c * a.step[k]] = t;
   }
 }
+
+__global__ void __launch_bounds__(1024) column_sum_kernel(ColSumArgs a) { column_sums<32>(a, blockIdx.x); }
 
 }  // namespace wkv

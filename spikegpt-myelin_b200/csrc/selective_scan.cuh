@@ -1001,18 +1001,34 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
   }
 }
 
-// gB and gC: the slices' partial sums in slice order, in the tensors' type.
+// The sums over CTAs, in one launch (three cost 10 us more): gB and gC, the channel
+// slices' partial rows in slice order, in the tensors' type; then gA, and gD and
+// gbias, over sequences and segments.
+struct ScanReduceArgs {
+  const float* bc;  // [slices][rows][2][N]
+  int slices, N;
+  int64_t rows;
+  void *gB, *gC;
+  int64_t bc_blocks, a_blocks;  // CTAs of the first two parts
+  ColSumArgs a, d;
+};
+constexpr int kScanReduceThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(256) scan_reduce_kernel(const float* part, int slices, int64_t rows, int N, void* gB,
-                                                          void* gC) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, width = rows * 2 * N;
+__global__ void __launch_bounds__(kScanReduceThreads) scan_reduce_kernel(ScanReduceArgs r) {
+  if (blockIdx.x >= r.bc_blocks) {
+    const int64_t block = blockIdx.x - r.bc_blocks;
+    column_sums<kScanReduceThreads / 32>(block < r.a_blocks ? r.a : r.d, block < r.a_blocks ? block : block - r.a_blocks);
+    return;
+  }
+  const int64_t i = (int64_t)blockIdx.x * kScanReduceThreads + threadIdx.x, width = r.rows * 2 * r.N;
   if (i >= width) return;
   float s = 0.f;
-  for (int k = 0; k < slices; ++k) s += part[k * width + i];
-  const int64_t row = i / (2 * N);
-  const int j = (int)(i - row * 2 * N);
-  T* to = static_cast<T*>(j < N ? gB : gC);
-  to[row * N + (j < N ? j : j - N)] = Pair<T>::from_float(s);
+#pragma unroll 8
+  for (int k = 0; k < r.slices; ++k) s += r.bc[k * width + i];
+  const int64_t row = i / (2 * r.N);
+  const int j = (int)(i - row * 2 * r.N);
+  T* to = static_cast<T*>(j < r.N ? r.gB : r.gC);
+  to[row * r.N + (j < r.N ? j : j - r.N)] = Pair<T>::from_float(s);
 }
 
 // One token: x, dt, z [B][C] and B, C [B][N]; the state is updated in place. LPC
