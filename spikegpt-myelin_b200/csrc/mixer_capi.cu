@@ -746,14 +746,14 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
   a.pitch = (int)((K + 31) / 32 * 16);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int es = (int)dtype_size(dtype);
-  const bool wide = vector_width(es, 16 / es, {x}, {x_stride, K}) == 16 / es;
+  const int vector = vector_width(es, 16 / es, {x}, {x_stride, K});
   // floor(i / d) is the upper word of i * (floor(2^32 / d) + 1) while i * d < 2^32
   const int64_t d = std::min(group, (K + 31) / 32 * 32) / 32;
   a.group_magic = d > 1 ? (uint32_t)((1ull << 32) / d + 1) : 0;
   return with_type(dtype, [&](auto e) {
     using E = decltype(e);
     constexpr int kTerms = Q4Type<E>::kTerms;
-    a.tokens = (int)std::min<int64_t>(M, kTerms == 1 ? 16 : 8);  // what the rings' shared memory allows
+    a.tokens = (int)std::min<int64_t>(M, kTerms == 1 ? 16 : 8);  // what a lane's registers hold of a stage
     const int tiles = (a.tokens * kTerms + 7) / 8;
     const int64_t my = (M + a.tokens - 1) / a.tokens;
     if (my > 65535) return fail(WKV_ERR_INVALID_ARGUMENT, "too many tokens: %lld", (long long)M);
@@ -767,6 +767,7 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
       a.wk = warps;
       while (a.wk > 1 && chunks < 3 * a.wk && ctas(a.wk / 2) >= sm_count()) a.wk /= 2;
       const int bytes = std::max(warps * q4_warp_bytes<E, R, NT, GW>(a.tokens), q4_sum_bytes<R, NT>(warps));
+      const bool wide = vector >= (q4_direct<E, NT>() ? 8 : 4);
       auto kernel = wide ? q4_matvec_kernel<E, R, NT, GW, true> : q4_matvec_kernel<E, R, NT, GW, false>;
       const cudaError_t err = allow_smem(kernel, q4_smem_max<E, R, NT, GW>());
       if (err != cudaSuccess) return cuda_fail(err, "setting the q4_matvec kernel's shared memory size");
@@ -781,8 +782,13 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
       if (group % 64 == 0) return launch_one(r, nt, std::integral_constant<int, 2>{});
       return launch_one(r, nt, std::integral_constant<int, 1>{});
     };
-    // 32 rows a warp where that still gives two CTAs an SM: x is read and paired half as often
-    if (tiles == 2) return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
+    // 32 rows a warp where that still gives two CTAs an SM, so that the inputs are read and
+    // paired half as often: 16 x 768 x 50257 31 us with 16 rows, 29 with 32; 16 x 8192 x 16384
+    // 76 and 66. (Three tiles' sums and operands leave no registers for 32 rows.)
+    if (tiles == 2) {
+      if (N >= 64 * sm_count()) return go(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+      return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
+    }
     if constexpr (kTerms > 1)
       if (tiles == 3) return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 3>{});
     if (N >= 64 * sm_count()) return go(std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{});

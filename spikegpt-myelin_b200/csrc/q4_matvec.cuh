@@ -97,26 +97,27 @@ __device__ __forceinline__ uint32_t q4_nibbles(uint32_t a, uint32_t mask, uint32
   return d;
 }
 
-// One tile of 16-bit tokens is read straight to registers a stage ahead (the rows of x
-// are short and stay in the L1 cache); more tokens are staged in the ring. float32 ones
-// come to registers a stage ahead too, and the warp splits each value once, into a
-// buffer of the terms' rows.
+// A stage's inputs come to registers a stage ahead. One tile of 16-bit tokens goes from
+// there to the products as each lane reads it (its rows of x are short and stay in the
+// L1 cache: 31 us for 8 x 8192 x 16384, through shared memory 39); more tokens (whose
+// registers would not do) and float32 ones (whose values are split once a warp) go
+// through shared memory.
 template <typename T, int NT>
-__host__ __device__ constexpr bool q4_staged() {
-  return NT > 1 && sizeof(T) == 2;
+__host__ __device__ constexpr bool q4_direct() {
+  return NT == 1 && sizeof(T) == 2;
 }
 // Bytes of a column's inputs of a stage: a shift of half the banks from one to the next.
 constexpr int kQ4ColumnBytes = kQ4Chunk * 2 + 64;
-template <typename T, int R, int NT, int GW>
-__host__ __device__ constexpr int q4_stage_bytes(int tokens) {
-  return R * 16 * q4_row_bytes(GW) + (q4_staged<T, NT>() ? tokens * kQ4ColumnBytes : 0);
+template <int R, int GW>
+__host__ __device__ constexpr int q4_stage_bytes() {
+  return R * 16 * q4_row_bytes(GW);
 }
-// A warp's ring, its scales and zeros (float, uint32_t) [2][16 R][4 / GW] and float32
-// tokens' terms.
+// A warp's ring, its scales and zeros (float, uint32_t) [2][16 R][4 / GW] and its
+// columns' inputs.
 template <typename T, int R, int NT, int GW>
 __host__ __device__ constexpr int q4_warp_bytes(int tokens) {
-  return kQ4Stages * q4_stage_bytes<T, R, NT, GW>(tokens) + 2 * R * 16 * (4 / GW) * 8 +
-         (sizeof(T) > 2 ? 3 * tokens * kQ4ColumnBytes : 0);
+  return kQ4Stages * q4_stage_bytes<R, GW>() + 2 * R * 16 * (4 / GW) * 8 +
+         (q4_direct<T, NT>() ? 0 : Q4Type<T>::kTerms * tokens * kQ4ColumnBytes);
 }
 template <int R, int NT>
 constexpr int q4_sum_bytes(int warps) {
@@ -137,8 +138,8 @@ __device__ __forceinline__ void q4_pairs(uint4 u, uint32_t (&b)[4]) {
 }
 // Four float32 values as three bfloat16 terms of 8 bits each (the upper half of a
 // float32 is its value cut to bfloat16), exactly; term e's four words side by side.
-__device__ __forceinline__ void q4_split(float4 v, uint2 (&t)[3]) {
-  const float f[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ void q4_split(uint4 v, uint2 (&t)[3]) {
+  const float f[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
   uint32_t u[3][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -155,15 +156,16 @@ __device__ __forceinline__ void q4_split(float4 v, uint2 (&t)[3]) {
 
 // GW: words of eight weights that a lane takes side by side, 1, 2 or 4: the four lanes'
 // 32, 64 or 128 inputs lie in one group, and are scaled at a time.
-// kWide: rows of x are whole aligned 16-byte words.
+// kWide: rows of x are whole aligned 16-byte words (8-byte ones are enough for more than
+// one tile of 16-bit tokens).
 template <typename T, int R, int NT, int GW, bool kWide>
 __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a) {
   using H = typename Q4Type<T>::half;
   using Math = Q4Math<H>;
   constexpr int kTerms = Q4Type<T>::kTerms, kTok = kQ4ColumnBytes, kRow = q4_row_bytes(GW);
   constexpr int kSpans = 4 / GW, kEntries = 16 * R * kSpans, kPer = (kEntries + 31) / 32;
-  constexpr bool kStaged = q4_staged<T, NT>(), kSplit = kTerms > 1;
-  constexpr int kSplitTokens = kSplit ? 8 * NT / kTerms : 1;
+  constexpr bool kDirect = q4_direct<T, NT>();
+  constexpr int kFetches = kDirect ? 4 : 8 * NT / kTerms;
   extern __shared__ __align__(16) char smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
   const int wk = warp % a.wk, wn = warp / a.wk;
@@ -171,10 +173,10 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
   const int cta_rows = rows * ((int)blockDim.x / 32 / a.wk);
   const int n0 = blockIdx.x * cta_rows + wn * rows, m0 = blockIdx.y * a.tokens;
   const int tokens = min(a.tokens, a.M - m0);
-  const int stage_bytes = q4_stage_bytes<T, R, NT, GW>(a.tokens);
+  constexpr int stage_bytes = q4_stage_bytes<R, GW>();
   char* ring = smem + warp * q4_warp_bytes<T, R, NT, GW>(a.tokens);
   float2* sz = reinterpret_cast<float2*>(ring + kQ4Stages * stage_bytes);
-  char* terms = reinterpret_cast<char*>(sz + 2 * kEntries);
+  char* columns = reinterpret_cast<char*>(sz + 2 * kEntries);
   const int chunks = (a.K + kQ4Chunk - 1) / kQ4Chunk;
   const int mine = n0 < a.N && chunks > wk ? (chunks - wk + a.wk - 1) / a.wk : 0;
   const T* x = static_cast<const T*>(a.x) + m0 * a.x_s;
@@ -192,33 +194,16 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
       const int off = on ? copy_k >> 1 : 0;
 #pragma unroll
       for (int p = 0; p < 2 * R; ++p) q4_copy(to + (p * 8 + g) * kRow + j * 16, pq[p] + off, on);
-      if constexpr (kStaged) {
-        char* tx = to + rows * kRow;
-        const int k0 = copy_k - j * 32;
-        constexpr int kWords = kQ4Chunk * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
-        if constexpr (kWide) {
-          for (int p = lane; p < tokens * kWords; p += 32) {
-            const int k = k0 + p % kWords * E;
-            q4_copy(tx + p / kWords * kTok + p % kWords * 16, x + p / kWords * a.x_s + (k < a.K ? k : 0), k < a.K);
-          }
-        } else {
-          for (int p = lane; p < tokens * kQ4Chunk; p += 32) {
-            const int k = k0 + p % kQ4Chunk;
-            reinterpret_cast<T*>(tx + p / kQ4Chunk * kTok)[p % kQ4Chunk] =
-                k < a.K ? x[p / kQ4Chunk * a.x_s + k] : Pair<T>::from_float(0.f);
-          }
-        }
-      }
       copy_k += a.wk * kQ4Chunk;
       copy_stage = copy_stage + 1 == kQ4Stages ? 0 : copy_stage + 1;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // The next stage's scales and zeros, kPer (row, span) pairs a lane, and unstaged tokens.
+  // The next stage's scales and zeros, kPer (row, span) pairs a lane, and its inputs: the
+  // lane's column of eight at a time (direct), or four of each token.
   uint16_t fs[kPer];
   uint8_t fz[kPer];
-  uint4 fx[4];
-  float4 fy[kSplitTokens];
+  Vec<T, kDirect ? 8 : 4> fx[kFetches];
   const T* px = x + (g < tokens ? g * a.x_s : 0);  // columns past the tokens are not written
   int fetch_k = wk * kQ4Chunk;
   auto fetch = [&]() {  // past the last stage: of inputs that exist, and are not used
@@ -230,38 +215,41 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
       fs[p] = reinterpret_cast<const uint16_t*>(a.scale)[at];
       fz[p] = a.zero ? a.zero[at] : 8;
     }
-    if constexpr (kSplit) {
-      const int k = fetch_k + lane * 4;
-#pragma unroll
-      for (int t = 0; t < kSplitTokens; ++t) {
-        fy[t] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (t < tokens && k < a.K) {
-          const float* p = reinterpret_cast<const float*>(x) + t * a.x_s + k;
-          if constexpr (kWide)
-            fy[t] = *reinterpret_cast<const float4*>(p);
-          else
-            fy[t] = make_float4(p[0], k + 1 < a.K ? p[1] : 0.f, k + 2 < a.K ? p[2] : 0.f, k + 3 < a.K ? p[3] : 0.f);
-        }
-      }
-    } else if constexpr (!kStaged) {
+    if constexpr (kDirect) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int k = fetch_k + j * 8 * GW + w / GW * (32 * GW) + w % GW * 8;
         if constexpr (kWide) {
-          fx[w] = *reinterpret_cast<const uint4*>(px + min(k, a.K - 8));
+          fx[w] = Vec<T, 8>::load(px + min(k, a.K - 8));
         } else {
           const uint16_t* h = reinterpret_cast<const uint16_t*>(px) + k;
           uint32_t u[4];
 #pragma unroll
           for (int n = 0; n < 4; ++n)
             u[n] = (k + 2 * n < a.K ? h[2 * n] : 0u) | (k + 2 * n + 1 < a.K ? (uint32_t)h[2 * n + 1] << 16 : 0u);
-          fx[w] = make_uint4(u[0], u[1], u[2], u[3]);
+          fx[w].w = make_uint4(u[0], u[1], u[2], u[3]);
         }
       }
       if (kWide && fetch_k + kQ4Chunk > a.K) {
 #pragma unroll
         for (int w = 0; w < 4; ++w)
-          if (fetch_k + j * 8 * GW + w / GW * (32 * GW) + w % GW * 8 >= a.K) fx[w] = make_uint4(0, 0, 0, 0);
+          if (fetch_k + j * 8 * GW + w / GW * (32 * GW) + w % GW * 8 >= a.K) fx[w] = Vec<T, 8>::zero();
+      }
+    } else {
+      const int k = fetch_k + lane * 4;
+#pragma unroll
+      for (int t = 0; t < kFetches; ++t) {
+        fx[t] = Vec<T, 4>::zero();
+        if (t < tokens && k < a.K) {
+          const T* p = x + t * a.x_s + k;
+          if constexpr (kWide) {
+            fx[t] = Vec<T, 4>::load(p);
+          } else {
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              if (k + n < a.K) fx[t].e[n] = p[n];
+          }
+        }
       }
     }
     fetch_k += a.wk * kQ4Chunk;
@@ -291,24 +279,28 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
     asm volatile("cp.async.wait_group %0;" ::"n"(kQ4Stages - 2) : "memory");
     __syncwarp();  // the stage and its scales are there, and every lane is done with the stage before
     issue(i + kQ4Stages - 1);
-    uint32_t bx[4][4];  // the unstaged tokens' operands: their words are free for the next stage's
-    if constexpr (kSplit) {
+    uint32_t bx[4][4];  // direct operands: their words are free for the next stage's
+    if constexpr (kDirect) {
 #pragma unroll
-      for (int t = 0; t < kSplitTokens; ++t)
+      for (int w = 0; w < 4; ++w) q4_pairs(fx[w].w, bx[w]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < kFetches; ++t)
         if (t < tokens) {
-          uint2 u[3];
-          q4_split(fy[t], u);
+          uint2 u[kTerms];
+          if constexpr (kTerms == 1)
+            u[0] = fx[t].w;
+          else
+            q4_split(fx[t].w, u);
 #pragma unroll
-          for (int e = 0; e < 3; ++e) *reinterpret_cast<uint2*>(terms + (3 * t + e) * kTok + lane * 8) = u[e];
+          for (int e = 0; e < kTerms; ++e)
+            *reinterpret_cast<uint2*>(columns + (kTerms * t + e) * kTok + lane * 8) = u[e];
         }
       __syncwarp();
-    } else if constexpr (!kStaged) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w) q4_pairs(fx[w], bx[w]);
     }
     fetch();
     const char* from = ring + stage * stage_bytes + g * kRow + j * 4 * GW;
-    const char* tx = (kSplit ? terms : ring + stage * stage_bytes + rows * kRow) + j * 8 * GW * 2;
+    const char* tx = columns + j * 8 * GW * 2;
     const float2* sc = sz + (i & 1) * kEntries + g * kSpans;
     stage = stage + 1 == kQ4Stages ? 0 : stage + 1;
 #pragma unroll
@@ -319,7 +311,7 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const int column = t * 8 + g;
-          if constexpr (!kStaged && !kSplit) {
+          if constexpr (kDirect) {
 #pragma unroll
             for (int n = 0; n < 4; ++n) b[w][t][n] = bx[span * GW + w][n];
           } else if (column < tokens * kTerms)
