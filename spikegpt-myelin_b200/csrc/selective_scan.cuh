@@ -115,8 +115,12 @@ __device__ __forceinline__ void reduce_scatter(float* v) {
 constexpr float kDecayShift = 2.4e-8f;
 __device__ __forceinline__ f2 decay2(f2 A2, f2 d) { return ex2x2(fma2(A2, d, splat(kDecayShift))); }
 
-// kS adjacent states of one channel, as packed pairs.
-template <int kS>
+// kS states of one channel, as packed pairs: groups of four adjacent ones, kGap apart.
+// Where lanes share a channel their groups alternate (kGap = 4 lanes), so that a group
+// of all lanes is one contiguous read of shared memory and whole sectors of the kept
+// states (eight adjacent states a lane met in the banks: forward of 16 x 1024 x 1536
+// with 64 states 1043 us).
+template <int kS, int kGap = 4>
 struct States {
   f2 p[kS / 2];
   __device__ __forceinline__ static States zero() {
@@ -125,20 +129,21 @@ struct States {
     for (int i = 0; i < kS / 2; ++i) r.p[i] = f2{0.f, 0.f};
     return r;
   }
-  // states n .. n + kS - 1 of a row of N float32 states; past N: zeros. `wide`: four
+  // the states from n on of a row of N float32 states; past N: zeros. `wide`: four
   // adjacent states move as one aligned word, and N is a multiple of 4.
   __device__ __forceinline__ static States load(const float* row, int n, int N, int wide) {
     States r;
 #pragma unroll
     for (int i = 0; i < kS; i += 4) {
+      const int m = n + i / 4 * kGap;
       if (wide) {
-        const float4 v = n + i < N ? *reinterpret_cast<const float4*>(row + n + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 v = m < N ? *reinterpret_cast<const float4*>(row + m) : make_float4(0.f, 0.f, 0.f, 0.f);
         r.p[i / 2] = f2{v.x, v.y};
         r.p[i / 2 + 1] = f2{v.z, v.w};
       } else {
 #pragma unroll
         for (int j = 0; j < 4; j += 2)
-          r.p[(i + j) / 2] = f2{n + i + j < N ? row[n + i + j] : 0.f, n + i + j + 1 < N ? row[n + i + j + 1] : 0.f};
+          r.p[(i + j) / 2] = f2{m + j < N ? row[m + j] : 0.f, m + j + 1 < N ? row[m + j + 1] : 0.f};
       }
     }
     return r;
@@ -146,14 +151,15 @@ struct States {
   __device__ __forceinline__ void store(float* row, int n, int N, int wide) const {
 #pragma unroll
     for (int i = 0; i < kS; i += 4) {
+      const int m = n + i / 4 * kGap;
       const f2 u = p[i / 2], v = p[i / 2 + 1];
       if (wide) {
-        if (n + i < N) *reinterpret_cast<float4*>(row + n + i) = make_float4(u.x, u.y, v.x, v.y);
+        if (m < N) *reinterpret_cast<float4*>(row + m) = make_float4(u.x, u.y, v.x, v.y);
       } else {
-        if (n + i < N) row[n + i] = u.x;
-        if (n + i + 1 < N) row[n + i + 1] = u.y;
-        if (n + i + 2 < N) row[n + i + 2] = v.x;
-        if (n + i + 3 < N) row[n + i + 3] = v.y;
+        if (m < N) row[m] = u.x;
+        if (m + 1 < N) row[m + 1] = u.y;
+        if (m + 2 < N) row[m + 2] = v.x;
+        if (m + 3 < N) row[m + 3] = v.y;
       }
     }
   }
@@ -162,7 +168,7 @@ struct States {
     States r;
 #pragma unroll
     for (int i = 0; i < kS; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(row + i);
+      const float4 v = *reinterpret_cast<const float4*>(row + i / 4 * kGap);
       r.p[i / 2] = f2{v.x, v.y};
       r.p[i / 2 + 1] = f2{v.z, v.w};
     }
@@ -234,19 +240,18 @@ struct ScanShape {
   static_assert(kIdle || kRows * kStep == TT, "whole rows a thread");
 };
 
-// The forward's and the summaries': eight states a lane (half the instructions of
-// four a lane for the reads of d, d x and the exchange of y), 1024 cells a tile.
-template <int LPC>
-using FwdShape = ScanShape<LPC, 8, kScanThreads, 8 * LPC < kScanRows ? 8 * LPC : kScanRows>;
+// The forward's and the summaries': kS states a lane, 1024 cells a tile.
+template <int LPC, int kS>
+using FwdShape = ScanShape<LPC, kS, kScanThreads, 8 * LPC < kScanRows ? 8 * LPC : kScanRows>;
 
 // The state a segment starts from: the earlier segments' contributions in order
 // (forward), or the adjoint that the later segments hand back.
-template <int kS>
-__device__ __forceinline__ States<kS> scan_carry(const ScanArgs& a, int b, int c, int n, States<kS> h,
-                                                 const States<kS>& A2, int from, int to, int step) {
+template <int kS, int kGap>
+__device__ __forceinline__ States<kS, kGap> scan_carry(const ScanArgs& a, int b, int c, int n, States<kS, kGap> h,
+                                                       const States<kS, kGap>& A2, int from, int to, int step) {
   for (int s = from; s != to; s += step) {
     const int64_t at = ((int64_t)b * a.nseg + s) * a.C + c;
-    const States<kS> add = States<kS>::load(a.seg_h + at * a.N, n, a.N, a.wide_n);
+    const auto add = States<kS, kGap>::load(a.seg_h + at * a.N, n, a.N, a.wide_n);
     const f2 d = splat(a.seg_d[at]);
 #pragma unroll
     for (int i = 0; i < kS / 2; ++i) h.p[i] = fma2(ex2x2(mul2(A2.p[i], d)), h.p[i], add.p[i]);
@@ -283,10 +288,10 @@ __device__ __forceinline__ bool scan_plain(const ScanArgs& a, int c_end) {
 
 // What a segment adds to a zero state (kAdjoint: to a zero adjoint, walking back:
 // g <- a (g + C gy)), and its sum of d: the decay across it is exp(A sum d).
-template <typename T, int LPC, bool kAdjoint>
+template <typename T, int LPC, int kS, bool kAdjoint>
 __global__ void __launch_bounds__(kScanThreads) scan_summary_kernel(ScanArgs a) {
-  using S = FwdShape<LPC>;
-  using St = States<8>;
+  using S = FwdShape<LPC, kS>;
+  using St = States<kS, 4 * LPC>;
   __shared__ float4 sdx[S::TT][S::CH];  // d, d, w, w: pairs as the packed arithmetic reads them
   __shared__ __align__(16) float sn[S::TT][S::NP];
   // the last segment's sum serves no later one (the first's, walking back)
@@ -294,7 +299,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_summary_kernel(ScanArgs a) 
   const int b = blockIdx.x / a.cblocks / (a.nseg - 1);
   const int q = threadIdx.x % LPC, ch = threadIdx.x / LPC, c0 = cb * S::CH, c = c0 + ch;
   const int t_begin = seg * a.seg_len, t_end = min(t_begin + a.seg_len, scan_length(a, b));
-  St A2 = St::load(a.A + (int64_t)min(c, a.C - 1) * a.N, 8 * q, a.N, a.wide_n);
+  St A2 = St::load(a.A + (int64_t)min(c, a.C - 1) * a.N, 4 * q, a.N, a.wide_n);
   A2.scale(kL2E);
   St h = St::zero();
   f2 dsum{0.f, 0.f};
@@ -354,9 +359,9 @@ __global__ void __launch_bounds__(kScanThreads) scan_summary_kernel(ScanArgs a) 
       const int i = kAdjoint ? S::TT - 1 - j : j;
       const float4 s = sdx[i][ch];
       const f2 d{s.x, s.y}, w{s.z, s.w};
-      const St v = St::shared(&sn[i][8 * q]);
+      const St v = St::shared(&sn[i][4 * q]);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+      for (int n = 0; n < kS / 2; ++n) {
         const f2 e = decay2(A2.p[n], d);
         h.p[n] = kAdjoint ? mul2(e, fma2(v.p[n], w, h.p[n])) : fma2(e, h.p[n], mul2(v.p[n], w));
       }
@@ -366,19 +371,19 @@ __global__ void __launch_bounds__(kScanThreads) scan_summary_kernel(ScanArgs a) 
   }
   if (c >= a.C) return;
   const int64_t at = ((int64_t)b * a.nseg + seg) * a.C + c;
-  h.store(a.seg_h + at * a.N, 8 * q, a.N, a.wide_n);
+  h.store(a.seg_h + at * a.N, 4 * q, a.N, a.wide_n);
   if (q == 0) a.seg_d[at] = dsum.x;
 }
 
 // A CTA walks one segment of CH channels of one sequence; LPC lanes share a
-// channel, eight states each. Tiles of TT steps are staged: d and d x of every
+// channel, kS states each. Tiles of TT steps are staged: d and d x of every
 // (step, channel) and B, C in float32, while the next tile's raw rows are already
 // under way to registers. The lanes' parts of y are summed by an exchange of four
 // steps at a time, and the gate and the output are done by whole rows again.
-template <typename T, int LPC>
+template <typename T, int LPC, int kS>
 __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(ScanArgs a) {
-  using S = FwdShape<LPC>;
-  using St = States<8>;
+  using S = FwdShape<LPC, kS>;
+  using St = States<kS, 4 * LPC>;
   __shared__ float4 sdx[S::TT][S::CH];  // d, d, d x, d x: pairs as the packed arithmetic reads them
   __shared__ __align__(16) float sbc[S::TT][2 * S::NP];
   __shared__ __align__(16) float sy[S::TT][S::CH + 8];
@@ -388,11 +393,11 @@ __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(ScanArgs a) {
   const int t_begin = seg * a.seg_len, t_end = min(t_begin + a.seg_len, a.T), t_live = min(t_end, len);
   const int64_t hc = ((int64_t)b * a.C + c) * a.N;
   const bool mine = c < a.C;
-  St A2 = St::load(a.A + (int64_t)min(c, a.C - 1) * a.N, 8 * q, a.N, a.wide_n);
+  St A2 = St::load(a.A + (int64_t)min(c, a.C - 1) * a.N, 4 * q, a.N, a.wide_n);
   A2.scale(kL2E);
   St h = St::zero();
-  if (mine && a.h0) h = St::load(a.h0 + hc, 8 * q, a.N, a.wide_n);
-  if (mine) h = scan_carry(a, b, c, 8 * q, h, A2, 0, seg, 1);
+  if (mine && a.h0) h = St::load(a.h0 + hc, 4 * q, a.N, a.wide_n);
+  if (mine) h = scan_carry(a, b, c, 4 * q, h, A2, 0, seg, 1);
 
   const int row0 = threadIdx.x / S::kPairs, cp = c0 + threadIdx.x % S::kPairs * 2;
   const bool plain = scan_plain(a, c0 + S::CH);
@@ -446,16 +451,16 @@ __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(ScanArgs a) {
 #pragma unroll 2
     for (int j = 0; j < S::TT; j += 4) {
       if (j % kScanCkpt == 0 && ckpt && t0 + j < t_live)
-        h.store(ckpt + (int64_t)((t0 + j) / kScanCkpt) * a.C * a.N, 8 * q, a.N, a.wide_n);
+        h.store(ckpt + (int64_t)((t0 + j) / kScanCkpt) * a.C * a.N, 4 * q, a.N, a.wide_n);
       float y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float4 s = sdx[j + i][ch];
         const f2 d{s.x, s.y}, w{s.z, s.w};
-        const St Bt = St::shared(&sbc[j + i][8 * q]), Ct = St::shared(&sbc[j + i][S::NP + 8 * q]);
+        const St Bt = St::shared(&sbc[j + i][4 * q]), Ct = St::shared(&sbc[j + i][S::NP + 4 * q]);
         f2 v[2];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < kS / 2; ++n) {
           h.p[n] = fma2(decay2(A2.p[n], d), h.p[n], mul2(Bt.p[n], w));
           v[n % 2] = n < 2 ? mul2(h.p[n], Ct.p[n]) : fma2(h.p[n], Ct.p[n], v[n % 2]);
         }
@@ -496,7 +501,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(ScanArgs a) {
     const int t = max(t_begin, t_live) + i / S::CH, k = c0 + i % S::CH;
     if (k < a.C) out[(int64_t)t * a.C + k] = Pair<T>::from_float(0.f);
   }
-  if (a.h_last && mine && seg == a.nseg - 1) h.store(a.h_last + hc, 8 * q, a.N, a.wide_n);
+  if (a.h_last && mine && seg == a.nseg - 1) h.store(a.h_last + hc, 4 * q, a.N, a.wide_n);
 }
 
 __device__ __forceinline__ void copy16(void* dst, const void* src, bool on) {
