@@ -180,45 +180,35 @@ int scan_check(int dtype, int64_t B, int64_t T, int64_t C, int64_t N) {
   return WKV_OK;
 }
 
-// Lanes that share a channel, with `per` states each: a power of two.
-int scan_lanes(int64_t N, int per) {
+// Lanes that share a channel with four states each: a power of two.
+int scan_lanes(int64_t N) {
   int lanes = 1;
-  while (lanes * per < N) lanes *= 2;
+  while (lanes * 4 < N) lanes *= 2;
   return lanes;
 }
 
-// Calls f(element, lanes) for the kernels of four states a lane, the backward and the step.
-template <class F>
-int scan_dispatch(int dtype, int lanes, F&& f) {
-  return with_type(dtype, [&](auto e) {
-    switch (lanes) {
-      case 1: return f(e, std::integral_constant<int, 1>{});
-      case 2: return f(e, std::integral_constant<int, 2>{});
-      case 4: return f(e, std::integral_constant<int, 4>{});
-      default: return f(e, std::integral_constant<int, 8>{});
-    }
-  });
-}
-
-// The forward's and the summaries' states a lane: eight share the reads of d, d x and
-// the exchange of y best, but up to eight states a channel two lanes of four are faster
-// than one lane of eight, with twice the CTAs and so fewer segments (16 x 1024 x 1536 with
-// 8 states 173 us and 89 + 152 us; 1 x 8000 x 1536 50 + 89 us and 54 + 101 us).
-int scan_forward_lanes(int64_t N) { return scan_lanes(N, N <= 8 ? 4 : 8); }
+// The forward's and the summaries' lanes and states a lane: eight share the reads of d,
+// d x and the exchange of y best, but up to eight states a channel two lanes of four are
+// faster than one lane of eight or of four, with twice the CTAs and so fewer segments (16 x
+// 1024 x 1536 with 8 states 173 us and 89 + 152 us, with 4 states 173 and 70 + 125).
+int scan_forward_lanes(int64_t N) { return N <= 16 ? 2 : N <= 32 ? 4 : 8; }
 template <class F>
 int scan_forward_dispatch(int dtype, int64_t N, F f) {
   return with_type(dtype, [&](auto e) {
+    constexpr std::integral_constant<int, 2> two;
     constexpr std::integral_constant<int, 4> four;
     constexpr std::integral_constant<int, 8> eight;
-    if (N <= 4) return f(e, std::integral_constant<int, 1>{}, four);
-    if (N <= 8) return f(e, std::integral_constant<int, 2>{}, four);
-    switch (scan_forward_lanes(N)) {
-      case 2: return f(e, std::integral_constant<int, 2>{}, eight);
-      case 4: return f(e, std::integral_constant<int, 4>{}, eight);
-      default: return f(e, std::integral_constant<int, 8>{}, eight);
-    }
+    if (N <= 8) return f(e, two, four);
+    if (N <= 16) return f(e, two, eight);
+    if (N <= 32) return f(e, four, eight);
+    return f(e, eight, eight);
   });
 }
+
+// Lanes of four states each that share a channel in the backward, which needs two at
+// least (one, of 128 channels a CTA, spills its registers: 657 us for 16 x 1024 x 1536
+// with 4 states, two lanes 443).
+int scan_backward_lanes(int64_t N) { return std::max(2, scan_lanes(N)); }
 
 int64_t scan_ckpts(int64_t T) { return (T + kScanCkpt - 1) / kScanCkpt; }
 
@@ -246,7 +236,8 @@ ScanPlan scan_forward_plan(int64_t B, int64_t T, int64_t C, int64_t N) {
   return scan_plan(B, T, C, kScanThreads / scan_forward_lanes(N), 6 * sm_count());
 }
 ScanPlan scan_backward_plan(int64_t B, int64_t T, int64_t C, int64_t N) {
-  return scan_plan(B, T, C, kScanBwdPer * kScanBwdThreads / scan_lanes(N, 4), 3 * sm_count());
+  const int lanes = scan_backward_lanes(N);
+  return scan_plan(B, T, C, scan_bwd_per(lanes) * kScanBwdThreads / lanes, 3 * sm_count());
 }
 
 struct ScanWs {
@@ -569,9 +560,14 @@ int selective_scan_backward(int dtype, const void* grad_out, const void* x, cons
       });
       return launched("selective_scan backward launch");
     };
-    const int lanes = scan_lanes(N, 4);
-    rc = lanes == 16 ? with_type(dtype, [&](auto e) { return main(e, std::integral_constant<int, 16>{}); })
-                     : scan_dispatch(dtype, lanes, main);
+    rc = with_type(dtype, [&](auto e) {
+      switch (scan_backward_lanes(N)) {
+        case 2: return main(e, std::integral_constant<int, 2>{});
+        case 4: return main(e, std::integral_constant<int, 4>{});
+        case 8: return main(e, std::integral_constant<int, 8>{});
+        default: return main(e, std::integral_constant<int, 16>{});
+      }
+    });
     if (rc) return rc;
   }
   const int64_t cells = B * T * 2 * N;
@@ -629,7 +625,7 @@ int selective_scan_step(int dtype, const void* x, const void* dt, const float* A
   a.B = (int)B, a.T = 1, a.C = (int)C, a.N = (int)N;
   a.softplus = softplus;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int es = (int)dtype_size(dtype), lanes = scan_lanes(N, 4);
+  const int es = (int)dtype_size(dtype), lanes = scan_lanes(N);
   a.wide_bc = N % 4 == 0 && vector_width(es, 4, {Bm, Cm}, {b_sb, c_sb}) == 4;
   a.wide_n = N % 4 == 0 && vector_width(4, 4, {A, state}, {}) == 4;
   auto go = [&](auto e, auto lanes_) {
@@ -641,8 +637,15 @@ int selective_scan_step(int dtype, const void* x, const void* dt, const float* A
     });
     return launched("selective_scan step launch");
   };
-  return lanes == 16 ? with_type(dtype, [&](auto e) { return go(e, std::integral_constant<int, 16>{}); })
-                     : scan_dispatch(dtype, lanes, go);
+  return with_type(dtype, [&](auto e) {
+    switch (lanes) {
+      case 1: return go(e, std::integral_constant<int, 1>{});
+      case 2: return go(e, std::integral_constant<int, 2>{});
+      case 4: return go(e, std::integral_constant<int, 4>{});
+      case 8: return go(e, std::integral_constant<int, 8>{});
+      default: return go(e, std::integral_constant<int, 16>{});
+    }
+  });
 }
 
 int layer_norm_forward(int dtype, const void* x, const float* weight, const float* bias, void* y, float* mean,

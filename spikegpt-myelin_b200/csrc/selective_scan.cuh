@@ -235,9 +235,8 @@ struct ScanShape {
   static constexpr int TT = kTT;         // steps of a staged tile
   static constexpr int kPairs = CH / 2;
   static constexpr int kStep = kThr / kPairs;
-  static constexpr int kRows = TT < kStep ? 1 : TT / kStep;
-  static constexpr bool kIdle = TT < kStep;  // threads of the rows past the tile stage nothing
-  static_assert(kIdle || kRows * kStep == TT, "whole rows a thread");
+  static constexpr int kRows = TT / kStep;
+  static_assert(kRows * kStep == TT, "whole rows a thread");
 };
 
 // The forward's and the summaries': kS states a lane, 1024 cells a tile.
@@ -560,10 +559,13 @@ __device__ __forceinline__ f2 tile_pair(const float (&a)[4], const float (&b)[4]
 
 // Shared memory of the backward kernel (see there), in bytes from the start.
 constexpr int kScanBwdThreads = 128;
-constexpr int kScanBwdPer = 2;  // channels of a thread
+// Channels of a thread: two share the reads of B and C and a tile's columns, where the
+// tensor core sums; with two lanes a channel one is faster (16 x 1024 x 1536 with 8
+// states 443 us, with two 488 and a pass over segments of 82).
+__host__ __device__ constexpr int scan_bwd_per(int lanes) { return lanes >= 4 ? 2 : 1; }
 template <typename T, int LPC>
 struct ScanBwdSmem {
-  using S = ScanShape<LPC, 4, kScanBwdThreads, LPC == 1 ? 8 : 16, kScanBwdPer>;
+  using S = ScanShape<LPC, 4, kScanBwdThreads, 16, scan_bwd_per(LPC)>;
   static constexpr int kWarps = kScanBwdThreads / 32;
   static constexpr int TS = S::TT;              // steps of a tile
   static constexpr int kCells = TS * S::CH;     // (step, channel) pairs of a tile
@@ -574,11 +576,11 @@ struct ScanBwdSmem {
   static constexpr int kRes = kBC + TS * 2 * S::NP * 4;              // float [3][TS][kPitch]
   static constexpr int kPart = kRes + 3 * TS * kPitch * 4;           // float [TS][warps][2 NP]
   static constexpr int kHeld = kPart + TS * kWarps * 2 * S::NP * 4;  // float [threads][4 kPer]
-  static constexpr int kBytes = kHeld + (LPC >= 4 ? kScanBwdThreads * 4 * kScanBwdPer * 4 : 0);
+  static constexpr int kBytes = kHeld + (LPC >= 4 ? kScanBwdThreads * 4 * scan_bwd_per(LPC) * 4 : 0);
 };
 
 // A CTA walks one segment of CH channels of one sequence backwards, in tiles of TS
-// steps. Per sub-chunk of 8 steps a thread runs four states of its two channels
+// steps. Per sub-chunk of 8 steps a thread runs four states of each of its channels
 // forward from the kept states, with p_t = a_t h_{t-1} in registers, and then back
 // with the adjoint (a_t again from the exponential unit, which has the time: held in
 // registers it would cost a quarter of the resident warps). The sums over states (for
@@ -590,7 +592,7 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
   using S = typename L::S;
   using St = States<4>;
   constexpr int NP = S::NP, CH = S::CH, TS = L::TS, kCells = L::kCells, kThr = kScanBwdThreads, kLane = 32 / LPC;
-  constexpr int kPer = kScanBwdPer;
+  constexpr int kPer = scan_bwd_per(LPC);
   extern __shared__ __align__(16) char smem[];
   float4* slot = reinterpret_cast<float4*>(smem);             // d, d, d x, d x of a cell
   float2* sgy = reinterpret_cast<float2*>(smem + L::kGy);     // gy, gy
@@ -712,7 +714,6 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
 #pragma unroll
     for (int k = 0; k < S::kRows; ++k) {
       const int r = row0 + k * S::kStep, at = r * CH + cl;
-      if (S::kIdle && r >= TS) break;
       const f2 x = pair_of(Vec<T, 2>::load(cur + at));
       f2 d = scan_delta(add2(pair_of(Vec<T, 2>::load(cur + kCells + at)), bias), a.softplus);
       if (t0 + r >= t_live) d = f2{0.f, 0.f};
@@ -784,7 +785,7 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
           const int i = two * 2 + ii;
           const St Bt = St::shared(bc + i * 2 * NP), Ct = St::shared(bc + i * 2 * NP + NP);
           f2 sumB[2], sumC[2];
-          float ra[kPer], rg[kPer], ry[kPer];
+          float ra[2] = {}, rg[2] = {}, ry[2] = {};
 #pragma unroll
           for (int u = 0; u < kPer; ++u) {
             const float4 s = sl[i * CH + u * kLane];
@@ -858,7 +859,7 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
               float v[3] = {u ? along[ii].y : along[ii].x, u ? gd[ii].y : gd[ii].x, u ? y[ii].y : y[ii].x};
 #pragma unroll
               for (int k = 0; k < 3; ++k) {
-                if constexpr (LPC == 2) v[k] += __shfl_xor_sync(kFull, v[k], 1);
+                v[k] += __shfl_xor_sync(kFull, v[k], 1);
                 if (q == 0) to[k * TS * L::kPitch + ii * L::kPitch + ch + u * kLane] = v[k];
               }
             }
@@ -929,7 +930,6 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
 #pragma unroll
     for (int k = 0; k < S::kRows; ++k) {
       const int r = row0 + k * S::kStep, at = r * CH + cl;
-      if (S::kIdle && r >= TS) break;
       const f2 d{slot[at].x, slot[at + 1].x};
       const float* v = res + r * L::kPitch + cl;
       const float2 al = *reinterpret_cast<const float2*>(v), ga = *reinterpret_cast<const float2*>(v + TS * L::kPitch);
