@@ -104,8 +104,13 @@ __device__ __forceinline__ void column_sums(const ColSumArgs& a, int64_t block) 
   float s = 0.f;
   if (col < width) {
     const float* p = a.in + col;
-#pragma unroll 4
-    for (int r = y; r < a.rows; r += kRows) s += p[(int64_t)r * width];
+    for (int r = y; r < a.rows; r += kRows * 10) {  // ten rows under way at a time
+      float v[10];
+#pragma unroll
+      for (int i = 0; i < 10; ++i) v[i] = r + i * kRows < a.rows ? p[(int64_t)(r + i * kRows) * width] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 10; ++i) s += v[i];
+    }
   }
   red[y][x] = s;
   __syncthreads();
