@@ -13,7 +13,12 @@
 // size e), the backward reads x and gy and writes gx. A thread holds V adjacent
 // channels and walks kConvSteps rows with the window in registers, so a row is
 // read once but for the W - 1 rows shared by neighbouring walks. The per-tap
-// sums of a walk go to a partial row and are added in a fixed order.
+// sums of a walk go to a partial row and are added in a fixed order. Measured at
+// 8 x 1024 x 1024 bfloat16: forward 16 us (2.0 TB/s), backward 30 us (1.7 TB/s), sums
+// 8 us: at this size the walks are short of warps (1024 CTAs of two) and bound by the
+// latency of their rows and the float32 arithmetic (about 10 operations an element
+// forward, 25 backward), not by memory; 5 x 1003 x 1536 float32 forward 16 us. Longer
+// walks would re-read less and leave SMs idle; shorter ones re-read more.
 #pragma once
 
 #include "row_io.cuh"

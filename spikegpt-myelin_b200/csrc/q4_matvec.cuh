@@ -4,16 +4,22 @@
 // q holds two weights a byte (even k in the low nibble), rows of ceil(K / 32) * 16
 // bytes; scales bfloat16, zeros one byte each (8 without them). float32 sums.
 //
-// Bound by the bytes of the weights while the tokens are few, so the weights are
-// read once for up to 16 tokens (8 in float32), by asynchronous copies kQ4Stages deep in a
-// ring of the warp's own: 16 R rows x 128 inputs a stage. Decoding is a logical operation and a packed subtraction for two
+// The least it can do is to read the weights once, for up to 16 tokens (8 in float32):
+// they come by asynchronous copies kQ4Stages deep in a ring of the warp's own, 16 R rows
+// x 128 inputs a stage. Decoding is a logical operation and a packed subtraction for two
 // weights (and a shift for three of four): a nibble or-ed into the mantissa of a 16-bit
 // float stands for 2^m + q, and less 2^m + zero it is exact. The products go to
 // m16n8k16 tiles (A the weights, B the tokens), whose k order is free: the pairs that a
 // word of eight nibbles gives, (0, 4), (1, 5), (2, 6), (3, 7), are taken as they come
 // and x is paired the same way. Four lanes' words make 32 inputs (64 or 128 where the
-// group allows), always of one group, whose sums are scaled in float32. float32 tokens enter as three bfloat16 terms
-// (8 + 8 + 8 bits, exact) in three columns that are added at the end.
+// group allows), always of one group, whose sums are scaled in float32. float32 tokens
+// enter as three bfloat16 terms (8 + 8 + 8 bits, exact) in three columns that are added
+// at the end.
+//
+// Measured: 6 x 8192 x 16384 bfloat16, groups of 128: 28.7 us, 2.5 TB/s of weights; 1 x 768
+// x 50257, groups of 64: 10.6 us. What bounds it is the decode: about 1.4 integer and
+// packed operations a weight, at two CTAs of eight warps an SM, take 2.5 times as long as
+// the bytes. 64 rows a warp and six stages were no faster.
 //
 // The warps of a CTA are `wk` along the inputs (every wk-th 128 of them) by the
 // others along the rows; the sums along the inputs meet in shared memory in warp order.

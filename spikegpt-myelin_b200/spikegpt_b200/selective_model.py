@@ -25,7 +25,14 @@ from torch import Tensor, nn
 
 from .norm import layer_norm
 from .q4 import dequantize_q4, q4_linear, quantize_q4
-from .selective import causal_conv, causal_conv_step_, selective_scan, selective_scan_step_
+from .selective import (
+    MAX_STATES,
+    MAX_TAPS,
+    causal_conv,
+    causal_conv_step_,
+    selective_scan,
+    selective_scan_step_,
+)
 
 # Tokens up to which a 4-bit projection decodes its weight on the fly; more are
 # multiplied by the weight decoded once (a library matrix product).
@@ -53,8 +60,8 @@ class SelectiveConfig:
         for name in ("vocab_size", "n_layer", "n_embd", "inner", "n_state", "taps", "dt_rank"):
             if getattr(self, name) <= 0:
                 raise ValueError(f"{name} must be positive")
-        if self.n_state > 64 or self.taps > 4:
-            raise ValueError("n_state must be at most 64 and taps at most 4")
+        if self.n_state > MAX_STATES or self.taps > MAX_TAPS:
+            raise ValueError(f"n_state must be at most {MAX_STATES} and taps at most {MAX_TAPS}")
 
 
 class Q4Linear(nn.Module):
