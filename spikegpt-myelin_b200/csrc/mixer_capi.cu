@@ -785,11 +785,17 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
       constexpr int R = decltype(r)::value, NT = decltype(nt)::value, GW = decltype(gw)::value;
       // Four warps a CTA where the rows alone make two such CTAs an SM, else eight; all of
       // them along the inputs as long as each has three stages or rows are short of SMs.
+      // With one tile of tokens fewer are along the inputs still while that leaves two
+      // CTAs an SM: 393 CTAs of six stages a warp run at once where 786 of three take two
+      // turns (1 x 768 x 50257 10.3 and 11.4 us a call back to back; with three tiles, whose
+      // CTAs are fewer an SM, 6 x 2048 x 16384 float32 22 and 20 us).
       const int64_t chunks = (K + kQ4Chunk - 1) / kQ4Chunk;
       const int warps = N >= 16 * R * 2 * sm_count() ? 4 : 8;
       auto ctas = [&](int wk) { return (N + 16 * R * (warps / wk) - 1) / (16 * R * (warps / wk)); };
       a.wk = warps;
-      while (a.wk > 1 && chunks < 3 * a.wk && ctas(a.wk / 2) >= sm_count()) a.wk /= 2;
+      while (a.wk > 1 && ((chunks < 3 * a.wk && ctas(a.wk / 2) >= sm_count()) ||
+                          (NT == 1 && chunks < 6 * a.wk && ctas(a.wk / 2) >= 2 * sm_count())))
+        a.wk /= 2;
       const int bytes = std::max(warps * q4_warp_bytes<E, R, NT, GW>(a.tokens), q4_sum_bytes<R, NT>(warps));
       const bool wide = vector >= (q4_direct<E, NT>() ? 8 : 4);
       auto kernel = wide ? q4_matvec_kernel<E, R, NT, GW, true> : q4_matvec_kernel<E, R, NT, GW, false>;
