@@ -14,10 +14,10 @@
 // teams, the warps' sums in warp order through shared memory, two buffers in turn so
 // that one barrier a sum is enough. The backward keeps gw and gb of its columns in
 // registers over all its rows, adds its teams' in team order and leaves one partial row
-// a CTA. Measured: 16384 x 4096 bfloat16 forward 62 us (4.3 TB/s), backward 84 us (4.8 TB/s)
-// and its column sums 10 us; 8192 x 512 float32 11, 21 and 7 us. Packed arithmetic is what
-// brought the forward of wide rows below 70 us: at two CTAs of 256 an SM it is the
-// instructions between a row's arrival and the next one's, not the bytes, that bound it.
+// a CTA. Measured, launches included: 16384 x 4096 bfloat16 forward 62 us (4.3 TB/s),
+// backward 88 us (4.6 TB/s) and its column sums 11 us; 8192 x 512 float32 15, 24 and 9 us.
+// The instructions between a row's arrival and the next one's bound it (issue slots half
+// busy, memory 42 to 51 % of its nominal rate), which is why the arithmetic is packed.
 //
 // Rows that are not 16-byte aligned (odd widths, odd pitches) move as words of V
 // values, neighbouring lanes' side by side, and are re-ordered into the same granules
@@ -173,10 +173,17 @@ __device__ __forceinline__ float2 norm_sums(float u, float v, int span, float2 (
   return make_float2(u, v);
 }
 
+// CTAs of the forward that share an SM: three of 256 threads where their 80 registers
+// hold a row without spilling, which is for whole aligned words of 16 bits (16384 x 4096
+// 61 us, with two 67; float32 rows of 1003 22 us with two, 29 with three).
+template <typename T, int V, int kThr>
+__host__ __device__ constexpr int norm_fwd_ctas() {
+  return kThr != 256 ? 1 : sizeof(T) == 2 && !NormIo<T, V>::kStaged ? 3 : 2;
+}
 // kThr: the CTA's threads, 256, 512 (rows past 4096) or 1024 (past 8192, where 64
 // registers a thread make both kernels spill: such rows are rare).
 template <typename T, int V, int kThr>
-__global__ void __launch_bounds__(kThr, kThr == 256 ? 2 : 1) layer_norm_fwd_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kThr, (norm_fwd_ctas<T, V, kThr>())) layer_norm_fwd_kernel(NormArgs a) {
   using Io = NormIo<T, V>;
   constexpr int P = Io::kPairs;
   extern __shared__ __align__(16) char smem[];
