@@ -188,6 +188,23 @@ def test_q4_what_lies_past_the_row_is_ignored(cuda):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [1, 2, 4, 5, 7, 9, 16, 19])
+@pytest.mark.parametrize("k,n,g", [(256, 9504, 128), (130, 9511, 32), (388, 19000, 64)])
+def test_q4_many_rows(cuda, m, k, n, g, dtype):
+    """Rows enough to fill the GPU, where a warp takes twice as many; a token that is not
+    finite touches no other."""
+    x, packed, scales, zp = _q4_case(m, k, n, g, dtype, cuda, seed=m)
+    ref = _q4_ref(x, packed, scales, zp, k, g)
+    y = sg.q4_linear(x, packed, scales, zp, group_size=g)
+    check("y", y, ref)
+    x[m // 2, k // 3] = float("inf")
+    spoilt = sg.q4_linear(x, packed, scales, zp, group_size=g)
+    others = torch.arange(m, device=cuda) != m // 2
+    assert torch.equal(spoilt[others], y[others])
+    assert not torch.isfinite(spoilt[m // 2]).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_q4_large_and_small_activations(cuda, dtype):
     """Tokens are independent: one at 1e4 beside one at 1e-3, and one with an infinity
     or a NaN, leave the others' values as they are."""
