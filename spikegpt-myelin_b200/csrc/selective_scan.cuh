@@ -656,7 +656,9 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
   f2 gD{0.f, 0.f}, gb{0.f, 0.f};
 
   // Raw rows come by asynchronous copies of 16 bytes, one thread always the same
-  // word of its tensors' tiles; rows without that alignment by plain loads.
+  // word of its tensors' tiles; rows without that alignment by plain loads. A copy that
+  // only writes zeros names a source all the same, which has to be aligned like any
+  // other: x's first word (`wide` says nothing of A).
   constexpr int E = 16 / (int)sizeof(T), kWords = kCells / E, kCopies = (4 * kWords + kThr - 1) / kThr;
   const T* src[kCopies];
   int64_t back[kCopies];
@@ -677,7 +679,7 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
         const int i = j * kThr + tid;
         if (kCopies * kThr > 4 * kWords && i >= 4 * kWords) break;
         const bool on = src[j] != nullptr && t0 + i % kWords * E / CH < t_live;
-        copy16(dst + i * E, on ? static_cast<const void*>(src[j] + t0 * back[j]) : a.A, on);
+        copy16(dst + i * E, on ? static_cast<const void*>(src[j] + t0 * back[j]) : a.x, on);
       }
     } else {
       for (int k = 0; k < (a.z ? 4 : 3); ++k) {
