@@ -428,8 +428,9 @@ WKV_API int layer_norm_backward(int dtype, const void* grad_y, const void* x, co
 
 /*
  * y[m][n] = bias[n] + sum_k x[m][k] scales[n][k / group] (q[n][k] - zeros[n][k / group]):
- * 4-bit weights for a few tokens. packed has rows of ceil(K / 32) * 16 bytes, weight k
- * in byte k / 2, even k in the low nibble (what lies past K is ignored). scales is
+ * 4-bit weights for a few tokens. packed is 16-byte aligned (WKV_ERR_INVALID_ARGUMENT
+ * elsewhere) and has rows of ceil(K / 32) * 16 bytes, weight k in byte k / 2, even k in
+ * the low nibble (what lies past K is ignored). scales is
  * bfloat16 and zeros uint8 (0..15; null: 8), both [N, ceil(K / group)], group a
  * multiple of 32; bias float32 [N] or null. x [M, K] has unit stride of k; y is
  * contiguous [M, N] of the same dtype. float32 sums.

@@ -755,8 +755,10 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
   if (int rc = q4_check(dtype, M, N, K, group)) return rc;
   if (M == 0 || N == 0) return WKV_OK;
   if (int rc = check_pointers({y})) return rc;
-  if (K > 0)
+  if (K > 0) {
     if (int rc = check_pointers({x, packed, scales})) return rc;
+    if (!aligned16(packed)) return fail(WKV_ERR_INVALID_ARGUMENT, "packed must be 16-byte aligned");
+  }
   Q4Args a{};
   a.x = x;
   a.q = packed;

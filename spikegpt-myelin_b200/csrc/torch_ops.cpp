@@ -616,6 +616,8 @@ Tensor q4_linear(const Tensor& x_, const Tensor& packed, const Tensor& scales, c
   }
   const c10::cuda::CUDAGuard guard(x_.device());
   const OptTensor bias = parameter(bias_);
+  // the weights come by 16-byte copies: a view at another offset of a flat buffer is copied
+  const Tensor weights = reinterpret_cast<uintptr_t>(packed.const_data_ptr()) % 16 == 0 ? packed : packed.clone();
   const Tensor x = rows(x_.dim() == 2 ? x_ : x_.reshape({-1, k}));
   const int64_t m = size_of(x, 0);
   Tensor y = empty(x, {m, n});
@@ -623,7 +625,7 @@ Tensor q4_linear(const Tensor& x_, const Tensor& packed, const Tensor& scales, c
     const int64_t few = std::min(kFewTokens, m - at);
     const char* from = static_cast<const char*>(x.const_data_ptr()) + at * x.stride(0) * x.element_size();
     char* to = static_cast<char*>(y.mutable_data_ptr()) + at * n * y.element_size();
-    check(lib().q4(code, from, static_cast<const uint8_t*>(packed.const_data_ptr()), scales.const_data_ptr(),
+    check(lib().q4(code, from, static_cast<const uint8_t*>(weights.const_data_ptr()), scales.const_data_ptr(),
                    static_cast<const uint8_t*>(ptr(zeros)), fptr(bias), to, few, n, k, group, x.stride(0),
                    stream_of(x)),
           "q4_matvec");

@@ -49,3 +49,19 @@ def test_scan_with_unaligned_parameters_and_aligned_rows(cuda, gated, b, t, c, n
     for i, a, p, r in zip(has, got, same, want):
         check(f"gradient of {ORDER[i]}", a, r)
         assert torch.equal(a, p), ORDER[i]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n,g", [(1, 64, 33, 64), (5, 300, 70, 32), (20, 130, 9511, 128)])
+def test_q4_weights_at_any_offset(cuda, m, k, n, g, dtype):
+    """Packed weights, scales and zero points as views into flat buffers: the values of
+    the same weights by themselves."""
+    gen = torch.Generator().manual_seed(k)
+    packed, scales, zeros = sg.quantize_q4((torch.randn(n, k, generator=gen) / k**0.5).to(cuda), g)
+    x = torch.randn(m, k, generator=gen).to(cuda, dtype)
+    want = sg.q4_linear(x, packed, scales, zeros, group_size=g)
+    check("y", want, x.double() @ sg.dequantize_q4(packed, scales, zeros, k, g).double().t())
+    for offset in (1, 2, 8, 16):
+        moved = [at_offset(v, offset) for v in (packed, scales, zeros)]
+        assert moved[0].data_ptr() % 16 == offset % 16
+        assert torch.equal(sg.q4_linear(x, *moved, group_size=g), want)
