@@ -387,8 +387,9 @@ WKV_API int causal_conv_step(int dtype, const void* x, const float* weight, cons
  * past its sequence's length is not read, leaves the state as it is and gives zeros.
  * kept (selective_scan_state_size bytes, or null): the states that the backward
  * starts from, written by the forward. The sums over sequences and channels have a
- * fixed order. selective_scan_step is one token (x, dt, z [B, C]; B, C [B, N]) that
- * updates the state in place.
+ * fixed order. A workspace (where its size is not 0) is 16-byte aligned, or the call
+ * returns WKV_ERR_INVALID_ARGUMENT. selective_scan_step is one token (x, dt, z [B, C];
+ * B, C [B, N]) that updates the state in place.
  */
 WKV_API size_t selective_scan_state_size(int64_t B, int64_t T, int64_t C, int64_t N);
 WKV_API size_t selective_scan_forward_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int64_t N);

@@ -455,6 +455,7 @@ int selective_scan_forward(int dtype, const void* x, const void* dt, const float
   if (workspace_bytes < need || (need > 0 && !workspace))
     return fail(WKV_ERR_WORKSPACE_TOO_SMALL, "selective_scan forward needs %zu workspace bytes, got %zu", need,
                 workspace_bytes);
+  if (need > 0 && !aligned16(workspace)) return fail(WKV_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
   scan_layout(a, p, scan_ws(p, false, B, T, C, N, workspace), dtype, {x, dt, z, out}, {A, state_in, state_out, kept});
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return scan_forward_dispatch(dtype, N, [&](auto e, auto lanes, auto states) {
@@ -505,6 +506,7 @@ int selective_scan_backward(int dtype, const void* grad_out, const void* x, cons
   if (workspace_bytes < need || (need > 0 && !workspace))
     return fail(WKV_ERR_WORKSPACE_TOO_SMALL, "selective_scan backward needs %zu workspace bytes, got %zu", need,
                 workspace_bytes);
+  if (need > 0 && !aligned16(workspace)) return fail(WKV_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
   const ScanWs ws = scan_ws(p, true, B, T, C, N, workspace);
   ScanArgs a{};
   a.gout = grad_out;

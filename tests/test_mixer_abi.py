@@ -23,3 +23,23 @@ def test_q4_matvec_refuses_unaligned_weights(dtype, offset):
     assert _capi.lib().q4_matvec(dtype, p, at(offset), p, None, None, p, 1, 8, 64, 64, 64, None) == (
         _capi.WKV_ERR_INVALID_ARGUMENT)
     assert "packed must be 16-byte aligned" in _capi.last_error()
+
+
+@pytest.mark.parametrize("offset", [1, 2, 4, 8])
+def test_scan_refuses_an_unaligned_workspace(offset):
+    """Its partial states move as 16-byte words."""
+    lib, p, null = _capi.lib(), at(), None
+    b, t, c, n = 1, 4096, 64, 16  # few channels and many steps: split over time
+    strides = [t * c, c, t * c, c, t * n, n, t * n, n, 0, 0]
+    size = lib.selective_scan_forward_workspace_size(0, b, t, c, n)
+    assert size > 0
+    assert lib.selective_scan_forward(0, p, p, p, p, p, null, null, null, null, null, p, null, null, 0, at(offset), size,
+                                      b, t, c, n, *strides, 1, null) == _capi.WKV_ERR_INVALID_ARGUMENT
+    assert "workspace must be 16-byte aligned" in _capi.last_error()
+    for t in (8, 4096):
+        strides = [t * c, c, t * c, c, t * c, c, t * n, n, t * n, n, 0, 0]
+        size = lib.selective_scan_backward_workspace_size(0, b, t, c, n)
+        assert lib.selective_scan_backward(0, p, p, p, p, p, p, null, null, null, p, null, null, p, p, p, p, p, null,
+                                           null, null, null, at(offset), size, b, t, c, n, *strides, 1, null) == (
+            _capi.WKV_ERR_INVALID_ARGUMENT)
+        assert "workspace must be 16-byte aligned" in _capi.last_error()
