@@ -145,6 +145,18 @@ class SelectiveBlock(nn.Module):
         return x + self.out_proj(y)
 
 
+def _last_rows(x: Tensor, lengths: Tensor | None) -> Tensor:
+    """The row of x [B, T, C] at each sequence's last token, zeros where it has none; lengths
+    outside 0..T count as the nearest of them, as in the operators."""
+    b, t, c = x.shape
+    if t == 0:
+        return x.new_zeros(b, c)
+    if lengths is None:
+        return x[:, -1].contiguous()
+    rows = x[torch.arange(b, device=x.device), lengths.long().clamp(1, t) - 1]
+    return torch.where(lengths[:, None] > 0, rows, rows.new_zeros(()))
+
+
 class SelectiveLM(nn.Module):
     """Embedding, ``SelectiveBlock``s, a final norm and the head. ``forward(ids,
     targets)`` returns the mean cross-entropy, ``forward(ids)`` the logits."""
@@ -175,14 +187,15 @@ class SelectiveLM(nn.Module):
     @torch.no_grad()
     def prefill(self, ids: Tensor, lengths: Tensor | None = None) -> tuple[Tensor, list[SelectiveState]]:
         """Logits after each sequence's last token [B, V] and the blocks' states. ``ids``
-        [B, T] is padded on the right to the longest of ``lengths`` (default: all T)."""
+        [B, T] is padded on the right to the longest of ``lengths`` (default: all T; more
+        than T counts as T). A sequence of length 0 has read nothing: its states are zeros
+        and its logits those of a residual stream of zeros."""
         x = self.embedding(ids)
         states = []
         for block in self.blocks:
             x, state = block(x, lengths=lengths, return_state=True)
             states.append(state)
-        last = x[:, -1] if lengths is None else x[torch.arange(x.shape[0], device=x.device), lengths.long() - 1]
-        return self.head(layer_norm(last.contiguous(), self.norm_weight, self.norm_bias)), states
+        return self.head(layer_norm(_last_rows(x, lengths), self.norm_weight, self.norm_bias)), states
 
     @torch.no_grad()
     def step(self, tokens: Tensor, states: list[SelectiveState]) -> Tensor:
