@@ -174,6 +174,14 @@ bool wants_grad(std::initializer_list<const OptTensor*> ts) {
 void no_grad_only(const char* op, std::initializer_list<const OptTensor*> ts) {
   TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad(ts), "spikegpt_b200.", op, " has no gradient; call it under torch.no_grad()");
 }
+// Forward-mode derivatives (dual tensors, torch.func.jvp) are not there; without this a
+// tangent would be lost below autograd without a word.
+void no_tangents(const char* op, std::initializer_list<const OptTensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const OptTensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!has(*t) || !(*t)->_fw_grad(/*level=*/0).defined(), "spikegpt_b200.", op,
+                                " has no forward-mode derivative");
+}
 template <class F>
 auto typed(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
@@ -253,6 +261,8 @@ Tensor norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, dou
   need_shape("weight", weight, {c});
   need_shape("bias", bias, {c});
   need_cuda("layer_norm", x, {&weight, &bias});
+  const OptTensor ox = x;
+  no_tangents("layer_norm", {&ox, &weight, &bias});
   const OptTensor w = parameter(weight), b = parameter(bias);
   const Tensor flat = rows(x.dim() == 2 ? x : x.reshape({-1, c}));
   Tensor y;
@@ -355,6 +365,8 @@ Tensor2 conv(const Tensor& x_, const Tensor& weight, const OptTensor& bias, cons
   need_dtype("initial_state", state, x_.scalar_type(), "x");
   const OptTensor weight_ = weight;
   need_cuda("causal_conv", x_, {&weight_, &bias, &state, &lengths});
+  const OptTensor ox_ = x_;
+  no_tangents("causal_conv", {&ox_, &weight_, &bias, &state});
   const Tensor wt = parameter(weight), x = rows(x_);
   const OptTensor bi = parameter(bias), lens = lengths_of(lengths, b);
   const OptTensor window = has(state) ? OptTensor(state->contiguous()) : OptTensor();
@@ -382,13 +394,12 @@ Tensor conv_step(const Tensor& x_, const Tensor& state, const Tensor& weight, co
   TORCH_CHECK_VALUE(x_.dim() == 2, "x must have shape [B, C]; got ", shape_of(x_));
   const int64_t b = size_of(x_, 0), c = size_of(x_, 1), w = conv_weight(weight, c);
   const int code = code_of("x", x_);
-  const OptTensor os = state, ow = weight, ox = x_;
+  const OptTensor os = state, ow = weight;
   need_shape("state", os, {b, w - 1, c});
   need_dtype("state", os, x_.scalar_type(), "x");
   need_shape("bias", bias, {c});
   need_cuda("causal_conv_step_", x_, {&os, &ow, &bias});
   TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous");
-  no_grad_only("causal_conv_step_", {&ox, &os, &ow, &bias});
   if (x_.is_meta()) return at::empty_like(x_, {}, at::MemoryFormat::Contiguous);
   const c10::cuda::CUDAGuard guard(x_.device());
   const Tensor x = rows(x_), wt = parameter(weight);
@@ -541,6 +552,7 @@ Tensor2 scan(const Tensor& x_, const Tensor& dt_, const Tensor& A_, const Tensor
   need_shape("initial_state", state, {b, c, n});
   TORCH_CHECK_VALUE(!has(state) || state->scalar_type() == at::kFloat, "initial_state must be float32");
   need_cuda("selective_scan", x_, {&od, &oA, &oB, &oC, &D_, &z_, &dt_bias_, &state, &lengths});
+  no_tangents("selective_scan", {&ox, &od, &oA, &oB, &oC, &D_, &z_, &dt_bias_, &state});
   const Tensor x = rows(x_), dt = rows(dt_), A = parameter(A_), B = rows(B_), C = rows(C_);
   const OptTensor D = parameter(D_), z = rows(z_), dt_bias = parameter(dt_bias_), lens = lengths_of(lengths, b);
   const OptTensor h0 = has(state) ? OptTensor(state->contiguous()) : OptTensor();
@@ -559,7 +571,7 @@ Tensor scan_step(const Tensor& x_, const Tensor& dt_, const Tensor& A_, const Te
   TORCH_CHECK_VALUE(x_.dim() == 2, "x must have shape [B, C]; got ", shape_of(x_));
   const int64_t b = size_of(x_, 0), c = size_of(x_, 1), n = scan_parameters(A_, D_, dt_bias_, c);
   const int code = code_of("x", x_);
-  const OptTensor od = dt_, oA = A_, oB = B_, oC = C_, ox = x_, os = state;
+  const OptTensor od = dt_, oA = A_, oB = B_, oC = C_, os = state;
   need_shape("dt", od, {b, c});
   need_shape("z", z_, {b, c});
   need_shape("B", oB, {b, n});
@@ -571,7 +583,6 @@ Tensor scan_step(const Tensor& x_, const Tensor& dt_, const Tensor& A_, const Te
   need_shape("state", os, {b, c, n});
   TORCH_CHECK_VALUE(state.scalar_type() == at::kFloat && state.is_contiguous(), "state must be contiguous float32");
   need_cuda("selective_scan_step_", x_, {&od, &oA, &oB, &oC, &os, &D_, &z_, &dt_bias_});
-  no_grad_only("selective_scan_step_", {&ox, &od, &oA, &oB, &oC, &os, &D_, &z_, &dt_bias_});
   if (x_.is_meta()) return at::empty_like(x_, {}, at::MemoryFormat::Contiguous);
   const c10::cuda::CUDAGuard guard(x_.device());
   const Tensor x = rows(x_), dt = rows(dt_), A = parameter(A_), B = rows(B_), C = rows(C_);
@@ -598,7 +609,7 @@ Tensor q4_linear(const Tensor& x_, const Tensor& packed, const Tensor& scales, c
                     "packed must be uint8 [N, ", pitch, "] for ", k, " inputs; got ", packed.scalar_type(), " ",
                     shape_of(packed));
   const int64_t n = size_of(packed, 0);
-  const OptTensor op = packed, os = scales, ox = x_;
+  const OptTensor op = packed, os = scales;
   need_shape("scales", os, {n, groups});
   need_shape("zeros", zeros, {n, groups});
   need_shape("bias", bias_, {n});
@@ -608,7 +619,6 @@ Tensor q4_linear(const Tensor& x_, const Tensor& packed, const Tensor& scales, c
   need_cuda("q4_linear", x_, {&op, &os, &zeros, &bias_});
   TORCH_CHECK_VALUE(packed.is_contiguous() && scales.is_contiguous() && (!has(zeros) || zeros->is_contiguous()),
                     "packed, scales and zeros must be contiguous");
-  no_grad_only("q4_linear", {&ox, &bias_});
   if (x_.is_meta()) {
     c10::SymDimVector shape(x_.sym_sizes().begin(), x_.sym_sizes().end());
     shape.back() = n;
@@ -634,6 +644,40 @@ Tensor q4_linear(const Tensor& x_, const Tensor& packed, const Tensor& scales, c
   auto shape = x_.sizes().vec();
   shape.back() = n;
   return y.view(shape);
+}
+
+// ------------------------------------- the operators without a gradient
+//
+// Autograd kernels that refuse inputs which want a derivative. They see what the kernels
+// below them do not: the tensors of torch.func's transforms.
+
+Tensor conv_step_autograd(const Tensor& x, const Tensor& state, const Tensor& weight, const OptTensor& bias,
+                          bool silu) {
+  static const auto op = typed<decltype(conv_step)>("spikegpt_b200::causal_conv_step_");
+  const OptTensor ox = x, os = state, ow = weight;
+  no_grad_only("causal_conv_step_", {&ox, &os, &ow, &bias});
+  no_tangents("causal_conv_step_", {&ox, &os, &ow, &bias});
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, state, weight, bias, silu);
+}
+Tensor scan_step_autograd(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
+                          const Tensor& state, const OptTensor& D, const OptTensor& z, const OptTensor& dt_bias,
+                          bool softplus) {
+  static const auto op = typed<decltype(scan_step)>("spikegpt_b200::selective_scan_step_");
+  const OptTensor ox = x, od = dt, oA = A, oB = B, oC = C, os = state;
+  no_grad_only("selective_scan_step_", {&ox, &od, &oA, &oB, &oC, &os, &D, &z, &dt_bias});
+  no_tangents("selective_scan_step_", {&ox, &od, &oA, &oB, &oC, &os, &D, &z, &dt_bias});
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, dt, A, B, C, state, D, z, dt_bias, softplus);
+}
+Tensor q4_linear_autograd(const Tensor& x, const Tensor& packed, const Tensor& scales, const OptTensor& zeros,
+                          const OptTensor& bias, int64_t group) {
+  static const auto op = typed<decltype(q4_linear)>("spikegpt_b200::q4_linear");
+  const OptTensor ox = x, os = scales;
+  no_grad_only("q4_linear", {&ox, &os, &bias});
+  no_tangents("q4_linear", {&ox, &os, &bias});
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, packed, scales, zeros, bias, group);
 }
 
 }  // namespace
@@ -686,10 +730,15 @@ TORCH_LIBRARY_IMPL(spikegpt_b200, Meta, m) {
   m.impl("selective_scan_bwd", &scan_bwd_meta);
 }
 
-// The steps and the 4-bit product have no gradient: one kernel each, which refuses
-// inputs that want one.
+// The steps and the 4-bit product have no gradient.
 TORCH_LIBRARY_IMPL(spikegpt_b200, CompositeExplicitAutograd, m) {
   m.impl("causal_conv_step_", &conv_step);
   m.impl("selective_scan_step_", &scan_step);
   m.impl("q4_linear", &q4_linear);
+}
+
+TORCH_LIBRARY_IMPL(spikegpt_b200, Autograd, m) {
+  m.impl("causal_conv_step_", &conv_step_autograd);
+  m.impl("selective_scan_step_", &scan_step_autograd);
+  m.impl("q4_linear", &q4_linear_autograd);
 }
