@@ -651,14 +651,25 @@ Tensor q4_linear(const Tensor& x_, const Tensor& packed, const Tensor& scales, c
 // Autograd kernels that refuse inputs which want a derivative. They see what the kernels
 // below them do not: the tensors of torch.func's transforms.
 
+// Tells autograd that a tensor was written in place, so that a backward which saved it
+// refuses to run. (An inference tensor cannot be saved and has no version.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
 Tensor conv_step_autograd(const Tensor& x, const Tensor& state, const Tensor& weight, const OptTensor& bias,
                           bool silu) {
   static const auto op = typed<decltype(conv_step)>("spikegpt_b200::causal_conv_step_");
   const OptTensor ox = x, os = state, ow = weight;
   no_grad_only("causal_conv_step_", {&ox, &os, &ow, &bias});
   no_tangents("causal_conv_step_", {&ox, &os, &ow, &bias});
-  at::AutoDispatchBelowADInplaceOrView below;
-  return op.call(x, state, weight, bias, silu);
+  Tensor y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    y = op.call(x, state, weight, bias, silu);
+  }
+  written(state);
+  return y;
 }
 Tensor scan_step_autograd(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
                           const Tensor& state, const OptTensor& D, const OptTensor& z, const OptTensor& dt_bias,
@@ -667,8 +678,13 @@ Tensor scan_step_autograd(const Tensor& x, const Tensor& dt, const Tensor& A, co
   const OptTensor ox = x, od = dt, oA = A, oB = B, oC = C, os = state;
   no_grad_only("selective_scan_step_", {&ox, &od, &oA, &oB, &oC, &os, &D, &z, &dt_bias});
   no_tangents("selective_scan_step_", {&ox, &od, &oA, &oB, &oC, &os, &D, &z, &dt_bias});
-  at::AutoDispatchBelowADInplaceOrView below;
-  return op.call(x, dt, A, B, C, state, D, z, dt_bias, softplus);
+  Tensor y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    y = op.call(x, dt, A, B, C, state, D, z, dt_bias, softplus);
+  }
+  written(state);
+  return y;
 }
 Tensor q4_linear_autograd(const Tensor& x, const Tensor& packed, const Tensor& scales, const OptTensor& zeros,
                           const OptTensor& bias, int64_t group) {

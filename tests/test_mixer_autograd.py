@@ -72,3 +72,37 @@ def test_function_transforms_do_not_lose_a_gradient(op):
     f, args = _inputs()[op]
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda v: f(**{**args, "x": v}).sum())(args["x"])
+
+
+@pytest.mark.parametrize("op", ["causal_conv_step_", "selective_scan_step_"])
+def test_steps_say_that_they_write_in_place(op):
+    f, args = _inputs()[op]
+    holder = zeros(2, *args["state"].shape)
+    for state in (args["state"], holder[1]):
+        before = state._version
+        f(**{**args, "state": state})
+        assert state._version == before + 1
+    assert holder._version == 1
+    with torch.no_grad():
+        f(**args)
+    assert args["state"]._version == 2
+    with pytest.raises(ValueError):
+        f(**{**args, "x": args["x"][:1]})
+    with torch.inference_mode():
+        held = zeros(*args["state"].shape)
+        f(**{**args, "state": held})
+    with torch.no_grad():
+        f(**{**args, "state": held})
+
+
+def test_a_step_on_a_saved_window_is_noticed():
+    """causal_conv saves its initial window; a step on that window before the backward
+    would give other gradients."""
+    weight = zeros(C, W).requires_grad_()
+    window = zeros(B, W - 1, C)
+    y = sg.causal_conv(zeros(B, T, C), weight, initial_state=window)
+    y.sum().backward(retain_graph=True)
+    with torch.no_grad():
+        sg.causal_conv_step_(zeros(B, C), window, weight)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
