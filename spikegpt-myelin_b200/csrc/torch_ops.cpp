@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -182,6 +183,17 @@ void no_tangents(const char* op, std::initializer_list<const OptTensor*> ts) {
     TORCH_CHECK_NOT_IMPLEMENTED(!has(*t) || !(*t)->_fw_grad(/*level=*/0).defined(), "spikegpt_b200.", op,
                                 " has no forward-mode derivative");
 }
+// A call of a backward operator. While a graph of the gradients is recorded
+// (create_graph) it goes through their Autograd kernel, which gives them a node that
+// raises: there are no second derivatives.
+template <class F>
+auto backward_call(const char* op, const Tensor& g, const OptTensor& other, F&& call) {
+  const OptTensor og = g;
+  no_tangents(op, {&og, &other});
+  if (at::GradMode::is_enabled()) return call();
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call();
+}
 template <class F>
 auto typed(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
@@ -247,8 +259,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const auto saved = ctx->get_saved_variables();
     const bool want_w = ctx->saved_data["w"].toBool(), want_b = ctx->saved_data["b"].toBool();
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    auto [gx, gw, gb] = op.call(grads[0].to(saved[0].scalar_type()), saved[0], some(saved[1]), saved[2], saved[3],
-                                want_w, want_b);
+    const Tensor g = grads[0].to(saved[0].scalar_type());
+    auto [gx, gw, gb] = backward_call("layer_norm", g, {}, [&] {
+      return op.call(g, saved[0], some(saved[1]), saved[2], saved[3], want_w, want_b);
+    });
     return {gx, want_w ? gw : Tensor(), want_b ? gb : Tensor(), Tensor()};
   }
 };
@@ -343,8 +357,10 @@ struct CausalConv : torch::autograd::Function<CausalConv> {
     const auto s = ctx->get_saved_variables();
     const bool want = ctx->saved_data["window"].toBool();
     if (!grads[0].defined()) return variable_list(6);
-    auto [gx, gw, gb, gwin] = op.call(grads[0].to(s[0].scalar_type()), s[0], s[1], some(s[2]), some(s[3]), some(s[4]),
-                                      ctx->saved_data["silu"].toBool(), want);
+    const Tensor g = grads[0].to(s[0].scalar_type());
+    auto [gx, gw, gb, gwin] = backward_call("causal_conv", g, {}, [&] {
+      return op.call(g, s[0], s[1], some(s[2]), some(s[3]), some(s[4]), ctx->saved_data["silu"].toBool(), want);
+    });
     return {gx, gw, s[2].defined() ? gb : Tensor(), want ? gwin : Tensor(), Tensor(), Tensor()};
   }
 };
@@ -517,8 +533,10 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
     variable_list r(12);
     if (!grads[0].defined() && !grads[1].defined()) return r;
     const Tensor g = grads[0].defined() ? grads[0].to(s[0].scalar_type()) : at::zeros_like(s[0]);
-    const auto got = op.call(g, s[0], s[1], s[2], s[3], s[4], some(s[5]), some(s[6]), some(s[7]), some(s[8]), s[9],
-                             some(grads[1]), ctx->saved_data["softplus"].toBool(), want_h0);
+    const auto got = backward_call("selective_scan", g, some(grads[1]), [&] {
+      return op.call(g, s[0], s[1], s[2], s[3], s[4], some(s[5]), some(s[6]), some(s[7]), some(s[8]), s[9],
+                     some(grads[1]), ctx->saved_data["softplus"].toBool(), want_h0);
+    });
     const bool on[9] = {true, true, true, true, true, s[5].defined(), s[6].defined(), s[7].defined(), want_h0};
     for (int i = 0; i < 9; ++i)
       if (on[i]) r[i] = got[i];
@@ -757,4 +775,7 @@ TORCH_LIBRARY_IMPL(spikegpt_b200, Autograd, m) {
   m.impl("causal_conv_step_", &conv_step_autograd);
   m.impl("selective_scan_step_", &scan_step_autograd);
   m.impl("q4_linear", &q4_linear_autograd);
+  m.impl("layer_norm_bwd", torch::autograd::autogradNotImplementedFallback());
+  m.impl("causal_conv_bwd", torch::autograd::autogradNotImplementedFallback());
+  m.impl("selective_scan_bwd", torch::autograd::autogradNotImplementedFallback());
 }

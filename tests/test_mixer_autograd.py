@@ -106,3 +106,42 @@ def test_a_step_on_a_saved_window_is_noticed():
         sg.causal_conv_step_(zeros(B, C), window, weight)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+DIFFERENTIABLE = [c for c in CASES if c[0] not in NO_GRADIENT]
+LINEAR = [("layer_norm", "bias"), ("selective_scan", "initial_state")]  # their gradients do not depend on them
+
+
+@pytest.mark.parametrize("op,name", DIFFERENTIABLE)
+def test_second_derivatives_are_refused(op, name):
+    """With create_graph the gradients can be used, and differentiating them raises: a
+    gradient penalty must not train on nothing."""
+    f, args = _inputs()[op]
+    leaf = args[name].requires_grad_()
+    y = f(**args)
+    (grad,) = torch.autograd.grad(y.sum(), leaf, create_graph=True)
+    assert grad.requires_grad == ((op, name) not in LINEAR) and grad.shape == leaf.shape
+    if grad.requires_grad:
+        with pytest.raises((RuntimeError, NotImplementedError), match="not implemented"):
+            grad.sum().backward()
+    y = f(**args)
+    cotangent = zeros(*y.shape).requires_grad_()
+    (grad,) = torch.autograd.grad(y, leaf, cotangent, create_graph=True)
+    with pytest.raises((RuntimeError, NotImplementedError), match="not implemented"):
+        torch.autograd.grad(grad.sum(), cotangent)
+    y = f(**args)
+    assert not torch.autograd.grad(y.sum(), leaf)[0].requires_grad
+
+
+@pytest.mark.parametrize("op", ["layer_norm", "causal_conv", "selective_scan"])
+def test_tangents_of_a_gradient_are_refused(op):
+    f, args = _inputs()[op]
+    x = args["x"].requires_grad_()
+    y = f(**args)
+    with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.autograd.grad(y, x, fwAD.make_dual(zeros(*y.shape), zeros(*y.shape)))
+    if op == "selective_scan":  # its gradients come as a list, which has no batched form
+        return
+    y = f(**args)
+    (many,) = torch.autograd.grad(y, x, zeros(3, *y.shape), is_grads_batched=True)
+    assert many.shape == (3, *x.shape)

@@ -49,3 +49,20 @@ def test_vmap_is_a_loop_over_calls(cuda):
     for f in (lambda v: sg.layer_norm(v, bias), lambda v: sg.causal_conv(v, weight, bias),
               lambda v: sg.q4_linear(v, *packed, group_size=32)):  # fmt: skip
         assert torch.equal(torch.vmap(f)(x), torch.stack([f(v) for v in x]))
+
+
+def test_gradients_recorded_for_a_graph_of_gradients_are_the_same(cuda):
+    ins, _, g = scan_inputs(2, 30, 40, 16, torch.float32, cuda, seed=53)
+    names = ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")
+    leaves = [ins[k].requires_grad_() for k in names]
+
+    def loss():
+        u = sg.causal_conv(leaves[0], weight, leaves[7])
+        return (sg.layer_norm(sg.selective_scan(u, *leaves[1:]), leaves[5]) * g).sum()
+
+    weight = torch.randn(40, 4, generator=torch.Generator().manual_seed(2)).to(cuda).requires_grad_()
+    plain = torch.autograd.grad(loss(), [*leaves, weight])
+    recorded = torch.autograd.grad(loss(), [*leaves, weight], create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, recorded))
+    with pytest.raises((RuntimeError, NotImplementedError), match="not implemented"):
+        sum((v * v).sum() for v in recorded).backward()
