@@ -495,7 +495,14 @@ int selective_scan_backward(int dtype, const void* grad_out, const void* x, cons
                             int64_t c_st, int64_t z_sb, int64_t z_st, int softplus, void* stream) {
   g_last_error[0] = '\0';
   if (int rc = scan_check(dtype, B, T, C, N)) return rc;
-  if (C == 0) return WKV_OK;
+  if (C == 0) {  // the sums over channels are there all the same
+    const size_t bytes = (size_t)B * T * N * dtype_size(dtype);
+    if (bytes == 0) return WKV_OK;
+    if (int rc = check_pointers({grad_B, grad_C})) return rc;
+    cudaError_t e = cudaMemsetAsync(grad_B, 0, bytes, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) e = cudaMemsetAsync(grad_C, 0, bytes, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WKV_OK : cuda_fail(e, "zeroing the gradients of B and C");
+  }
   if (int rc = check_pointers({A, grad_A})) return rc;
   if (B > 0 && T > 0)
     if (int rc = check_pointers({grad_out, x, dt, Bm, Cm, kept, grad_x, grad_dt, grad_B, grad_C})) return rc;

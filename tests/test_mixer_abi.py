@@ -43,3 +43,13 @@ def test_scan_refuses_an_unaligned_workspace(offset):
                                            null, null, null, at(offset), size, b, t, c, n, *strides, 1, null) == (
             _capi.WKV_ERR_INVALID_ARGUMENT)
         assert "workspace must be 16-byte aligned" in _capi.last_error()
+
+
+def test_scan_backward_without_channels_has_sums_to_write():
+    """grad_B and grad_C [B, T, N] exist where there is no channel to add up."""
+    lib, p, null = _capi.lib(), at(), None
+    strides = [0] * 12
+    for b, t, want in ((2, 3, _capi.WKV_ERR_INVALID_ARGUMENT), (0, 3, 0), (2, 0, 0)):
+        assert lib.selective_scan_backward(0, null, null, null, null, p, p, null, null, null, null, null, null, null,
+                                           null, null, null, null, null, null, null, null, null, 0, b, t, 0, 4,
+                                           *strides, 1, null) == want
