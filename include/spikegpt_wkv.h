@@ -432,9 +432,9 @@ WKV_API int layer_norm_backward(int dtype, const void* grad_y, const void* x, co
  * 4-bit weights for a few tokens. packed is 16-byte aligned (WKV_ERR_INVALID_ARGUMENT
  * elsewhere) and has rows of ceil(K / 32) * 16 bytes, weight k in byte k / 2, even k in
  * the low nibble (what lies past K is ignored). scales is
- * bfloat16 and zeros uint8 (0..15; null: 8), both [N, ceil(K / group)], group a
- * multiple of 32; bias float32 [N] or null. x [M, K] has unit stride of k; y is
- * contiguous [M, N] of the same dtype. float32 sums.
+ * bfloat16 and zeros uint8 (any value, made for 0..15; null: 8), both
+ * [N, ceil(K / group)], group a multiple of 32; bias float32 [N] or null. x [M, K] has
+ * unit stride of k; y is contiguous [M, N] of the same dtype. float32 sums.
  */
 WKV_API int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scales, const uint8_t* zeros,
               const float* bias, void* y, int64_t M, int64_t N, int64_t K, int64_t group, int64_t x_stride,

@@ -2,13 +2,14 @@
 //
 //   y[m][n] = sum_k x[m][k] * scale[n][k / G] * (q[n][k] - zero[n][k / G]) (+ bias[n])
 // q holds two weights a byte (even k in the low nibble), rows of ceil(K / 32) * 16
-// bytes; scales bfloat16, zeros one byte each (8 without them). float32 sums.
+// bytes; scales bfloat16, zeros one byte each (8 without them; any value). float32 sums.
 //
 // The least it can do is to read the weights once, for up to 16 tokens (8 in float32):
 // they come by asynchronous copies kQ4Stages deep in a ring of the warp's own, 16 R rows
 // x 128 inputs a stage. Decoding is a logical operation and a packed subtraction for two
 // weights (and a shift for three of four): a nibble or-ed into the mantissa of a 16-bit
-// float stands for 2^m + q, and less 2^m + zero it is exact. The products go to
+// float stands for 2^m + q, and less 2^m + zero it is exact (in bfloat16 up to a zero of
+// 127; for the others see q4_far_zeros). The products go to
 // m16n8k16 tiles (A the weights, B the tokens), whose k order is free: the pairs that a
 // word of eight nibbles gives, (0, 4), (1, 5), (2, 6), (3, 7), are taken as they come
 // and x is paired the same way. Four lanes' words make 32 inputs (64 or 128 where the
@@ -68,6 +69,7 @@ struct Q4Math;
 template <>
 struct Q4Math<__nv_bfloat16> {
   static constexpr uint32_t kBase = 0x43004300u;  // 128: a nibble fills the mantissa's last bits
+  static constexpr int kMostZero = 127;           // 128 + zero keeps the exponent
   static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -83,6 +85,7 @@ struct Q4Math<__nv_bfloat16> {
 template <>
 struct Q4Math<__half> {
   static constexpr uint32_t kBase = 0x64006400u;  // 1024
+  static constexpr int kMostZero = 255;           // any byte
   static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -158,6 +161,26 @@ __device__ __forceinline__ void q4_split(uint4 v, uint2 (&t)[3]) {
 #pragma unroll
   for (int e = 0; e < 3; ++e)
     t[e] = make_uint2(__byte_perm(u[e][0], u[e][1], 0x7632), __byte_perm(u[e][2], u[e][3], 0x7632));
+}
+
+// The product of token m and row n once more, if one of the row's zero points has no room
+// next to kBase. Zero points of 4-bit weights are 0 to 15, so this is made to cost the
+// usual path nothing, not for speed.
+template <typename T>
+__device__ __forceinline__ void q4_far_zeros(const Q4Args& a, int m, int n, int most) {
+  const uint8_t *zero = a.zero + (int64_t)n * a.groups, *q = a.q + (int64_t)n * a.pitch;
+  const T* x = static_cast<const T*>(a.x) + m * a.x_s;
+  bool far = false;
+  for (int g = 0; g < a.groups; ++g) far |= zero[g] > most;
+  if (!far) return;
+  float y = a.bias ? a.bias[n] : 0.f;
+  for (int g = 0, k = 0; g < a.groups; ++g) {
+    float sum = 0.f;
+    for (const int end = k + min(a.K - k, a.G); k < end; ++k)
+      sum = fmaf((float)((q[k >> 1] >> (k & 1) * 4 & 15) - zero[g]), Pair<T>::scalar(x[k]), sum);
+    y = fmaf(__bfloat162float(a.scale[(int64_t)n * a.groups + g]), sum, y);
+  }
+  static_cast<T*>(a.y)[(int64_t)m * a.N + n] = Pair<T>::from_float(y);
 }
 
 // GW: words of eight weights that a lane takes side by side, 1, 2 or 4: the four lanes'
@@ -262,10 +285,12 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
   };
   auto keep = [&](int i) {
 #pragma unroll
-    for (int p = 0; p < kPer; ++p)
+    for (int p = 0; p < kPer; ++p) {
+      if (fz[p] > Math::kMostZero) fs[p] = 0xffff;  // a NaN: the row is worked out again at the end
       if (kEntries % 32 == 0 || lane < kEntries)
         sz[(i & 1) * kEntries + p * 32 + lane] =
             make_float2(__uint_as_float((uint32_t)fs[p] << 16), __uint_as_float(Math::kBase + fz[p] * 0x10001u));
+    }
   };
 
   float acc[R][NT][4];
@@ -372,6 +397,7 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
       for (int i = 0; i < 4; ++i)
         sum[(warp * rows + r * 16 + g + i / 2 * 8) * kPitch + t * 8 + j * 2 + i % 2] = acc[r][t][i];
   __syncthreads();
+  bool bad = false;
   for (int i = threadIdx.x; i < cta_rows * tokens; i += blockDim.x) {
     const int row = i % cta_rows, t = i / cta_rows, n = blockIdx.x * cta_rows + row;
     if (n >= a.N) continue;
@@ -380,8 +406,17 @@ __global__ void __launch_bounds__(kQ4MaxWarps * 32, 2) q4_matvec_kernel(Q4Args a
 #pragma unroll
       for (int e = 0; e < kTerms; ++e)
         s += sum[((row / rows * a.wk + k) * rows + row % rows) * kPitch + t * kTerms + e];
+    bad |= isnan(s);
     if (a.bias) s += a.bias[n];
     static_cast<T*>(a.y)[(int64_t)(m0 + t) * a.N + n] = Pair<T>::from_float(s);
+  }
+  // the rows with a NaN for a scale, in a loop of their own: the one above is pipelined
+  if constexpr (Math::kMostZero < 255) {
+    if (!bad || a.zero == nullptr) return;
+    for (int i = threadIdx.x; i < cta_rows * tokens; i += blockDim.x) {
+      const int t = i / cta_rows, n = blockIdx.x * cta_rows + i % cta_rows;
+      if (n < a.N) q4_far_zeros<T>(a, m0 + t, n, Math::kMostZero);
+    }
   }
 }
 

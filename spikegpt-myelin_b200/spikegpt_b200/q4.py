@@ -69,6 +69,7 @@ def q4_linear(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None = 
     """``x @ W.T + bias`` for x [..., K] (CUDA, float32 / bfloat16 / float16) and the
     weight W [N, K] that ``quantize_q4`` packed with the same ``group_size``; in x's
     dtype. Made for up to 64 tokens a call (more run in turns that read the weight
-    again). A ``packed`` that is not 16-byte aligned (a view into a flat buffer) is
-    copied at every call."""
+    again). ``zeros`` may hold any byte (a row with one above 127 takes longer for
+    bfloat16 and float32 tokens). A ``packed`` that is not 16-byte aligned (a view into a
+    flat buffer) is copied at every call."""
     return (_op or _native.op("q4_linear"))(x, packed, scales, zeros, bias, group_size)
