@@ -18,14 +18,16 @@ LIB_PATH = _capi.PKG_ROOT / "lib" / "libspikegpt_torch.so"
 
 _lock = threading.Lock()
 _loaded = False
+_ops = torch.ops.spikegpt_b200
 
 
-def load() -> None:
+@torch.compiler.assume_constant_result  # a compiled caller loads it while it is traced
+def load() -> bool:
     """Load the binding (once) and bind it to the CUDA library."""
     global _loaded
     with _lock:
         if _loaded:
-            return
+            return True
         _capi.lib()  # raises with the build command if it is not built
         if not LIB_PATH.exists():
             raise RuntimeError(
@@ -33,17 +35,15 @@ def load() -> None:
                 "`python spikegpt-myelin_b200/build.py` (or __graft_entry__.build())"
             )
         torch.ops.load_library(str(LIB_PATH))
-        torch.ops.spikegpt_b200.bind_library(str(_capi.library_path()))
+        _ops.bind_library(str(_capi.library_path()))
         _loaded = True
+    return True
 
 
-def op(name: str):
-    """The operator ``spikegpt_b200::<name>``."""
-    load()
-    return getattr(torch.ops.spikegpt_b200, name).default
-
-
-def op_if_built(name: str):
-    """The operator, or None while the libraries are not built (``op`` then tells why):
-    modules look theirs up when they are imported, so that calls need no look-up."""
-    return op(name) if LIB_PATH.exists() and _capi.library_path().exists() else None
+def ops():
+    """The operators' namespace. The binding is loaded at the first call and not when the
+    package is imported: it is built against one torch, and what does not need it (the WKV
+    operators) has to work without."""
+    if not _loaded:
+        load()
+    return _ops

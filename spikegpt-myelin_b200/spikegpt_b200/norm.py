@@ -14,8 +14,6 @@ from torch import Tensor
 
 from . import _native
 
-_op = _native.op_if_built("layer_norm")
-
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:
     """Layer norm of ``x`` [..., C] (CUDA, float32 / bfloat16 / float16, C <= 16384)
@@ -24,4 +22,4 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     last index (others are copied); any row pitch is read in place. Raises
     ValueError for shapes and dtypes it does not take and NotImplementedError for
     tensors that are not on CUDA."""
-    return (_op or _native.op("layer_norm"))(x, weight, bias, eps)
+    return _native.ops().layer_norm.default(x, weight, bias, eps)

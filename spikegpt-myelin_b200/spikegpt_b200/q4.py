@@ -14,8 +14,6 @@ from torch import Tensor
 
 from . import _native
 
-_op = _native.op_if_built("q4_linear")
-
 
 def packed_pitch(in_features: int) -> int:
     """Bytes of one packed row."""
@@ -72,4 +70,4 @@ def q4_linear(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None = 
     again). ``zeros`` may hold any byte (a row with one above 127 takes longer for
     bfloat16 and float32 tokens). A ``packed`` that is not 16-byte aligned (a view into a
     flat buffer) is copied at every call."""
-    return (_op or _native.op("q4_linear"))(x, packed, scales, zeros, bias, group_size)
+    return _native.ops().q4_linear.default(x, packed, scales, zeros, bias, group_size)
