@@ -13,6 +13,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from importlib.metadata import version
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -48,9 +49,25 @@ def _newer(lib: Path, deps: list[Path]) -> bool:
     return lib.exists() and lib.stat().st_mtime >= max(p.stat().st_mtime for p in deps)
 
 
+def _torch_stamp() -> Path:
+    """The file that says which torch the binding was built against."""
+    return TORCH_LIB.with_suffix(".torch")
+
+
+def _binding_current() -> bool:
+    """Built from this source, and against the torch that would load it: the binding uses
+    torch's C++ interface, which another version may have changed."""
+    stamp = _torch_stamp()
+    return (
+        _newer(TORCH_LIB, [TORCH_SOURCE, REPO_ROOT / "include" / "spikegpt_wkv.h"])
+        and stamp.exists()
+        and stamp.read_text() == version("torch")
+    )
+
+
 def _start_binding(force: bool) -> tuple[subprocess.Popen, Path] | None:
     """The compiler of the torch binding, started (it runs beside nvcc)."""
-    if not force and _newer(TORCH_LIB, [TORCH_SOURCE, REPO_ROOT / "include" / "spikegpt_wkv.h"]):
+    if not force and _binding_current():
         return None
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
@@ -78,6 +95,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if status:
             raise subprocess.CalledProcessError(status, binding[0].args)
         binding[1].replace(TORCH_LIB)
+        _torch_stamp().write_text(version("torch"))
     return lib
 
 

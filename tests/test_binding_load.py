@@ -61,3 +61,26 @@ assert y.shape == x.shape and y.requires_grad and _native._loaded
 print("fine")
 """)
     assert done.returncode == 0 and "fine" in done.stdout, done.stdout + done.stderr
+
+
+def test_another_torch_means_another_binding(tmp_path, monkeypatch):
+    """The build takes the binding for current only if the torch it was built against is
+    the one that is installed."""
+    import importlib.util
+    import os
+
+    spec = importlib.util.spec_from_file_location("recipe", PACKAGE / "build.py")
+    recipe = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(recipe)
+    monkeypatch.setattr(recipe, "TORCH_LIB", tmp_path / "libspikegpt_torch.so")
+    assert not recipe._binding_current()
+    recipe.TORCH_LIB.write_bytes(b"")
+    os.utime(recipe.TORCH_LIB, (2**32, 2**32))
+    assert not recipe._binding_current()  # built before there was a stamp
+    recipe._torch_stamp().write_text(recipe.version("torch"))
+    assert recipe._binding_current() and recipe._start_binding(False) is None
+    os.utime(recipe.TORCH_LIB, (0, 0))  # older than its source
+    assert not recipe._binding_current()
+    os.utime(recipe.TORCH_LIB, (2**32, 2**32))
+    monkeypatch.setattr(recipe, "version", lambda name: "0.0.1")
+    assert not recipe._binding_current()
