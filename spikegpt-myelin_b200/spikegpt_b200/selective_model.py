@@ -77,6 +77,13 @@ class Q4Linear(nn.Module):
         self.register_buffer("zeros", zeros)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float())
 
+    def _apply(self, fn, recurse: bool = True):
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype != scales.dtype:  # a part of the 4-bit format, not of the model's type
+            self.scales = scales.to(self.scales.device)
+        return self
+
     def weight(self) -> Tensor:
         """The float32 weight that the packed form stands for."""
         return dequantize_q4(self.packed, self.scales, self.zeros, self.in_features, self.group_size)
