@@ -217,6 +217,10 @@ class SelectiveLM(nn.Module):
     def generate(self, ids: Tensor, count: int, lengths: Tensor | None = None) -> Tensor:
         """``count`` tokens after each prompt [B, count], the most likely ones (the first
         of equals)."""
+        if count < 0:
+            raise ValueError(f"count must not be negative; got {count}")
+        if count == 0:
+            return ids.new_empty(ids.shape[0], 0, dtype=torch.long)
         logits, states = self.prefill(ids, lengths)
         out = [logits.argmax(-1)]
         for _ in range(count - 1):

@@ -56,3 +56,16 @@ def test_a_prompt_of_no_tokens_reads_no_padding(cuda):
     # a sequence that has read nothing goes on as one that starts with its next token
     token = ids[:, 0]
     torch.testing.assert_close(model.step(token, none), model.prefill(ids[:, :1])[0], rtol=1e-4, atol=1e-5)
+
+
+def test_generate_gives_as_many_tokens_as_it_is_asked_for(monkeypatch):
+    model = SelectiveLM(CONFIG)
+    logits = torch.arange(100.0).view(2, 50)
+    monkeypatch.setattr(model, "prefill", lambda ids, lengths=None: (logits, []))
+    monkeypatch.setattr(model, "step", lambda tokens, states: logits)
+    ids = torch.zeros(2, 4, dtype=torch.int32)
+    for count in (0, 1, 2, 5):
+        out = model.generate(ids, count)
+        assert out.shape == (2, count) and out.dtype == torch.int64 and (out == 49).all()
+    with pytest.raises(ValueError):
+        model.generate(ids, -1)
