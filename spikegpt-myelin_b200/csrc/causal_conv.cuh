@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_fwd_kernel(ConvArgs 
         float u = bias[v];
 #pragma unroll
         for (int j = 0; j < W; ++j) u = fmaf(w[j][v], win[j][v], u);
-        f[v] = a.silu ? u * sigmoid1(u) : u;
+        f[v] = a.silu ? u * sigmoid1<T>(u) : u;
       }
       Vec<T, V> out;
       out.set(f);
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_bwd_kernel(ConvArgs 
           float u = bias[v];
 #pragma unroll
           for (int j = 0; j < W; ++j) u = fmaf(w[j][v], win[j][v], u);
-          const float s = sigmoid1(u);
+          const float s = sigmoid1<T>(u);
           g[v] *= s * fmaf(u, 1.f - s, 1.f);
         }
         if (t >= len) g[v] = 0.f;  // a window of infinities gives its row no gradient
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(ConvArgs
   }
   if (a.silu) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) u[v] *= sigmoid1(u[v]);
+    for (int v = 0; v < V; ++v) u[v] *= sigmoid1<T>(u[v]);
   }
   Vec<T, V> out;
   out.set(u);

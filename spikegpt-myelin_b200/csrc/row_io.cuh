@@ -80,8 +80,27 @@ struct Vec {
   }
 };
 
-// 1 / (1 + e^-v); 0 and 1 at the infinities.
-__device__ __forceinline__ float sigmoid1(float v) { return rcp(1.f + ex2(-v * kL2E)); }
+// 1 / (1 + e^-v) for results of type T; 0 and 1 at the infinities. The product v log2(e)
+// is off by up to half an ulp of itself, which the exponential turns into a relative
+// error of |v| 2^-24: nothing next to a 16-bit type's rounding. For float32 what the
+// product lost, and what its factor lacks of log2(e), go into a correction of the
+// exponential. (The clamp keeps the correction finite; the sigmoid is 0 or 1 by then. A
+// NaN leaves it finite: its callers multiply by v, or by what v has made a NaN.)
+constexpr float kL2ELow = 1.9259629911e-8f;  // log2(e) - kL2E
+template <typename T>
+__device__ __forceinline__ float sigmoid1(float v) {
+  if constexpr (sizeof(T) == 2) return rcp(1.f + ex2(-v * kL2E));
+  const float n = fminf(fmaxf(-v, -200.f), 200.f), hi = n * kL2E;
+  const float lo = fmaf(n, kL2ELow, fmaf(n, kL2E, -hi));
+  return rcp(fmaf(ex2(hi), fmaf(lo, 0.6931471806f, 1.f), 1.f));
+}
+template <typename T>
+__device__ __forceinline__ f2 sigmoid2(f2 v) {
+  if constexpr (sizeof(T) == 2) return rcpx2(add2(ex2x2(mul2(v, splat(-kL2E))), splat(1.f)));
+  const f2 n{fminf(fmaxf(-v.x, -200.f), 200.f), fminf(fmaxf(-v.y, -200.f), 200.f)}, hi = mul2(n, splat(kL2E));
+  const f2 lo = fma2(n, splat(kL2ELow), fma2(n, splat(kL2E), f2{-hi.x, -hi.y}));
+  return rcpx2(fma2(ex2x2(hi), fma2(lo, splat(0.6931471806f), splat(1.f)), splat(1.f)));
+}
 
 // Column sums of `rows` float32 rows of `blocks` groups of C columns, in row order
 // within each of kRows strides and then over the strides in order, so the result does

@@ -67,7 +67,7 @@ struct ScanArgs {
 __device__ __forceinline__ f2 softplus2(f2 v) {
   const f2 n{fmaxf(-fabsf(v.x), -100.f), fmaxf(-fabsf(v.y), -100.f)};
   const f2 hi = mul2(n, splat(kL2E));
-  const f2 lo = fma2(n, splat(1.9259629911e-8f), fma2(n, splat(kL2E), f2{-hi.x, -hi.y}));  // log2(e) - kL2E
+  const f2 lo = fma2(n, splat(kL2ELow), fma2(n, splat(kL2E), f2{-hi.x, -hi.y}));
   f2 u = ex2x2(hi);
   u = fma2(mul2(u, splat(0.6931471806f)), lo, u);
   const f2 s = mul2(u, rcpx2(add2(u, splat(2.f)))), w = mul2(s, s);
@@ -81,9 +81,6 @@ __device__ __forceinline__ f2 softplus2(f2 v) {
   return add2(f2{v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y}, p);  // a NaN stays one
 }
 __device__ __forceinline__ f2 scan_delta(f2 v, int softplus) { return softplus ? softplus2(v) : v; }
-__device__ __forceinline__ f2 sigmoid2(f2 v) {
-  return rcpx2(add2(ex2x2(mul2(v, splat(-kL2E))), splat(1.f)));
-}
 
 __device__ __forceinline__ int scan_length(const ScanArgs& a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
@@ -343,7 +340,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_summary_kernel(ScanArgs a) 
       if constexpr (kAdjoint) {
         if (a.z) {
           const f2 z = pair_of(rz[k]);
-          w = mul2(w, mul2(z, sigmoid2(z)));
+          w = mul2(w, mul2(z, sigmoid2<T>(z)));
         }
       } else {
         w = mul2(d, w);
@@ -497,7 +494,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(ScanArgs a) {
       f2 y = fma2(D, pair_of(cx[k]), f2{v.x, v.y});
       if (a.z) {
         const f2 z = pair_of(cz[k]);
-        y = mul2(y, mul2(z, sigmoid2(z)));
+        y = mul2(y, mul2(z, sigmoid2<T>(z)));
       }
       if (whole) {
         Vec<T, 2> o;
@@ -738,7 +735,7 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
       f2 gy = pair_of(Vec<T, 2>::load(cur + 2 * kCells + at));
       if (a.z) {
         const f2 z = pair_of(Vec<T, 2>::load(cur + 3 * kCells + at));
-        gy = mul2(gy, mul2(z, sigmoid2(z)));
+        gy = mul2(gy, mul2(z, sigmoid2<T>(z)));
       }
       const f2 dx = mul2(d, x);
       slot[at] = make_float4(d.x, d.x, dx.x, dx.x);
@@ -955,14 +952,14 @@ __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a
       const f2 go = pair_of(Vec<T, 2>::load(cur + 2 * kCells + at));
       f2 gy = go, gz{0.f, 0.f};
       if (a.z) {
-        const f2 z = pair_of(Vec<T, 2>::load(cur + 3 * kCells + at)), sz = sigmoid2(z);
+        const f2 z = pair_of(Vec<T, 2>::load(cur + 3 * kCells + at)), sz = sigmoid2<T>(z);
         const float2 yv = *reinterpret_cast<const float2*>(v + 2 * TS * L::kPitch);
         const f2 gs = mul2(go, sz), y = fma2(D, x, f2{yv.x, yv.y});
         gy = mul2(gs, z);
         gz = mul2(mul2(gs, y), fma2(z, sub2(splat(1.f), sz), splat(1.f)));
       }
       f2 gdt = fma2(x, along, mul2(f2{ga.x, ga.y}, splat(0.6931471806f)));
-      if (a.softplus) gdt = mul2(gdt, sigmoid2(add2(pair_of(Vec<T, 2>::load(cur + kCells + at)), bias)));
+      if (a.softplus) gdt = mul2(gdt, sigmoid2<T>(add2(pair_of(Vec<T, 2>::load(cur + kCells + at)), bias)));
       const f2 gx = fma2(d, along, mul2(D, gy));
       if (whole) {
         const uint32_t off = r * (uint32_t)a.C + cp;
@@ -1117,7 +1114,7 @@ __global__ void __launch_bounds__(kScanStepThreads) scan_step_kernel(ScanArgs a)
   reduce_scatter<LPC, LPC, 1>(y);
   if (!mine || q >= rows) return;
   float s = fmaf(D, x, y[0]);
-  if (a.z) s *= z * sigmoid1(z);
+  if (a.z) s *= z * sigmoid1<T>(z);
   static_cast<T*>(a.out)[(int64_t)own * a.C + c] = Pair<T>::from_float(s);
 }
 
