@@ -1,5 +1,5 @@
 """GPU tests that float32 tensors are worked on with float32's bits where a result does not
-hide it: gates at large arguments."""
+hide it: gates at large arguments, and sums over states of terms that cancel."""
 
 from __future__ import annotations
 
@@ -51,3 +51,26 @@ def test_gates_at_their_limits(cuda, dtype):
     leaf = x.clone().requires_grad_()
     (g,) = torch.autograd.grad(sg.causal_conv(leaf, torch.ones(8, 1, device=cuda)).sum(), leaf)
     assert (g[0, 0, :3].abs() <= 1e-30).all() and (g[0, 0, 3:6] == 1).all() and g[0, 0, 7].isnan()
+
+
+@pytest.mark.parametrize("n", [3, 8, 9, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("c", [33, 64])
+def test_sums_over_states_keep_their_terms_last_bits(cuda, n, c):
+    """Two terms that cancel but for their last bits, at many pairs of states: the gradients of
+    x and dt, and of the gate through y, are what float32 leaves of them, exactly."""
+    t, first, second = 40, 2.0 - 2.0**-23, -(2.0 - 2.0**-21)
+    C, want = torch.zeros(1, t, n, device=cuda), first + second
+    for i in range(t):
+        C[0, i, i % n], C[0, i, (i + 1 + i // n) % n] = first, second
+    pair = (C != 0).sum(-1)[0] == 2
+    assert pair.sum() >= t // 2
+    one = torch.ones(1, t, c, device=cuda)
+    A, B = torch.full((c, n), -1e30, device=cuda), torch.ones(1, t, n, device=cuda)  # no memory: every step alone
+    x, dt, z = (one.clone().requires_grad_() for _ in range(3))
+    plain = sg.selective_scan(x, dt, A, B, C, dt_softplus=False)
+    for name, v in zip(("x", "dt"), torch.autograd.grad(plain.sum(), (x, dt))):
+        assert (v[0, pair] == want).all(), (name, float(v[0, pair].min()), float(v[0, pair].max()), want)
+    (gz,) = torch.autograd.grad(sg.selective_scan(x, dt, A, B, C, None, z, dt_softplus=False).sum(), z)
+    s = torch.sigmoid(torch.ones(()).double())
+    slope = float(s * (1 + (1 - s)))
+    assert float((gz[0, pair].double() / slope - want).abs().max()) <= GATE * want
