@@ -53,3 +53,12 @@ def test_scan_backward_without_channels_has_sums_to_write():
         assert lib.selective_scan_backward(0, null, null, null, null, p, p, null, null, null, null, null, null, null,
                                            null, null, null, null, null, null, null, null, null, 0, b, t, 0, 4,
                                            *strides, 1, null) == want
+
+
+def test_layer_norm_backward_fills_the_gpu_at_every_width():
+    """The workspace holds one partial row of both sums for each CTA: at least one an SM where
+    there are rows enough, whatever the CTAs' threads."""
+    size, sms = _capi.lib().layer_norm_workspace_size, 148  # what the plan assumes without a GPU
+    for c, want in ((64, 2 * sms), (4096, 2 * sms), (8192, sms), (8193, sms), (16384, sms)):
+        assert -(-size(0, 100000, c) // (2 * c * 4)) >= want, c
+    assert size(0, 3, 16384) == 3 * 2 * 16384 * 4
