@@ -82,24 +82,21 @@ struct Vec {
 
 // 1 / (1 + e^-v) for results of type T; 0 and 1 at the infinities. The product v log2(e)
 // is off by up to half an ulp of itself, which the exponential turns into a relative
-// error of |v| 2^-24: nothing next to a 16-bit type's rounding. For float32 what the
-// product lost, and what its factor lacks of log2(e), go into a correction of the
-// exponential. (The clamp keeps the correction finite; the sigmoid is 0 or 1 by then. A
-// NaN leaves it finite: its callers multiply by v, or by what v has made a NaN.)
-constexpr float kL2ELow = 1.9259629911e-8f;  // log2(e) - kL2E
+// error of |v| 2^-24: nothing next to a 16-bit type's rounding. For float32 what is
+// missing, -v less the product times ln(2), corrects the exponential. (Where the product
+// overflows that is no number, and the maximum leaves the infinity or zero as it is.)
 template <typename T>
 __device__ __forceinline__ float sigmoid1(float v) {
-  if constexpr (sizeof(T) == 2) return rcp(1.f + ex2(-v * kL2E));
-  const float n = fminf(fmaxf(-v, -200.f), 200.f), hi = n * kL2E;
-  const float lo = fmaf(n, kL2ELow, fmaf(n, kL2E, -hi));
-  return rcp(fmaf(ex2(hi), fmaf(lo, 0.6931471806f, 1.f), 1.f));
+  const float p = -v * kL2E;
+  if constexpr (sizeof(T) == 2) return rcp(1.f + ex2(p));
+  return rcp(fmaf(ex2(p), fmaxf(1.f + fmaf(p, -0.6931471806f, -v), 0.5f), 1.f));
 }
 template <typename T>
 __device__ __forceinline__ f2 sigmoid2(f2 v) {
-  if constexpr (sizeof(T) == 2) return rcpx2(add2(ex2x2(mul2(v, splat(-kL2E))), splat(1.f)));
-  const f2 n{fminf(fmaxf(-v.x, -200.f), 200.f), fminf(fmaxf(-v.y, -200.f), 200.f)}, hi = mul2(n, splat(kL2E));
-  const f2 lo = fma2(n, splat(kL2ELow), fma2(n, splat(kL2E), f2{-hi.x, -hi.y}));
-  return rcpx2(fma2(ex2x2(hi), fma2(lo, splat(0.6931471806f), splat(1.f)), splat(1.f)));
+  const f2 p = mul2(v, splat(-kL2E));
+  if constexpr (sizeof(T) == 2) return rcpx2(add2(ex2x2(p), splat(1.f)));
+  const f2 c = add2(fma2(p, splat(-0.6931471806f), f2{-v.x, -v.y}), splat(1.f));
+  return rcpx2(fma2(ex2x2(p), f2{fmaxf(c.x, 0.5f), fmaxf(c.y, 0.5f)}, splat(1.f)));
 }
 
 // Column sums of `rows` float32 rows of `blocks` groups of C columns, in row order

@@ -67,7 +67,7 @@ struct ScanArgs {
 __device__ __forceinline__ f2 softplus2(f2 v) {
   const f2 n{fmaxf(-fabsf(v.x), -100.f), fmaxf(-fabsf(v.y), -100.f)};
   const f2 hi = mul2(n, splat(kL2E));
-  const f2 lo = fma2(n, splat(kL2ELow), fma2(n, splat(kL2E), f2{-hi.x, -hi.y}));
+  const f2 lo = fma2(n, splat(1.9259629911e-8f), fma2(n, splat(kL2E), f2{-hi.x, -hi.y}));  // log2(e) - kL2E
   f2 u = ex2x2(hi);
   u = fma2(mul2(u, splat(0.6931471806f)), lo, u);
   const f2 s = mul2(u, rcpx2(add2(u, splat(2.f)))), w = mul2(s, s);

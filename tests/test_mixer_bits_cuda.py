@@ -10,8 +10,9 @@ import spikegpt_b200 as sg
 
 pytestmark = pytest.mark.gpu
 
-# An exponential within 2^-22 of its value, a reciprocal within 2^-23, and six roundings of
-# 2^-24 around them: 7.2e-7 of the value, whatever the argument.
+# An exponential within 2^-22 of its value, a reciprocal within 2^-23, three roundings of 2^-24
+# around them, and the rounding of ln(2) times the exponent, 2e-9 * 115 at the largest
+# argument here: 7.7e-7 of the value.
 GATE = 8 * 2.0**-23
 
 
