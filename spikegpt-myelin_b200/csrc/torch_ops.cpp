@@ -166,30 +166,32 @@ Tensor empty(const Tensor& like, at::IntArrayRef shape, at::ScalarType type) {
   return at::empty(shape, like.options().dtype(type));
 }
 Tensor empty(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options()); }
-bool wants_grad(std::initializer_list<const OptTensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const OptTensor* t : ts)
-    if (has(*t) && (*t)->requires_grad()) return true;
-  return false;
+bool requires_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+bool requires_grad(const OptTensor& t) { return t.has_value() && requires_grad(*t); }
+template <class... Ts>
+bool wants_grad(const Ts&... ts) {
+  return at::GradMode::is_enabled() && (requires_grad(ts) || ...);
 }
-void no_grad_only(const char* op, std::initializer_list<const OptTensor*> ts) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad(ts), "spikegpt_b200.", op, " has no gradient; call it under torch.no_grad()");
+template <class... Ts>
+void no_grad_only(const char* op, const Ts&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad(ts...), "spikegpt_b200.", op,
+                              " has no gradient; call it under torch.no_grad()");
 }
 // Forward-mode derivatives (dual tensors, torch.func.jvp) are not there; without this a
 // tangent would be lost below autograd without a word.
-void no_tangents(const char* op, std::initializer_list<const OptTensor*> ts) {
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <class... Ts>
+void no_tangents(const char* op, const Ts&... ts) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-  for (const OptTensor* t : ts)
-    TORCH_CHECK_NOT_IMPLEMENTED(!has(*t) || !(*t)->_fw_grad(/*level=*/0).defined(), "spikegpt_b200.", op,
-                                " has no forward-mode derivative");
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(ts) || ...), "spikegpt_b200.", op, " has no forward-mode derivative");
 }
 // A call of a backward operator. While a graph of the gradients is recorded
 // (create_graph) it goes through their Autograd kernel, which gives them a node that
 // raises: there are no second derivatives.
 template <class F>
 auto backward_call(const char* op, const Tensor& g, const OptTensor& other, F&& call) {
-  const OptTensor og = g;
-  no_tangents(op, {&og, &other});
+  no_tangents(op, g, other);
   if (at::GradMode::is_enabled()) return call();
   at::AutoDispatchBelowADInplaceOrView below;
   return call();
@@ -275,13 +277,11 @@ Tensor norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, dou
   need_shape("weight", weight, {c});
   need_shape("bias", bias, {c});
   need_cuda("layer_norm", x, {&weight, &bias});
-  const OptTensor ox = x;
-  no_tangents("layer_norm", {&ox, &weight, &bias});
+  no_tangents("layer_norm", x, weight, bias);
   const OptTensor w = parameter(weight), b = parameter(bias);
   const Tensor flat = rows(x.dim() == 2 ? x : x.reshape({-1, c}));
   Tensor y;
-  const OptTensor fx = flat;
-  if (wants_grad({&fx, &w, &b})) {
+  if (wants_grad(flat, w, b)) {
     y = LayerNorm::apply(flat, w, b, eps);
   } else {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -381,13 +381,11 @@ Tensor2 conv(const Tensor& x_, const Tensor& weight, const OptTensor& bias, cons
   need_dtype("initial_state", state, x_.scalar_type(), "x");
   const OptTensor weight_ = weight;
   need_cuda("causal_conv", x_, {&weight_, &bias, &state, &lengths});
-  const OptTensor ox_ = x_;
-  no_tangents("causal_conv", {&ox_, &weight_, &bias, &state});
+  no_tangents("causal_conv", x_, weight, bias, state);
   const Tensor wt = parameter(weight), x = rows(x_);
   const OptTensor bi = parameter(bias), lens = lengths_of(lengths, b);
   const OptTensor window = has(state) ? OptTensor(state->contiguous()) : OptTensor();
-  const OptTensor ox = x, ow = wt;
-  if (!wants_grad({&ox, &ow, &bi, &window})) {
+  if (!wants_grad(x, wt, bi, window)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return conv_fwd_op().call(x, wt, bi, window, lens, silu, return_state);
   }
@@ -558,7 +556,7 @@ Tensor2 scan(const Tensor& x_, const Tensor& dt_, const Tensor& A_, const Tensor
   TORCH_CHECK_VALUE(x_.dim() == 3, "x must have shape [B, T, C]; got ", shape_of(x_));
   const int64_t b = size_of(x_, 0), t = size_of(x_, 1), c = size_of(x_, 2), n = scan_parameters(A_, D_, dt_bias_, c);
   code_of("x", x_);
-  const OptTensor od = dt_, oA = A_, oB = B_, oC = C_, ox = x_;
+  const OptTensor od = dt_, oA = A_, oB = B_, oC = C_;
   need_shape("dt", od, {b, t, c});
   need_shape("z", z_, {b, t, c});
   need_shape("B", oB, {b, t, n});
@@ -570,11 +568,11 @@ Tensor2 scan(const Tensor& x_, const Tensor& dt_, const Tensor& A_, const Tensor
   need_shape("initial_state", state, {b, c, n});
   TORCH_CHECK_VALUE(!has(state) || state->scalar_type() == at::kFloat, "initial_state must be float32");
   need_cuda("selective_scan", x_, {&od, &oA, &oB, &oC, &D_, &z_, &dt_bias_, &state, &lengths});
-  no_tangents("selective_scan", {&ox, &od, &oA, &oB, &oC, &D_, &z_, &dt_bias_, &state});
+  no_tangents("selective_scan", x_, dt_, A_, B_, C_, D_, z_, dt_bias_, state);
   const Tensor x = rows(x_), dt = rows(dt_), A = parameter(A_), B = rows(B_), C = rows(C_);
   const OptTensor D = parameter(D_), z = rows(z_), dt_bias = parameter(dt_bias_), lens = lengths_of(lengths, b);
   const OptTensor h0 = has(state) ? OptTensor(state->contiguous()) : OptTensor();
-  if (wants_grad({&ox, &od, &oA, &oB, &oC, &D, &z, &dt_bias, &h0})) {
+  if (wants_grad(x_, dt_, A_, B_, C_, D, z, dt_bias, h0)) {
     const auto r = SelectiveScan::apply(x, dt, A, B, C, D, z, dt_bias, h0, lens, softplus, return_state);
     return {r[0], r[1]};
   }
@@ -678,9 +676,8 @@ void written(const Tensor& t) {
 Tensor conv_step_autograd(const Tensor& x, const Tensor& state, const Tensor& weight, const OptTensor& bias,
                           bool silu) {
   static const auto op = typed<decltype(conv_step)>("spikegpt_b200::causal_conv_step_");
-  const OptTensor ox = x, os = state, ow = weight;
-  no_grad_only("causal_conv_step_", {&ox, &os, &ow, &bias});
-  no_tangents("causal_conv_step_", {&ox, &os, &ow, &bias});
+  no_grad_only("causal_conv_step_", x, state, weight, bias);
+  no_tangents("causal_conv_step_", x, state, weight, bias);
   Tensor y;
   {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -693,9 +690,8 @@ Tensor scan_step_autograd(const Tensor& x, const Tensor& dt, const Tensor& A, co
                           const Tensor& state, const OptTensor& D, const OptTensor& z, const OptTensor& dt_bias,
                           bool softplus) {
   static const auto op = typed<decltype(scan_step)>("spikegpt_b200::selective_scan_step_");
-  const OptTensor ox = x, od = dt, oA = A, oB = B, oC = C, os = state;
-  no_grad_only("selective_scan_step_", {&ox, &od, &oA, &oB, &oC, &os, &D, &z, &dt_bias});
-  no_tangents("selective_scan_step_", {&ox, &od, &oA, &oB, &oC, &os, &D, &z, &dt_bias});
+  no_grad_only("selective_scan_step_", x, dt, A, B, C, state, D, z, dt_bias);
+  no_tangents("selective_scan_step_", x, dt, A, B, C, state, D, z, dt_bias);
   Tensor y;
   {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -707,9 +703,8 @@ Tensor scan_step_autograd(const Tensor& x, const Tensor& dt, const Tensor& A, co
 Tensor q4_linear_autograd(const Tensor& x, const Tensor& packed, const Tensor& scales, const OptTensor& zeros,
                           const OptTensor& bias, int64_t group) {
   static const auto op = typed<decltype(q4_linear)>("spikegpt_b200::q4_linear");
-  const OptTensor ox = x, os = scales;
-  no_grad_only("q4_linear", {&ox, &os, &bias});
-  no_tangents("q4_linear", {&ox, &os, &bias});
+  no_grad_only("q4_linear", x, scales, bias);
+  no_tangents("q4_linear", x, scales, bias);
   at::AutoDispatchBelowADInplaceOrView below;
   return op.call(x, packed, scales, zeros, bias, group);
 }

@@ -18,7 +18,6 @@ LIB_PATH = _capi.PKG_ROOT / "lib" / "libspikegpt_torch.so"
 
 _lock = threading.Lock()
 _loaded = False
-_ops = torch.ops.spikegpt_b200
 
 
 @torch.compiler.assume_constant_result  # a compiled caller loads it while it is traced
@@ -35,15 +34,21 @@ def load() -> bool:
                 "`python spikegpt-myelin_b200/build.py` (or __graft_entry__.build())"
             )
         torch.ops.load_library(str(LIB_PATH))
-        _ops.bind_library(str(_capi.library_path()))
+        torch.ops.spikegpt_b200.bind_library(str(_capi.library_path()))
         _loaded = True
     return True
 
 
-def ops():
-    """The operators' namespace. The binding is loaded at the first call and not when the
-    package is imported: it is built against one torch, and what does not need it (the WKV
-    operators) has to work without."""
-    if not _loaded:
+class _Operators:
+    """The operators as attributes. The binding is loaded when the first one is looked up and
+    not when the package is imported: it is built against one torch, and what does not need
+    it (the WKV operators) has to work without."""
+
+    def __getattr__(self, name: str):  # once a name: what it finds becomes an attribute
         load()
-    return _ops
+        found = getattr(torch.ops.spikegpt_b200, name).default
+        setattr(self, name, found)
+        return found
+
+
+ops = _Operators()

@@ -12,7 +12,7 @@ from __future__ import annotations
 
 from torch import Tensor
 
-from . import _native
+from ._native import ops
 
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:
@@ -22,4 +22,4 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     last index (others are copied); any row pitch is read in place. Raises
     ValueError for shapes and dtypes it does not take and NotImplementedError for
     tensors that are not on CUDA."""
-    return _native.ops().layer_norm.default(x, weight, bias, eps)
+    return ops.layer_norm(x, weight, bias, eps)

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import _native
+from ._native import ops
 
 
 def packed_pitch(in_features: int) -> int:
@@ -70,4 +70,4 @@ def q4_linear(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None = 
     again). ``zeros`` may hold any byte (a row with one above 127 takes longer for
     bfloat16 and float32 tokens). A ``packed`` that is not 16-byte aligned (a view into a
     flat buffer) is copied at every call."""
-    return _native.ops().q4_linear.default(x, packed, scales, zeros, bias, group_size)
+    return ops.q4_linear(x, packed, scales, zeros, bias, group_size)

@@ -20,7 +20,7 @@ from __future__ import annotations
 
 from torch import Tensor
 
-from . import _native
+from ._native import ops
 
 MAX_TAPS = 4
 MAX_STATES = 64
@@ -47,7 +47,7 @@ def causal_conv(
     adds the last W - 1 rows to the result, the next call's initial state. With
     ``lengths`` [B], what lies past a sequence's length is not read, gives zeros and
     has no gradient. Differentiable in x, weight, bias and initial_state."""
-    y, state = _native.ops().causal_conv.default(x, weight, bias, initial_state, lengths, silu, return_state)
+    y, state = ops.causal_conv(x, weight, bias, initial_state, lengths, silu, return_state)
     return (y, state) if return_state else y
 
 
@@ -55,7 +55,7 @@ def causal_conv_step_(x: Tensor, state: Tensor, weight: Tensor, bias: Tensor | N
                       silu: bool = True) -> Tensor:
     """One token of ``causal_conv``: x [B, C], ``state`` [B, W-1, C] (contiguous, x's
     dtype) is moved on by x in place. No gradient."""
-    return _native.ops().causal_conv_step_.default(x, state, weight, bias, silu)
+    return ops.causal_conv_step_(x, state, weight, bias, silu)
 
 
 def selective_scan(
@@ -85,8 +85,7 @@ def selective_scan(
     what lies past a sequence's length is not read, gives zeros, and leaves the
     state as it is. Differentiable in every tensor but lengths; the backward keeps
     the state of every 8th step (float32, N / 2 bytes for each element of x)."""
-    out, state = _native.ops().selective_scan.default(x, dt, A, B, C, D, z, dt_bias, initial_state, lengths,
-                                                      dt_softplus, return_state)
+    out, state = ops.selective_scan(x, dt, A, B, C, D, z, dt_bias, initial_state, lengths, dt_softplus, return_state)
     return (out, state) if return_state else out
 
 
@@ -105,4 +104,4 @@ def selective_scan_step_(
 ) -> Tensor:
     """One token of ``selective_scan``: x, dt, z [B, C] and B, C [B, N]; ``state``
     [B, C, N] (float32, contiguous) is moved on in place. No gradient."""
-    return _native.ops().selective_scan_step_.default(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus)
+    return ops.selective_scan_step_(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus)
