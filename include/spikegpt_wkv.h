@@ -356,7 +356,8 @@ WKV_API int wkv_set_debug_pipeline(long long wait_limit_cycles, int withhold_fir
  * float32 [C] or null. window_in [B, W-1, C] holds the rows before t = 0 (null:
  * zeros), window_out receives the last W - 1 rows (null: not wanted). lengths [B]
  * (int32, null: all T): the rows past a sequence's length are not read, their y and
- * grad_x are zero, and window_out holds the last rows inside the length.
+ * grad_x are zero, and window_out holds the last rows inside the length. What a call
+ * writes does not overlap what it reads: window_out is another buffer than window_in.
  * The backward takes what the forward took and writes every gradient that is asked
  * for (grad_bias, grad_window may be null); the parameters' sums have a fixed order.
  * causal_conv_step is one token, x [B, C]: y from the window and x, and the window
@@ -385,7 +386,8 @@ WKV_API int causal_conv_step(int dtype, const void* x, const float* weight, cons
  * gradients are contiguous. A [C, N], D [C], dt_bias [C] and the states [B, C, N]
  * are float32; D, z, dt_bias, state_in, lengths and state_out may be null. A row
  * past its sequence's length is not read, leaves the state as it is and gives zeros.
- * kept (selective_scan_state_size bytes, or null): the states that the backward
+ * What a call writes does not overlap what it reads (state_out is another buffer than
+ * state_in). kept (selective_scan_state_size bytes, or null): the states that the backward
  * starts from, written by the forward. The sums over sequences and channels have a
  * fixed order. A workspace (where its size is not 0) is 16-byte aligned, or the call
  * returns WKV_ERR_INVALID_ARGUMENT. selective_scan_step is one token (x, dt, z [B, C];

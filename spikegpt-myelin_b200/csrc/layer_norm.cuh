@@ -15,7 +15,8 @@
 // that one barrier a sum is enough. The backward keeps gw and gb of its columns in
 // registers over all its rows, adds its teams' in team order and leaves one partial row
 // a CTA. Measured, launches included: 16384 x 4096 bfloat16 forward 62 us (4.3 TB/s),
-// backward 88 us (4.6 TB/s) and its column sums 11 us; 8192 x 512 float32 15, 24 and 9 us.
+// backward 88 us (4.6 TB/s) and its column sums 11 us; 8192 x 512 float32 14, 23 and 9 us;
+// 8192 x 16384 bfloat16 133, 368 and 21 us.
 // The instructions between a row's arrival and the next one's bound it (issue slots half
 // busy, memory 42 to 51 % of its nominal rate), which is why the arithmetic is packed.
 //
@@ -181,7 +182,10 @@ __host__ __device__ constexpr int norm_fwd_ctas() {
   return kThr != 256 ? 1 : sizeof(T) == 2 && !NormIo<T, V>::kStaged ? 3 : 2;
 }
 // kThr: the CTA's threads, 256, 512 (rows past 4096) or 1024 (past 8192, where 64
-// registers a thread make both kernels spill: such rows are rare).
+// registers a thread make both kernels spill, 28 to 872 bytes: such rows are rare). Below
+// that, 16-bit rows of whole words do not spill; the backward of aligned float32 rows
+// spills 56 bytes of its 128 registers' worth, that of unaligned rows up to 296, and the
+// forward of rows that move value by value 40 to 64.
 template <typename T, int V, int kThr>
 __global__ void __launch_bounds__(kThr, (norm_fwd_ctas<T, V, kThr>())) layer_norm_fwd_kernel(NormArgs a) {
   using Io = NormIo<T, V>;

@@ -833,7 +833,8 @@ int q4_matvec(int dtype, const void* x, const uint8_t* packed, const void* scale
     };
     // 32 rows a warp where that still gives two CTAs an SM, so that the inputs are read and
     // paired half as often: 16 x 768 x 50257 31 us with 16 rows, 29 with 32; 16 x 8192 x 16384
-    // 76 and 66. (Three tiles' sums and operands leave no registers for 32 rows.)
+    // 76 and 66, though with groups of 128 the kernel spills 108 bytes. (Three tiles' sums and
+    // operands leave no registers for 32 rows.)
     if (tiles == 2) {
       if (N >= 64 * sm_count()) return go(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
       return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});

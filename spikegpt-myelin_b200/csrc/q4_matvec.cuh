@@ -18,9 +18,11 @@
 // at the end.
 //
 // Measured: 6 x 8192 x 16384 bfloat16, groups of 128: 28.7 us, 2.5 TB/s of weights; 1 x 768
-// x 50257, groups of 64: 10.6 us. What bounds it is the decode: about 1.4 integer and
-// packed operations a weight, at two CTAs of eight warps an SM, take 2.5 times as long as
-// the bytes. 64 rows a warp and six stages were no faster.
+// x 50257, groups of 64: 10.3 us. What bounds it is latency: 512 CTAs of four warps, 13
+// warps an SM, issue in 51 % of their slots and keep the integer pipe 54 % busy (about 1.4
+// integer and packed operations a weight), and wait most (1.6 warps an issue) for global
+// loads, which the scales, zero points and tokens are, one stage ahead, next to the
+// weights' ring. 64 rows a warp and six stages were no faster.
 //
 // The warps of a CTA are `wk` along the inputs (every wk-th 128 of them) by the
 // others along the rows; the sums along the inputs meet in shared memory in warp order.

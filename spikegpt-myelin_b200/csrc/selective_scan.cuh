@@ -17,7 +17,8 @@
 // over channels and states, and over segments of the time axis where those are too few.
 // Measured at 16 x 1024 x 1536, 16 states, bfloat16: forward 243 us (1.7e12
 // exponentials a second, 37 % of the unit's rate; 232 us without the kept states),
-// backward 714 us, sums 15 us. 1 x 8191 x 1536: summaries 72 us, forward 113 us.
+// backward 714 us, sums 20 us; float32 242, 1045 and 21 us. 1 x 8191 x 1536: summaries
+// 72 us, forward 113 us.
 #pragma once
 
 #include "row_io.cuh"
@@ -540,8 +541,9 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], float a0, float a1, floa
 // rounding to bfloat16 does). For 16-bit tensors the upper ones are cut off, which keeps 22
 // bits of the term. For float32 tensors they are rounded: the rest is then half as large and
 // of either sign, at most the last of float32's 24 bits is lost, and the gradients' errors
-// are those of sums in float32 (of the step's 2.3e-7 -> 1.9e-7, 16 states; 16 x 1024 x 1536
-// 1030 -> 1058 us; a third value, which keeps all bits, gave the same errors in 1106 us).
+// are those of sums in float32 (of the step's 2.3e-7 -> 1.9e-7, 16 states), for 2.7 % of the
+// kernel's time at 16 x 1024 x 1536 (a third value, which keeps all bits, gave the same
+// errors for 7 %).
 // A term that is infinite or NaN makes all rows of its tile NaN: the caller then adds by
 // shuffles instead.
 template <typename T>
@@ -606,7 +608,10 @@ struct ScanBwdSmem {
 // exchanged among the lanes, added over the warps and left as one partial row of the
 // CTA's channels. Bound by issue and latency at 2.6 warps a scheduler: 26 instructions for
 // 32 state updates, of which 8 are staging and the epilogue. 255 registers a thread, longer
-// and shorter tiles and a delayed read of the tensor core's sums were no faster.
+// and shorter tiles and a delayed read of the tensor core's sums were no faster. The bounds
+// and the plan are for three CTAs an SM, which 16-bit tensors have (32 to 44 bytes spilled);
+// float32 with 9 to 16 states takes 85,504 bytes of shared memory, so two fit, and spills 124
+// bytes for a third that does not come.
 template <typename T, int LPC>
 __global__ void __launch_bounds__(kScanBwdThreads, 3) scan_bwd_kernel(ScanArgs a) {
   using L = ScanBwdSmem<T, LPC>;
