@@ -11,7 +11,9 @@ It trains (``forward``), reads prompts of several lengths in one right-padded ba
 (``prefill``) and generates token by token (``step``) from the states that prefill
 left, with ``quantize_`` turning the projections into 4-bit ones first if wanted.
 u, z are halves of one projection and dt, B, C parts of another: the operators read
-them in place. Train under ``torch.autocast("cuda", torch.bfloat16)`` or in float32.
+them in place. Train under ``torch.autocast("cuda", torch.bfloat16)`` or in float32;
+``.to(torch.bfloat16)``, for generation, rounds A_log, D and the biases with the rest,
+and the operators widen what is left of them.
 """
 
 from __future__ import annotations
